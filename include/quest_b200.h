@@ -323,6 +323,72 @@ int producer_hadamard_quantize_cuda_bf16(void* codes_ptr, int int8_operand, void
  * pointers 16-byte aligned (QB200_ERR_UNSUPPORTED otherwise). */
 int rmsnorm_cuda_bf16(void* y, const void* x, const void* weight, float eps, int group_size, int batch_size, cudaStream_t stream);
 
+/*
+ * Serving over a paged cache (no counterpart in the reference, whose attention is torch's over dense tensors).  Keys and values
+ * lie in pools of pages of page_size tokens; row b of page_table int32 [batch, width] lists the pages of request b in the order
+ * of its tokens, and the slot of a token is page * page_size + its place in the page.  The free pages are a stack: entries
+ * 0 .. *free_count - 1 of free_pages.  Lengths, tables and counts live on the device; nothing here is read by the host, so a
+ * captured graph replays a step with the lengths of the moment.
+ *
+ * page_assign_cuda: request b holds cached_lens[b] tokens and gets new_lens[b] more (negative: 0).  Requests are served in order;
+ * one whose rows, table width or pages do not suffice is refused as a whole: no pages, slots -1, positions 0, kv_lens 0.
+ *   page_table  new pages are written, taken from the end of the stack      free_left[1]  the count afterwards (not free_count itself)
+ *   cu_new      [batch + 1] first row of each request (at most rows)        kv_lens [batch]  tokens to attend over, 0: refused
+ *   lens        [batch] tokens held afterwards (cached_lens where refused)  slots int64 / positions int32 [rows], -1 / 0 behind the last
+ * page_release_cuda: request b keeps keep_lens[b] of lens[b] tokens; the pages behind them return to the stack (what does not fit
+ * into its `pool` entries is dropped).  The outputs of both must not overlap their inputs.  At most 8192 requests
+ * (QB200_ERR_UNSUPPORTED beyond), width * page_size below 2^31.
+ */
+int page_assign_cuda(int* page_table, const int* free_pages, const int* free_count, const int* cached_lens, const int* new_lens,
+                     int* cu_new, int* kv_lens, int* lens, long long* slots, int* positions, int* free_left, int batch, int width,
+                     int pool, int rows, int page_size, cudaStream_t stream);
+int page_release_cuda(const int* page_table, int* free_pages, const int* free_count, const int* lens, const int* keep_lens,
+                      int* free_left, int batch, int width, int pool, int page_size, cudaStream_t stream);
+
+/*
+ * qkv bf16 [rows, ld]: n_head query, n_kv_head key and n_kv_head value heads of head_dim per row.  q and k are rotated as
+ * rope_inplace_cuda_bf16 does (row positions[r] of table [table_len, head_dim / 2, 2]); q goes to q_out [rows, n_head, head_dim],
+ * k and v to slot slots[r] of the caches [num_pages, page_size, n_kv_head, head_dim] with strides (page, token, head) in
+ * elements.  Rows whose slot or position lies outside the cache or the table are left out entirely.  Slots must differ.
+ * head_dim, ld and strides multiples of 8, bases 16-byte aligned (QB200_ERR_UNSUPPORTED otherwise).
+ */
+int rope_paged_append_cuda_bf16(const void* qkv, long long ld, const void* table, int table_is_bf16, const int* positions,
+                                const long long* slots, void* k_cache, const long long* k_strides, void* v_cache,
+                                const long long* v_strides, void* q_out, int rows, int n_head, int n_kv_head, int head_dim,
+                                int table_len, int num_pages, int page_size, cudaStream_t stream);
+
+/*
+ * Attention of new tokens over the pages.  Rows cu_new[b] .. cu_new[b + 1] - 1 of q [rows, n_head, head_dim] are the last tokens of
+ * request b, whose kv_lens[b] tokens lie in its pages; row t of n sees the keys 0 .. kv_lens[b] - n + t:
+ *   out = softmax(scale * q . k) . v,  query head h over key and value head h / (n_head / n_kv_head).
+ * A row that sees no key gives zeros; rows outside every request stay as they were.  Keys and values behind kv_lens[b] are not
+ * looked at, whatever they hold.  Strides in elements: q, out (token, head); caches (page, token, head).
+ * head_dim 64 or 128; page_size 16, 32, 64 or a multiple of 128; n_head a multiple of n_kv_head; strides multiples of 8, bases
+ * 16-byte aligned (QB200_ERR_UNSUPPORTED otherwise).  workspace: paged_attention_workspace(...) bytes, 16-byte aligned, used by
+ * this call alone while it runs.
+ */
+int paged_attention_cuda_bf16(void* out, const long long* out_strides, const void* q, const long long* q_strides,
+                              const void* k_cache, const long long* k_strides, const void* v_cache, const long long* v_strides,
+                              const int* page_table, const int* kv_lens, const int* cu_new, void* workspace, float scale, int rows,
+                              int batch, int width, int n_head, int n_kv_head, int head_dim, int num_pages, int page_size,
+                              cudaStream_t stream);
+int paged_attention_workspace(int rows, int batch, int n_head, int n_kv_head, int head_dim);
+
+/*
+ * Drafted tokens against the target's probabilities.  Request b drafted the tokens cu_drafts[b] .. cu_drafts[b + 1] - 1 of
+ * draft_tokens [n_drafts]; its rows of target_probs [n_drafts + batch, vocab] begin at cu_drafts[b] + b and number one more, and
+ * uniforms [n_drafts + batch] are laid out alike.  Draft i is kept while u_i * draft_probs[i, x_i] < target_probs[i, x_i]
+ * (draft_probs [n_drafts, vocab], NULL: 1 on the drafted token).  The next token is drawn with the request's last uniform, by
+ * inverting the running sum of max(target - draft, 0) of the first refused row (of its target row where that is zero
+ * everywhere) or of the row behind the last draft: the first token whose running sum passes u times the total.
+ *   tokens int64 [batch, max_drafts + 1]: the kept drafts, the drawn token, -1 behind it     accepted int32 [batch]: drafts kept
+ * Drafts beyond max_drafts are not looked at.  Probabilities fp32 or bf16; negative ones and NaN count as 0, a drafted token
+ * outside the vocabulary is refused.  vocab at most 8388608 (QB200_ERR_UNSUPPORTED beyond).
+ */
+int verify_drafts_cuda(const void* target_probs, const void* draft_probs, int probs_are_bf16, const long long* draft_tokens,
+                       const int* cu_drafts, const float* uniforms, long long* tokens, int* accepted, int batch, int n_drafts,
+                       int vocab, int max_drafts, cudaStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

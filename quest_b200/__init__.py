@@ -519,3 +519,4 @@ def hadamard_transform(x: torch.Tensor, block: int = 128, weight_side: bool = Fa
 
 from .layer import (Linear4bit, fused_matmul_dequantize_int4_bf16, linear_forward, preprocess_weight,  # noqa: E402,F401
                     unpack_int4)
+from .paged import (PageStep, page_assign, page_release, paged_attention, rope_paged_append, verify_drafts)  # noqa: E402,F401

@@ -44,6 +44,12 @@ SIGNATURES = {
     "rmsnorm_cuda_bf16": [_P, _P, _P, ctypes.c_float, _I, _I, _P],
     "rope_inplace_cuda_bf16": [_P, _P, _I, _I, _I, _I, _I, _LL, _P],
     "producer_hadamard_quantize_cuda_bf16": [_P, _I, _P, _P, _I, _P, _P, _P, _P, ctypes.c_float, _I, _I, _I, _P],
+    "page_assign_cuda": [_P] * 11 + [_I] * 5 + [_P],
+    "page_release_cuda": [_P] * 6 + [_I] * 4 + [_P],
+    "rope_paged_append_cuda_bf16": [_P, _LL, _P, _I, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P],
+    "paged_attention_cuda_bf16": [_P] * 12 + [ctypes.c_float] + [_I] * 8 + [_P],
+    "paged_attention_workspace": [_I] * 5,
+    "verify_drafts_cuda": [_P, _P, _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P],
     "quest_b200_test_bounded_wait_cuda": [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _LL, _P],
     "quest_b200_device_status": [ctypes.POINTER(ctypes.c_int)],
     "quest_b200_version": [],

@@ -1,0 +1,497 @@
+// Serving over a paged cache: page tables and slots from request lengths, pages given back, rotary embedding into the pages,
+// and the check of drafted tokens.  The attention that reads the pages is in paged_attention.cu.
+#include <cooperative_groups.h>
+
+#include "common.cuh"
+
+namespace qb {
+
+namespace cg = cooperative_groups;
+
+constexpr int kPageThreads = 512;
+constexpr int kMaxRequests = 8192;  // of one step: two arrays of that length lie in shared memory (64 KB)
+
+// Inclusive sum over the block; `carry` is the sum of all earlier rounds and is advanced.  scratch: one word per warp.
+__device__ __forceinline__ long long block_inclusive_sum(long long v, long long& carry, long long* scratch) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const long long o = __shfl_up_sync(~0u, v, d);
+        if (lane >= d) v += o;
+    }
+    __syncthreads();
+    if (lane == 31) scratch[warp] = v;
+    __syncthreads();
+    long long before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < kPageThreads / 32; ++w) {
+        const long long s = scratch[w];
+        before += w < warp ? s : 0;
+        all += s;
+    }
+    v += carry + before;
+    carry += all;
+    return v;
+}
+
+__device__ __forceinline__ int saturate_int(long long v) { return (int)(v > 0x7fffffffll ? 0x7fffffffll : v); }
+
+// First index whose (non-decreasing) end lies behind i.
+__device__ __forceinline__ int find_request(const int* ends, int n, int i) {
+    int lo = 0, hi = n;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (ends[mid] > i) hi = mid; else lo = mid + 1;
+    }
+    return lo;
+}
+
+struct AssignParams {
+    int* page_table;
+    const int *free_pages, *free_count, *cached, *added;
+    int *cu, *kv_lens, *lens, *free_left;
+    long long* slots;
+    int* positions;
+    int batch, width, pool, rows, page;
+};
+
+// Page tables and slots of a step.  With c cached and n new tokens a request needs the pages ceil(c/P) .. ceil((c+n)/P) - 1;
+// they are taken from the end of the free list in the order of the requests, so that a running sum of the needs says which
+// request gets which entry and whether the list holds them.  Every block computes both running sums for itself (a few
+// microseconds at most, no second launch and no block that waits for another) and then deals with its share of the rows; the
+// first row of a page writes its entry into the table.  Latency: three dependent loads and two block sums.
+__global__ void __launch_bounds__(kPageThreads) page_assign_kernel(const AssignParams p) {
+    extern __shared__ int sm[];
+    int* ends = sm;              // rows up to and with the request
+    int* first = sm + p.batch;   // its first place below the end of the free list, -1: refused
+    __shared__ long long scratch[kPageThreads / 32];
+    const int held = min(max(*p.free_count, 0), p.pool);
+    long long row_carry = 0, page_carry = 0, used = 0;
+    for (int b0 = 0; b0 < p.batch; b0 += kPageThreads) {
+        const int b = b0 + threadIdx.x;
+        const bool there = b < p.batch;
+        const long long c = there ? max(p.cached[b], 0) : 0, n = there ? max(p.added[b], 0) : 0;
+        const long long end = block_inclusive_sum(n, row_carry, scratch);
+        const long long have = (c + p.page - 1) / p.page, want = (c + n + p.page - 1) / p.page;
+        const bool fits = end <= p.rows && want <= p.width;
+        const long long need = there && fits ? want - have : 0;
+        const long long taken = block_inclusive_sum(need, page_carry, scratch);
+        const bool granted = fits && (need == 0 || taken <= held);
+        if (there) {
+            ends[b] = saturate_int(end);
+            first[b] = granted ? (int)(taken - need) : -1;
+            if (blockIdx.x == 0) {
+                p.cu[b + 1] = (int)(end < p.rows ? end : p.rows);
+                p.kv_lens[b] = granted ? (int)(c + n) : 0;
+                p.lens[b] = (int)(granted ? c + n : c);
+            }
+        }
+        if (granted && need > 0) used = taken;
+    }
+    if (blockIdx.x == 0) {
+        __shared__ int most;
+        if (threadIdx.x == 0) most = 0;
+        __syncthreads();
+        atomicMax(&most, (int)used);
+        __syncthreads();
+        if (threadIdx.x == 0) *p.free_left = held - most, p.cu[0] = 0;
+    }
+    __syncthreads();
+    for (int i = blockIdx.x * kPageThreads + threadIdx.x; i < p.rows; i += gridDim.x * kPageThreads) {
+        const int b = find_request(ends, p.batch, i);
+        long long slot = -1;
+        int pos = 0;
+        if (b < p.batch && first[b] >= 0) {
+            const int c = max(p.cached[b], 0), start = b == 0 ? 0 : ends[b - 1];
+            pos = c + (i - start);
+            const int at = pos / p.page, have = (int)(((long long)c + p.page - 1) / p.page);
+            int* entry = p.page_table + (long long)b * p.width + at;
+            int id;
+            if (at >= have) {
+                id = p.free_pages[held - 1 - (first[b] + at - have)];
+                if (pos % p.page == 0) *entry = id;
+            } else {
+                id = *entry;
+            }
+            if (id >= 0) slot = (long long)id * p.page + pos % p.page;
+        }
+        p.slots[i] = slot;
+        p.positions[i] = pos;
+    }
+}
+
+struct ReleaseParams {
+    const int* page_table;
+    int* free_pages;
+    const int *free_count, *lens, *keep;
+    int* free_left;
+    int batch, width, pool, page;
+};
+
+// The pages behind the tokens that are kept go to the end of the free list, in the order of requests and pages: a running sum
+// of the counts gives every page its place.
+__global__ void __launch_bounds__(kPageThreads) page_release_kernel(const ReleaseParams p) {
+    extern __shared__ int sm[];
+    int* ends = sm;              // pages given back up to and with the request
+    int* stay = sm + p.batch;    // pages that it keeps
+    __shared__ long long scratch[kPageThreads / 32];
+    const int held = min(max(*p.free_count, 0), p.pool);
+    long long carry = 0;
+    for (int b0 = 0; b0 < p.batch; b0 += kPageThreads) {
+        const int b = b0 + threadIdx.x;
+        const bool there = b < p.batch;
+        const long long n = there ? max(p.lens[b], 0) : 0;
+        const long long k = there ? min((long long)max(p.keep[b], 0), n) : 0;
+        const long long have = min((n + p.page - 1) / p.page, (long long)p.width), left = min((k + p.page - 1) / p.page, (long long)p.width);
+        const long long end = block_inclusive_sum(have - left, carry, scratch);
+        if (there) ends[b] = saturate_int(end), stay[b] = (int)left;
+    }
+    __syncthreads();
+    const int total = (int)min(carry, (long long)(p.pool - held));
+    if (blockIdx.x == 0 && threadIdx.x == 0) *p.free_left = held + total;
+    for (int i = blockIdx.x * kPageThreads + threadIdx.x; i < total; i += gridDim.x * kPageThreads) {
+        const int b = find_request(ends, p.batch, i);
+        const int start = b == 0 ? 0 : ends[b - 1];
+        p.free_pages[held + i] = p.page_table[(long long)b * p.width + stay[b] + (i - start)];
+    }
+}
+
+struct AppendParams {
+    const __nv_bfloat16* qkv;
+    long long ld;
+    const void* table;
+    const int* positions;
+    const long long* slots;
+    __nv_bfloat16 *k, *v, *q_out;
+    long long k_page, k_token, k_head, v_page, v_token, v_head;  // strides in elements
+    long long capacity;                                          // slots of the cache
+    int rows, hq, hkv, head_dim, table_len, page;
+};
+
+// One block per row: q and k are rotated (interleaved pairs, fp32 products and sums rounded one by one as torch rounds them,
+// then to bf16 once), k and v go to the row's slot.  A row without a slot or a position outside the table leaves everything as
+// it was.  Bound by HBM: every element is read and written once, in 16-byte pieces.
+template <typename T>
+__global__ void __launch_bounds__(256) rope_paged_append_kernel(const AppendParams p) {
+    const int row = blockIdx.x;
+    const long long slot = p.slots[row];
+    const int pos = p.positions[row];
+    if (slot < 0 || slot >= p.capacity || pos < 0 || pos >= p.table_len) return;
+    const long long page = slot / p.page, token = slot - page * p.page;
+    const int head_chunks = p.head_dim / 8, chunks = (p.hq + 2 * p.hkv) * head_chunks;
+    const uint4* src = reinterpret_cast<const uint4*>(p.qkv + row * p.ld);
+    for (int i = threadIdx.x; i < chunks; i += 256) {
+        const uint4 x = ld_stream16(src + i);
+        const int head = i / head_chunks, c = (i - head * head_chunks) * 8;
+        __nv_bfloat16* dst;
+        uint32_t w[4] = {x.x, x.y, x.z, x.w};
+        if (head < p.hq + p.hkv) {
+            const T* t = static_cast<const T*>(p.table) + (long long)pos * p.head_dim + c;
+            float cs[8];
+            if (sizeof(T) == 4) {
+                const float4 a = __ldg(reinterpret_cast<const float4*>(t)), b = __ldg(reinterpret_cast<const float4*>(t) + 1);
+                cs[0] = a.x; cs[1] = a.y; cs[2] = a.z; cs[3] = a.w; cs[4] = b.x; cs[5] = b.y; cs[6] = b.z; cs[7] = b.w;
+            } else {
+                const uint4 a = __ldg(reinterpret_cast<const uint4*>(t));
+                const uint32_t u[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) cs[2 * j] = bf16lo_to_f32(u[j]), cs[2 * j + 1] = bf16hi_to_f32(u[j]);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float x0 = bf16lo_to_f32(w[j]), x1 = bf16hi_to_f32(w[j]), c0 = cs[2 * j], s0 = cs[2 * j + 1];
+                w[j] = pack_bf16x2(__fsub_rn(__fmul_rn(x0, c0), __fmul_rn(x1, s0)), __fadd_rn(__fmul_rn(x0, s0), __fmul_rn(x1, c0)));
+            }
+            dst = head < p.hq ? p.q_out + ((long long)row * p.hq + head) * p.head_dim
+                              : p.k + page * p.k_page + token * p.k_token + (head - p.hq) * p.k_head;
+        } else {
+            dst = p.v + page * p.v_page + token * p.v_token + (head - p.hq - p.hkv) * p.v_head;
+        }
+        *reinterpret_cast<uint4*>(dst + c) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+
+struct VerifyParams {
+    const void *target, *draft;
+    const long long* tokens;
+    const int* cu;
+    const float* u;
+    long long* out;
+    int* accepted;
+    int batch, n_tokens, vocab, most;
+};
+
+constexpr int kVerifyThreads = 256, kVerifyCluster = 8, kSegment = 256;
+constexpr int kMaxSegments = 4096;  // of one block: a vocabulary of up to 8 Mi entries
+
+__device__ __forceinline__ double as_double(float v) { return v; }
+__device__ __forceinline__ double as_double(__nv_bfloat16 v) { return __bfloat162float(v); }
+// A weight: what is not positive (a NaN among it) counts as nothing.
+__device__ __forceinline__ double weight_of(double p, double q) { const double w = p - q; return w > 0 ? w : 0; }
+
+// Eight neighbouring entries of a row of probabilities, zeros behind its end.
+template <typename T, bool VEC>
+__device__ __forceinline__ void load8(double (&x)[8], const T* row, int at, int vocab) {
+    if (VEC && at + 8 <= vocab) {
+        if (sizeof(T) == 4) {
+            const uint4 a = __ldg(reinterpret_cast<const uint4*>(row + at)), b = __ldg(reinterpret_cast<const uint4*>(row + at) + 1);
+            const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = __uint_as_float(w[j]);
+        } else {
+            const uint4 a = __ldg(reinterpret_cast<const uint4*>(row + at));
+            const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[2 * j] = bf16lo_to_f32(w[j]), x[2 * j + 1] = bf16hi_to_f32(w[j]);
+        }
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = at + j < vocab ? as_double(row[at + j]) : 0;
+}
+
+// Rejection sampling against a draft, one cluster of eight blocks per request.  Draft i is kept while u_i q_i(x_i) < p_i(x_i);
+// the next token is drawn from max(p - q, 0) of the first refused row, or from the row behind the last draft, by inverting the
+// running sum at u times the total.  Every block takes an eighth of the vocabulary and sums segments of 256 entries in 64 bits
+// (sums decide which token it is: in 32 bits the border between two tokens would depend on the order); the totals go round the
+// cluster, and the block that holds the border reads that one segment again.  So a row is read once; without clusters a
+// request would have a single SM's bandwidth (V 131072, two fp32 rows: 1 MB) or a second launch.
+template <typename T, bool VEC>
+__global__ void __cluster_dims__(kVerifyCluster, 1, 1) __launch_bounds__(kVerifyThreads) verify_drafts_kernel(const VerifyParams p) {
+    extern __shared__ double seg_sum[];
+    __shared__ int s_refused;
+    __shared__ double s_total;
+    __shared__ int s_last;  // last entry of this block with a weight, -1: none
+    cg::cluster_group cluster = cg::this_cluster();
+    const int b = blockIdx.x / kVerifyCluster, rank = blockIdx.x % kVerifyCluster;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int c0 = min(max(p.cu[b], 0), p.n_tokens), c1 = min(max(p.cu[b + 1], c0), p.n_tokens);
+    const int drafts = min(c1 - c0, p.most);
+    const T* target = static_cast<const T*>(p.target) + (long long)(c0 + b) * p.vocab;
+    const T* draft = static_cast<const T*>(p.draft) + (p.draft == nullptr ? 0 : (long long)c0 * p.vocab);
+    if (threadIdx.x == 0) s_refused = drafts;
+    __syncthreads();
+    for (int i = threadIdx.x; i < drafts; i += kVerifyThreads) {
+        const long long x = p.tokens[c0 + i];
+        bool good = false;
+        if (x >= 0 && x < p.vocab) {
+            const double q = p.draft == nullptr ? 1.0 : as_double(draft[(long long)i * p.vocab + x]);
+            good = (double)p.u[c0 + b + i] * q < as_double(target[(long long)i * p.vocab + x]);
+        }
+        if (!good) atomicMin(&s_refused, i);
+    }
+    __syncthreads();
+    const int kept = s_refused;
+    const bool refused = kept < drafts;
+    const T* prow = target + (long long)kept * p.vocab;
+    const T* qrow = draft + (long long)kept * p.vocab;
+    const long long hot = refused && p.draft == nullptr ? p.tokens[c0 + kept] : -1;  // a draft without probabilities: all on its token
+
+    const int segments = (p.vocab + kSegment - 1) / kSegment;
+    const int share = (segments + kVerifyCluster - 1) / kVerifyCluster;
+    const int seg0 = min(rank * share, segments), seg1 = min(seg0 + share, segments);
+    bool residual = refused;
+    double total = 0, before = 0;
+    int last = -1;
+    auto weights = [&](double (&w)[8], int at) {
+        load8<T, VEC>(w, prow, at, p.vocab);
+        if (residual && p.draft != nullptr) {
+            double q[8];
+            load8<T, VEC>(q, qrow, at, p.vocab);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) w[j] = weight_of(w[j], q[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) w[j] = residual && at + j == hot ? 0 : weight_of(w[j], 0);
+        }
+    };
+    while (true) {
+        if (threadIdx.x == 0) s_total = 0, s_last = -1;
+        __syncthreads();
+        for (int s = seg0 + warp; s < seg1; s += kVerifyThreads / 32) {
+            double w[8];
+            const int at = s * kSegment + lane * 8;
+            weights(w, at);
+            double sum = 0;
+            int mine = -1;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                sum += w[j];
+                if (w[j] > 0) mine = at + j;
+            }
+#pragma unroll
+            for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
+            mine = __reduce_max_sync(~0u, mine);
+            if (lane == 0) {
+                seg_sum[s - seg0] = sum;
+                if (mine >= 0) atomicMax(&s_last, mine);
+            }
+        }
+        __syncthreads();
+        if (warp == 0) {  // running sums of the segments
+            double carry = 0;
+            for (int s = 0; s < seg1 - seg0; s += 32) {
+                double v = s + lane < seg1 - seg0 ? seg_sum[s + lane] : 0;
+#pragma unroll
+                for (int d = 1; d < 32; d <<= 1) {
+                    const double o = __shfl_up_sync(~0u, v, d);
+                    if (lane >= d) v += o;
+                }
+                v += carry;
+                if (s + lane < seg1 - seg0) seg_sum[s + lane] = v;
+                carry = __shfl_sync(~0u, v, min(31, seg1 - seg0 - s - 1));  // the very value of the last segment
+            }
+            if (lane == 0) s_total = carry;
+        }
+        cluster.sync();
+        total = before = 0;
+        last = -1;
+        for (int r = 0; r < kVerifyCluster; ++r) {
+            const double t = *cluster.map_shared_rank(&s_total, r);
+            if (r == rank) before = total;
+            total += t;
+            last = max(last, *cluster.map_shared_rank(&s_last, r));
+        }
+        cluster.sync();  // nobody leaves or starts over while another block reads
+        if (total > 0 || !residual) break;
+        residual = false;  // a refused draft whose distribution covers the target's: the target's own row
+    }
+
+    const double aim = fmax((double)p.u[c1 + b] * total, 0.0);
+    if (rank == 0) {
+        for (int i = threadIdx.x; i <= p.most; i += kVerifyThreads)
+            if (i != kept) p.out[(long long)b * (p.most + 1) + i] = i < kept ? p.tokens[c0 + i] : -1;
+        if (threadIdx.x == 0) p.accepted[b] = kept;
+    }
+    if (warp != 0) return;
+    long long* slot = p.out + (long long)b * (p.most + 1) + kept;
+    const bool beyond = !(aim < total);  // u that rounds to one, or no weight at all
+    if (beyond) {
+        if (rank == 0 && lane == 0) *slot = last < 0 ? 0 : last;
+        return;
+    }
+    const int mine = seg1 - seg0;
+    if (mine == 0 || !(before <= aim && aim < before + seg_sum[mine - 1])) return;
+    int lo = 0, hi = mine - 1;  // first segment whose running sum passes the aim
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (before + seg_sum[mid] > aim) hi = mid; else lo = mid + 1;
+    }
+    int hit = 0x7fffffff, fall = -1;
+    for (;; ++lo) {
+        const double base = before + (lo == 0 ? 0 : seg_sum[lo - 1]);
+        double w[8];
+        const int at = (seg0 + lo) * kSegment + lane * 8;
+        weights(w, at);
+        double sum = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum += w[j];
+        double run = sum;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const double o = __shfl_up_sync(~0u, run, d);
+            if (lane >= d) run += o;
+        }
+        run += base - sum;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            run += w[j];
+            if (w[j] > 0) {
+                if (run > aim) hit = min(hit, at + j);
+                fall = at + j;
+            }
+        }
+        hit = __reduce_min_sync(~0u, hit);
+        fall = __reduce_max_sync(~0u, fall);
+        if (fall >= 0 || lo + 1 >= mine) break;  // the sums' rounding can point at a segment without weights: the next one
+    }
+    if (lane == 0) *slot = hit != 0x7fffffff ? hit : fall >= 0 ? fall : last;  // ... or behind a segment's last weight: that one
+}
+
+}  // namespace qb
+
+using namespace qb;
+
+// More than 48 KB of dynamic shared memory has to be asked for, once per device.
+template <typename Kernel>
+static int allow_smem(Kernel kernel, size_t bytes) {
+    return bytes <= 48 * 1024 ? QB200_OK : cuda_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+}
+
+extern "C" int page_assign_cuda(int* page_table, const int* free_pages, const int* free_count, const int* cached_lens,
+                                const int* new_lens, int* cu_new, int* kv_lens, int* lens, long long* slots, int* positions,
+                                int* free_left, int batch, int width, int pool, int rows, int page_size, cudaStream_t stream) {
+    if (batch < 0 || width < 0 || pool < 0 || rows < 0 || page_size <= 0) return QB200_ERR_INVALID_ARGUMENT;
+    if (batch > kMaxRequests || (long long)width * page_size > 0x7fffffffll) return QB200_ERR_UNSUPPORTED;
+    if (!free_count || !cu_new || !free_left || (batch && (!cached_lens || !new_lens || !kv_lens || !lens)) || (rows && (!slots || !positions)) ||
+        (batch && width && !page_table) || (pool && !free_pages))
+        return QB200_ERR_INVALID_ARGUMENT;
+    AssignParams p{page_table, free_pages, free_count, cached_lens, new_lens, cu_new, kv_lens, lens, free_left, slots, positions,
+                   batch, width, pool, rows, page_size};
+    const size_t smem = 8u * batch;
+    const int st = allow_smem(page_assign_kernel, smem);
+    if (st != QB200_OK) return st;
+    const int blocks = (rows + kPageThreads - 1) / kPageThreads;
+    page_assign_kernel<<<blocks < 1 ? 1 : blocks > 148 ? 148 : blocks, kPageThreads, smem, stream>>>(p);
+    return launch_status();
+}
+
+extern "C" int page_release_cuda(const int* page_table, int* free_pages, const int* free_count, const int* lens,
+                                 const int* keep_lens, int* free_left, int batch, int width, int pool, int page_size,
+                                 cudaStream_t stream) {
+    if (batch < 0 || width < 0 || pool < 0 || page_size <= 0) return QB200_ERR_INVALID_ARGUMENT;
+    if (batch > kMaxRequests) return QB200_ERR_UNSUPPORTED;
+    if (!free_count || !free_left || (batch && (!lens || !keep_lens)) || (batch && width && !page_table) || (pool && !free_pages))
+        return QB200_ERR_INVALID_ARGUMENT;
+    ReleaseParams p{page_table, free_pages, free_count, lens, keep_lens, free_left, batch, width, pool, page_size};
+    const size_t smem = 8u * batch;
+    const int st = allow_smem(page_release_kernel, smem);
+    if (st != QB200_OK) return st;
+    const int blocks = pool / (8 * kPageThreads);  // a block has eight pages per thread where the whole pool comes back
+    page_release_kernel<<<blocks < 1 ? 1 : blocks > 148 ? 148 : blocks, kPageThreads, smem, stream>>>(p);
+    return launch_status();
+}
+
+extern "C" int rope_paged_append_cuda_bf16(const void* qkv, long long ld, const void* table, int table_is_bf16,
+                                           const int* positions, const long long* slots, void* k_cache, const long long* k_strides,
+                                           void* v_cache, const long long* v_strides, void* q_out, int rows, int n_head,
+                                           int n_kv_head, int head_dim, int table_len, int num_pages, int page_size,
+                                           cudaStream_t stream) {
+    if (rows < 0 || n_head < 0 || n_kv_head < 0 || head_dim <= 0 || table_len < 0 || num_pages < 0 || page_size <= 0 ||
+        ld < (long long)(n_head + 2ll * n_kv_head) * head_dim)
+        return QB200_ERR_INVALID_ARGUMENT;
+    if (rows == 0 || n_head + n_kv_head == 0 || num_pages == 0 || table_len == 0) return QB200_OK;
+    if (!qkv || !table || !positions || !slots || (n_head && !q_out) || !k_strides || !v_strides || (n_kv_head && (!k_cache || !v_cache)))
+        return QB200_ERR_INVALID_ARGUMENT;
+    if (head_dim % 8 != 0 || ld % 8 != 0 || !aligned16(qkv) || !aligned16(table) || !aligned16(q_out) || !aligned16(k_cache) || !aligned16(v_cache))
+        return QB200_ERR_UNSUPPORTED;
+    for (int i = 0; i < 3; ++i)
+        if (k_strides[i] % 8 != 0 || v_strides[i] % 8 != 0) return QB200_ERR_UNSUPPORTED;
+    AppendParams p{static_cast<const __nv_bfloat16*>(qkv), ld, table, positions, slots, static_cast<__nv_bfloat16*>(k_cache),
+                   static_cast<__nv_bfloat16*>(v_cache), static_cast<__nv_bfloat16*>(q_out), k_strides[0], k_strides[1], k_strides[2],
+                   v_strides[0], v_strides[1], v_strides[2], (long long)num_pages * page_size, rows, n_head, n_kv_head, head_dim,
+                   table_len, page_size};
+    if (table_is_bf16) rope_paged_append_kernel<__nv_bfloat16><<<rows, 256, 0, stream>>>(p);
+    else rope_paged_append_kernel<float><<<rows, 256, 0, stream>>>(p);
+    return launch_status();
+}
+
+template <typename T, bool VEC>
+static int launch_verify(const VerifyParams& p, cudaStream_t stream) {
+    const int segments = (p.vocab + kSegment - 1) / kSegment, share = (segments + kVerifyCluster - 1) / kVerifyCluster;
+    verify_drafts_kernel<T, VEC><<<(unsigned)p.batch * kVerifyCluster, kVerifyThreads, sizeof(double) * share, stream>>>(p);
+    return launch_status();
+}
+
+extern "C" int verify_drafts_cuda(const void* target_probs, const void* draft_probs, int probs_are_bf16, const long long* draft_tokens,
+                                  const int* cu_drafts, const float* uniforms, long long* tokens, int* accepted, int batch,
+                                  int n_drafts, int vocab, int max_drafts, cudaStream_t stream) {
+    if (batch < 0 || n_drafts < 0 || vocab <= 0 || max_drafts < 0) return QB200_ERR_INVALID_ARGUMENT;
+    if (batch == 0) return QB200_OK;
+    if (!target_probs || !cu_drafts || !uniforms || !tokens || !accepted || (n_drafts && !draft_tokens)) return QB200_ERR_INVALID_ARGUMENT;
+    if (vocab > kMaxSegments * kVerifyCluster * kSegment || batch > (1 << 27)) return QB200_ERR_UNSUPPORTED;
+    VerifyParams p{target_probs, draft_probs, draft_tokens, cu_drafts, uniforms, tokens, accepted, batch, n_drafts, vocab, max_drafts};
+    const bool vec = vocab % 8 == 0 && aligned16(target_probs) && aligned16(draft_probs);
+    if (probs_are_bf16) return vec ? launch_verify<__nv_bfloat16, true>(p, stream) : launch_verify<__nv_bfloat16, false>(p, stream);
+    return vec ? launch_verify<float, true>(p, stream) : launch_verify<float, false>(p, stream);
+}
