@@ -363,7 +363,7 @@ int rope_paged_append_cuda_bf16(const void* qkv, long long ld, const void* table
  *   out = softmax(scale * q . k) . v,  query head h over key and value head h / (n_head / n_kv_head).
  * A row that sees no key gives zeros; rows outside every request stay as they were.  Keys and values behind kv_lens[b] are not
  * looked at, whatever they hold.  Strides in elements: q, out (token, head); caches (page, token, head).
- * head_dim 64 or 128; page_size 16, 32, 64 or a multiple of 128; n_head a multiple of n_kv_head; strides multiples of 8, bases
+ * head_dim 64 or 128; page_size a power of two from 16 to 1024; n_head a multiple of n_kv_head; strides multiples of 8, bases
  * 16-byte aligned (QB200_ERR_UNSUPPORTED otherwise).  workspace: paged_attention_workspace(...) bytes, 16-byte aligned, used by
  * this call alone while it runs.
  */

@@ -81,6 +81,8 @@ extern thread_local int qb_tl_quantiser_kernel;
 
 // Reads and clears the device status word of the row-kernel translation unit (see tcgen05.cuh).
 int hq_tc_fetch_and_clear_device_status(int* out);
+// The same of the attention kernel's translation unit.
+int paged_attention_fetch_and_clear_device_status(int* out);
 
 // The activation side of a layer on the int8-operand route: scale, quantise (behind the block transform; block 0: none) and
 // write the GEMM's operand.  Any K that is a multiple of 128.

@@ -1967,8 +1967,11 @@ extern "C" int quest_b200_device_status(int* status) {
     if (st != QB200_OK) return st;
     st = hq_tc_fetch_and_clear_device_status(&v2);  // the tensor-core quantiser keeps its own status word
     if (st != QB200_OK) return st;
+    int v3 = 0;
+    st = paged_attention_fetch_and_clear_device_status(&v3);  // and so does the attention over pages
+    if (st != QB200_OK) return st;
     if (v != 0) reset_split_counters();  // a GEMM that gave up may have left split-K tile counters half way
-    *status = v != 0 ? v : v2;
+    *status = v != 0 ? v : v2 != 0 ? v2 : v3;
     return QB200_OK;
 }
 

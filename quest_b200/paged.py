@@ -151,7 +151,7 @@ def paged_attention(
     ``kv_lens[b]`` tokens (the new ones among them) lie in the pages ``page_table[b]``: one row while decoding, a chunk of a
     prompt, drafted tokens, or a mixture over the batch.  Query head h reads key and value head h / (n_head / n_kv_head).  Rows
     that see no key (kv_lens 0: refused by ``page_assign``) give zeros; rows outside every request are not written.  What the
-    pages hold behind a request's tokens does not matter.  head_dim 64 or 128, page_size 16, 32, 64 or a multiple of 128;
+    pages hold behind a request's tokens does not matter.  head_dim 64 or 128, page_size a power of two from 16 to 1024;
     q and out may be views (strides in multiples of 8 elements)."""
     _check_caches(k_cache, v_cache)
     num_pages, page_size, n_kv_head, head_dim = k_cache.shape
