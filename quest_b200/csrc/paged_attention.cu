@@ -1,21 +1,24 @@
 // Attention of new tokens over a paged cache: out = softmax(scale q k^T) v, causal, for any mixture of single tokens, drafted
 // tokens and chunks of prompts in one launch (and a second, small one that joins what was split).
 //
-// The rows of a request and a key/value head are its new tokens times the query heads that share the head; a tile has 256 of
-// them (two streams of 128), a step 128 keys:
+// The rows of a request and a key/value head are its new tokens times the query heads that share the head; a stream works on 128 of
+// them, a step has 128 keys:
 //   S = Q K^T   tcgen05.mma kind::f16, M128 N128, Q and K in shared memory (128-byte swizzle), S in tensor memory
 //   P = exp2(c S - c m), running maximum m and sum l per row in fp32: thread = row, four warps per stream
 //   O += P V    tcgen05.mma with P (bf16, over its S) in tensor memory, V [keys][columns] in shared memory as it lies in the page
 // While one stream's warps work on its scores the tensor core works for the other stream.  P is rounded to bf16 (2^-9 of itself,
 // the weight of one key among many) because the second product takes 16-bit operands; O, m and l stay in fp32.  O is rescaled only
 // when a row's maximum has grown by more than 2^8: until then P and l simply exceed one.
-// Where a tile has at most 128 rows (decoding) both streams share its queries and take every second step; their sums meet in
-// shared memory at the end.
+// A tile has whole tokens: 128 / group of them per stream.  The two streams of a block work in one of two ways.  As a pair they share
+// the keys and values of one tile of 256 rows, and while one stream's warps work on its scores the tensor core works for the
+// other.  Alone (tiles of at most 128 rows: decoding, the ends of chunks) each stream has tiles of its own, with half of the
+// shared memory, an issuing warp and a copying warp of its own: such work is bound by HBM, and what an item costs besides its
+// steps (its queries, its result) disappears behind the other stream.
 //
-// Work is cut by steps, not by rows: all steps of all (request, head, tile) items form one line, every block takes an equal
-// piece of it, whatever the lengths are; each block computes the line from the lengths on the device.  An item that crosses
-// from one block to the next leaves partial (O, m, l) in the workspace, and the second kernel joins the pieces in order, so
-// results do not depend on timing.
+// Work is cut by steps, not by tiles: the steps of all pair items form one line, those of all single items another; every block
+// takes an equal piece of the first, then each of its streams an equal piece of the second, whatever the lengths are.  Each block
+// computes its places in the lines from the lengths on the device.  An item that crosses from one piece to the next leaves partial
+// (O, m, l) in the workspace, and a second kernel joins them in order, so results do not depend on timing.
 #include <math_constants.h>
 
 #include "tcgen05.cuh"
@@ -23,55 +26,56 @@
 namespace qb {
 namespace pa {
 
-constexpr int BM = 128, BN = 128, TILE_ROWS = 2 * BM;
+constexpr int BM = 128, BN = 128, HN = BN / 2;  // rows of a stream, keys of a step, keys of a slot
 constexpr int kThreads = 384;
-constexpr int kTmaWarp = 0, kMmaWarp = 1, kItemWarp = 2, kFirstSoftmax = 4;
-constexpr int ITEMS = 4;            // descriptors in flight between the item warp and the other roles
-constexpr int kItemReaders = 10;    // copy warp, MMA warp, eight softmax warps
+constexpr int kCopyWarp0 = 0, kMmaWarp0 = 1, kMmaWarp1 = 2, kCopyWarp1 = 3, kFirstSoftmax = 4;
+constexpr int ITEMS = 4;                            // descriptors in flight on each list
 constexpr int kControlRegs = 72, kSoftmaxRegs = 216;  // 128 x 72 + 256 x 216 = 384 x 168, what the block is launched with
 static_assert(128 * kControlRegs + 256 * kSoftmaxRegs <= kThreads * 168, "register shares exceed the launch");
+constexpr int kItemCost = 1;                        // steps that an item's queries and result are worth in the lines
 
 template <int D>
 struct Cfg {
     static constexpr int Q_BYTES = BM * D * 2;
-    static constexpr int STAGE_BYTES = BN * D * 2;
-    static constexpr int STAGES = D == 128 ? 5 : 10;
+    static constexpr int SLOT_BYTES = HN * D * 2;         // the ring of a single stream has slots of 64 keys
+    static constexpr int STAGE_BYTES = 2 * SLOT_BYTES;    // that of a pair stages of 128
+    static constexpr int STAGES = D == 128 ? 5 : 10;      // stages of the pair's ring = slots of each stream's
     static constexpr int HALVES = D / 64;
-    static constexpr int HALF_BYTES = BM * 128;
-    static constexpr int NUM_BARS = 2 * STAGES + 8 + 2 * ITEMS + 9;
-    static constexpr int SMEM = 1024 + 2 * Q_BYTES + STAGES * STAGE_BYTES + NUM_BARS * 8 + ITEMS * 64 + 2 * BM * 4 + 16;
-    static_assert(SMEM + 256 <= 232448, "shared memory of an SM");
-    // f32 accumulate, bf16 x bf16; S: both K-major, N = 128; O: the second operand lies with its columns together (MN-major)
+    // barriers: pair ring, slots; queries, scores, probabilities, outputs (of the pair's streams, of single ones); three lists; ends
+    static constexpr int PAIR_FULL = 0, PAIR_EMPTY = PAIR_FULL + STAGES, SLOT_FULL = PAIR_EMPTY + STAGES, SLOT_EMPTY = SLOT_FULL + 2 * STAGES,
+                         Q_FULL = SLOT_EMPTY + 2 * STAGES, Q_EMPTY = Q_FULL + 4, S_FULL = Q_EMPTY + 4, P_FULL = S_FULL + 4, O_FULL = P_FULL + 4,
+                         LIST_FULL = O_FULL + 4, LIST_EMPTY = LIST_FULL + 3 * ITEMS, PAIRS_DONE = LIST_EMPTY + 3 * ITEMS, DONE = PAIRS_DONE + 1,
+                         NUM_BARS = DONE + 2;
+    static constexpr int SMEM = 1024 + 2 * Q_BYTES + STAGES * STAGE_BYTES + NUM_BARS * 8 + 16 + 3 * ITEMS * 64;
+    static_assert(SMEM + 512 <= 232448, "shared memory of an SM");
+    // f32 accumulate, bf16 x bf16; S: both K-major; O: the second operand lies with its columns together (MN-major)
     static constexpr uint32_t IDESC = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BM >> 4) << 24);
-    static constexpr uint32_t IDESC_S = IDESC | ((uint32_t)(BN >> 3) << 17);
+    static constexpr uint32_t IDESC_S = IDESC | ((uint32_t)(BN >> 3) << 17), IDESC_S_SLOT = IDESC | ((uint32_t)(HN >> 3) << 17);
     static constexpr uint32_t IDESC_O = IDESC | (1u << 16) | ((uint32_t)(D >> 3) << 17);
     static constexpr uint32_t S_COL = 0, O_COL = 256;  // per stream: S (and P over it) 128 columns, O D columns
 };
 
 struct Params {
     __nv_bfloat16* out;
-    const __nv_bfloat16* q;
     const int *page_table, *kv_lens, *cu;
-    float* partial;   // per block two slots of slot_rows x (D + 2) floats
-    int* headers;     // per block: the item that begins there and goes on in the next block
-    long long o_token, o_head, q_token, q_head;
-    float c;          // |scale| log2(e)
-    uint32_t flip;    // sign bits of a negative scale, applied to q
-    int rows, batch, width, hkv, group, num_pages, page, page_shift, slot_rows, min_steps;
+    float* partial;   // 8 slots per block of slot_rows x (D + 2) floats: for each worker a piece that began before it, one that goes on
+    int* headers;     // 4 per block: for each worker the item that begins there and goes on
+    long long o_token, o_head;
+    float c;          // scale log2(e)
+    int rows, batch, width, hkv, group, tokens /* of a stream's tile */, num_pages, page, page_shift, slot_rows, wide_stores;
 };
 
-// One item, or the piece of it that a block works on.
+// One item, or the piece of it that a worker (the pair, or a single stream) has.
 struct Item {
     int start, n, kv, b, hk;  // rows start .. start + n of the batch, kv keys
-    int r0, rows;             // packed rows (token * group + head) r0 .. r0 + rows
+    int tok0;                 // first token (the second stream of a pair: p.tokens further)
     int t0, steps[2];         // first step, steps of each stream
-    int single;               // one stream's worth of rows: both streams share them and alternate
-    int slot;                 // -1: the whole item; else the slot of the partial result
+    int slot;                 // -1: the whole item; else the place of the partial result (second stream: 2 gridDim.x further)
     int last;                 // nothing behind this descriptor (it carries no work)
 };
 static_assert(sizeof(Item) <= 64, "descriptor");
 
-constexpr int HEADER = 8;  // ints: pieces (0: none), start, hk, r0, rows
+constexpr int HEADER = 8;  // ints: pieces (0: none), start, hk, tok0, rows
 
 struct Request {
     int start, n, kv;
@@ -80,10 +84,12 @@ __device__ __forceinline__ Request request_of(const Params& p, int b) {
     const int lo = min(max(p.cu[b], 0), p.rows), hi = min(max(p.cu[b + 1], lo), p.rows);
     return {lo, hi - lo, min(max(p.kv_lens[b], 0), p.width * p.page)};
 }
-// Keys that packed row r of a request sees.
-__device__ __forceinline__ int keys_of(const Request& q, int r, int group) { return min(max(q.kv - q.n + r / group + 1, 0), q.kv); }
-// Steps of a row range that ends with row r; a range that sees nothing still takes one, which gives its zeros.
+// Keys that a token of a request sees, and the steps of a tile that ends with it; a tile that sees nothing still takes one
+// step, which gives its zeros.
+__device__ __forceinline__ int keys_of(const Request& q, int token) { return min(max(q.kv - q.n + token + 1, 0), q.kv); }
 __device__ __forceinline__ int steps_of(int keys) { return max((keys + BN - 1) / BN, 1); }
+__device__ __forceinline__ int pair_tiles(const Request& q, int tokens) { return (q.n + tokens - 1) / (2 * tokens); }
+__device__ __forceinline__ bool has_single(const Request& q, int tokens) { return q.n > 0 && (q.n - 1) % (2 * tokens) < tokens; }
 
 // sum over i < n of floor((a i + b) / m), a, b >= 0 (the Euclidean descent on a and m)
 __device__ __forceinline__ long long floor_sum(long long n, long long m, long long a, long long b) {
@@ -99,21 +105,27 @@ __device__ __forceinline__ long long floor_sum(long long n, long long m, long lo
     }
     return sum;
 }
-// Steps of the first `tiles` tiles of a request and one head.  A full tile i ends with token floor((256 i + 255) / group), so
-// it takes max(floor((256 i + 255 + (kv - n) group) / (128 group)), 0) + 1 steps; the last one ends with the last token.
-__device__ __forceinline__ long long steps_before(const Request& q, int tiles, int group) {
-    const int all = (int)(((long long)q.n * group + TILE_ROWS - 1) / TILE_ROWS);
-    long long sum = 0;
-    if (tiles == all && tiles > 0) sum += steps_of(q.kv), --tiles;
+// Places that the first `tiles` pair tiles of a request and one head take in the line: their steps and kItemCost each.  A full
+// tile i of w = 2 tokens ends with token (i + 1) w - 1, so it takes max(floor(((i + 1) w - 1 + kv - n) / 128), 0) + 1 steps;
+// one that is not full ends with the last token.
+__device__ __forceinline__ long long pairs_before(const Request& q, int tiles, int tokens) {
+    long long sum = (long long)tiles * kItemCost;
+    if ((long long)tiles * 2 * tokens > q.n) sum += steps_of(q.kv), --tiles;
     if (tiles > 0) {
-        const long long e = 255 + (long long)(q.kv - q.n) * group;
-        const long long first = e >= 0 ? 0 : (-e + 255) / 256;
+        const int w = 2 * tokens, e = w - 1 + q.kv - q.n;
+        const int first = e >= 0 ? 0 : (-e + w - 1) / w;
         sum += tiles;
-        if (tiles > first) sum += floor_sum(tiles - first, 128ll * group, 256, e + 256 * first);
+        if (tiles > first) sum += floor_sum(tiles - first, BN, w, e + w * first);
     }
     return sum;
 }
-__device__ __forceinline__ int tiles_of(const Request& q, int group) { return (int)(((long long)q.n * group + TILE_ROWS - 1) / TILE_ROWS); }
+__device__ __forceinline__ long long pair_places(const Params& p, const Request& q) {
+    const int tiles = pair_tiles(q, p.tokens);
+    return tiles == 0 ? 0 : pairs_before(q, tiles, p.tokens) * p.hkv;
+}
+__device__ __forceinline__ long long single_places(const Params& p, const Request& q) {
+    return has_single(q, p.tokens) ? (long long)(steps_of(q.kv) + kItemCost) * p.hkv : 0;
+}
 
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -157,6 +169,12 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
         ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar)
         : "memory");
 }
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+        ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
+        : "memory");
+}
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
@@ -168,8 +186,6 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
           "r"(r[31]), "r"(taddr)
         : "memory");
 }
-__device__ __forceinline__ void named_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
-
 // mbar_wait of tcgen05.cuh without a call: behind one the compiler keeps to the registers of the launch.
 __device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, int where) {
     if (mbar_try_wait(bar, parity)) return true;
@@ -188,6 +204,20 @@ __device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, int wher
 // Weight of a partial result with maximum m (in log2 units) when the common maximum is `top`.
 __device__ __forceinline__ float weight_to(float m, float top) { return m == -CUDART_INF_F ? 0.f : ex2(m - top); }
 
+// 32 columns of a row, in 32-byte stores where its alignment allows: a thread has a row of its own, so a store instruction
+// touches 32 lines either way.
+__device__ __forceinline__ void store_row32(__nv_bfloat16* dst, const uint32_t (&w)[16], int wide) {
+    if (wide) {
+#pragma unroll
+        for (int i = 0; i < 16; i += 8)
+            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst + 2 * i), "r"(w[i]), "r"(w[i + 1]), "r"(w[i + 2]),
+                         "r"(w[i + 3]), "r"(w[i + 4]), "r"(w[i + 5]), "r"(w[i + 6]), "r"(w[i + 7]) : "memory");
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) *reinterpret_cast<uint4*>(dst + 2 * i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+    }
+}
+
 // What the softmax warps of a stream keep of an item: the reference maximum and the sum of the thread's row.
 struct RowState {
     float m, l;  // m in units of the scores; -inf: nothing seen
@@ -195,7 +225,7 @@ struct RowState {
 
 // One step of a row: scores in tensor memory -> probabilities over them.  `seen` keys of this step are visible to the row.
 template <int D>
-__device__ __forceinline__ void softmax_step(RowState& st, const uint32_t s_addr, const uint32_t o_addr, const int seen, const bool first, const float c) {
+__device__ __forceinline__ void softmax_step(RowState& st, const uint32_t s_addr, const uint32_t o_addr, const int seen, const bool live, const bool first, const float c) {
     uint32_t s[4][32];
 #pragma unroll
     for (int i = 0; i < 4; ++i) tmem_ld32(s_addr + 32 * i, s[i]);
@@ -217,7 +247,7 @@ __device__ __forceinline__ void softmax_step(RowState& st, const uint32_t s_addr
     }
     top = fmaxf(top, st.m);
     // 2^8 of growth is harmless in fp32 sums and bf16 probabilities alike
-    const bool grown = top * c > st.m * c + 8.f || (st.m == -CUDART_INF_F && top != -CUDART_INF_F);
+    const bool grown = live && (top * c > st.m * c + 8.f || (st.m == -CUDART_INF_F && top != -CUDART_INF_F));
     if (__any_sync(~0u, grown)) {
         const float a = st.m == -CUDART_INF_F ? 0.f : ex2((st.m - top) * c);
         st.m = top;
@@ -258,522 +288,561 @@ __device__ __forceinline__ void softmax_step(RowState& st, const uint32_t s_addr
     tmem_st_wait();
 }
 
+// A worker's place in a line: from u to end, beginning in request b `rest` places behind the request's first.
+struct Place {
+    long long u, end, rest, share;
+    int b;
+};
+
 template <int D>
-__global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Params p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
+__global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Params p, const __grid_constant__ CUtensorMap qmap,
+                                                                      const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
     using C = Cfg<D>;
     extern __shared__ uint8_t raw[];
     const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
     uint8_t* const gen = raw + (base - smem_u32(raw));
     const uint32_t q_smem = base, ring = base + 2 * C::Q_BYTES, bars = ring + C::STAGES * C::STAGE_BYTES;
-    const uint32_t kv_full = bars, kv_empty = kv_full + 8 * C::STAGES, q_full = kv_empty + 8 * C::STAGES, s_full = q_full + 16, p_full = s_full + 16,
-                   o_full = p_full + 16, item_full = o_full + 16, item_empty = item_full + 8 * ITEMS, merge_full = item_empty + 8 * ITEMS, merge_empty = merge_full + 32,
-                   done = merge_empty + 32;
-    Item* const items = reinterpret_cast<Item*>(gen + (bars + 8 * C::NUM_BARS - base));
-    float* const merge_m = reinterpret_cast<float*>(items) + ITEMS * 16;
-    float* const merge_l = merge_m + BM;
-    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(merge_l + BM);
-    __shared__ long long scan[kThreads / 32];
-    __shared__ long long found_before;  // steps of all requests before the one in which this block's piece begins
-    __shared__ int found;
+    auto bar = [&](int i) { return bars + 8u * (uint32_t)i; };
+    Item* const items = reinterpret_cast<Item*>(gen + (bars - base) + 8 * C::NUM_BARS);  // three lists: pairs, stream 0, stream 1
+    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(items + 3 * ITEMS);
+    __shared__ long long scan[2][kThreads / 32];
+    __shared__ Place places[3];  // of this block's pair, of its streams
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (warp == kMmaWarp) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, blocks = gridDim.x;
+    if (warp == kMmaWarp0) {
         tmem_alloc(smem_u32(tmem_slot), 512);
         tmem_relinquish();
-    } else if (warp == kTmaWarp && lane == 0) {
-        tma_prefetch_desc(&kmap), tma_prefetch_desc(&vmap);
-        for (int i = 0; i < C::STAGES; ++i) mbar_init(kv_full + 8 * i, 1), mbar_init(kv_empty + 8 * i, 1);
-        for (int i = 0; i < 2; ++i) mbar_init(q_full + 8 * i, 4), mbar_init(s_full + 8 * i, 1), mbar_init(p_full + 8 * i, 4), mbar_init(o_full + 8 * i, 1);
-        for (int i = 0; i < ITEMS; ++i) mbar_init(item_full + 8 * i, 1), mbar_init(item_empty + 8 * i, kItemReaders);
-        for (int i = 0; i < 4; ++i) mbar_init(merge_full + 8 * i, 1), mbar_init(merge_empty + 8 * i, 1);
-        mbar_init(done, 1);
+    } else if (warp == kCopyWarp0 && lane == 0) {
+        tma_prefetch_desc(&qmap), tma_prefetch_desc(&kmap), tma_prefetch_desc(&vmap);
+        for (int i = 0; i < C::NUM_BARS; ++i) {
+            int count = 1;
+            if (i >= C::P_FULL && i < C::P_FULL + 4) count = 4;                   // four warps of a stream
+            if (i >= C::LIST_EMPTY && i < C::LIST_EMPTY + ITEMS) count = 10;      // MMA warp, copier of the queries, eight softmax warps
+            if (i >= C::LIST_EMPTY + ITEMS && i < C::LIST_EMPTY + 3 * ITEMS) count = 5;  // MMA warp, four softmax warps
+            mbar_init(bar(i), count);
+        }
         fence_barrier_init();
     }
+    if (threadIdx.x < 3) places[threadIdx.x].b = -1;
+    if (threadIdx.x >= 32 && threadIdx.x < 36) p.headers[((threadIdx.x - 32) * blocks + blockIdx.x) * HEADER] = 0;
     let_dependents_launch();  // the joining kernel, which waits for this one's end
 
-    // ---- the line of steps: all requests' sums, and the request in which this block's piece begins
-    long long total = 0, u0 = 0, u1 = 0, share = 0;
-    if (threadIdx.x == 0) found = -1;
-    for (int pass = 0; pass < 2; ++pass) {  // the total first, then the place
-        long long carry = 0;
+    // ---- the lines: all requests' sums, and the requests in which this block's pieces begin
+    long long total[2] = {0, 0}, share[2] = {0, 0};
+    for (int pass = 0; pass < 2; ++pass) {  // the totals first, then the places
+        long long carry[2] = {0, 0};
         for (int b0 = 0; b0 < p.batch; b0 += kThreads) {
             const int b = b0 + threadIdx.x;
-            long long mine = 0;
+            long long mine[2] = {0, 0};
             if (b < p.batch) {
                 const Request q = request_of(p, b);
-                mine = steps_before(q, tiles_of(q, p.group), p.group) * p.hkv;
+                mine[0] = pair_places(p, q), mine[1] = single_places(p, q);
             }
-            long long run = mine;
+            long long run[2] = {mine[0], mine[1]};
 #pragma unroll
             for (int d = 1; d < 32; d <<= 1) {
-                const long long o = __shfl_up_sync(~0u, run, d);
-                if (lane >= d) run += o;
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const long long o = __shfl_up_sync(~0u, run[k], d);
+                    if (lane >= d) run[k] += o;
+                }
             }
             __syncthreads();
-            if (lane == 31) scan[warp] = run;
+            if (lane == 31) scan[0][warp] = run[0], scan[1][warp] = run[1];
             __syncthreads();
-            long long all = 0;
-            for (int w = 0; w < kThreads / 32; ++w) {
-                if (w < warp) run += scan[w];
-                all += scan[w];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                long long all = 0;
+                for (int w = 0; w < kThreads / 32; ++w) {
+                    if (w < warp) run[k] += scan[k][w];
+                    all += scan[k][w];
+                }
+                run[k] += carry[k];
+                carry[k] += all;
             }
-            run += carry;
-            carry += all;
-            if (pass == 1 && u0 >= run - mine && u0 < run) found = b, found_before = run - mine;
+            if (pass == 1) {
+#pragma unroll
+                for (int w = 0; w < 3; ++w) {
+                    const int k = w > 0;
+                    const long long u = share[k] * (w == 2 ? blocks + (int)blockIdx.x : (int)blockIdx.x), before = run[k] - mine[k];
+                    if (u >= before && u < run[k]) places[w] = Place{u, min(u + share[k], total[k]), u - before, share[k], b};
+                }
+            }
         }
         if (pass == 0) {
-            total = carry;
-            share = (total + gridDim.x - 1) / gridDim.x;
-            if (share < p.min_steps) share = p.min_steps;
-            u0 = share * blockIdx.x, u1 = u0 + share < total ? u0 + share : total;
+            total[0] = carry[0], total[1] = carry[1];
+            share[0] = max((total[0] + blocks - 1) / blocks, 1ll), share[1] = max((total[1] + 2 * blocks - 1) / (2 * blocks), 1ll);
         }
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    int* const header = p.headers + blockIdx.x * HEADER;
-    if (found < 0) {  // no step for this block (and none behind it)
-        if (threadIdx.x == 0) header[0] = 0;
-        __syncthreads();
-        if (warp == kMmaWarp) tmem_dealloc(tmem, 512);
-        return;
-    }
+    const bool has_pairs = places[0].b >= 0;
+    const bool none = !has_pairs && places[1].b < 0 && places[2].b < 0;
 
     bool ok = true;  // false: a wait has given up; every role leaves its loop, no role waits for another without a limit
 
+    // Takes the next descriptor of a list; false: the list has ended (or a wait has given up).
+    auto take = [&](int list, uint32_t& it, Item& d) {
+        const uint32_t at = it % ITEMS, ph = (it / ITEMS) & 1u;
+        ++it;
+        ok = __all_sync(~0u, ok && wait_bar(bar(C::LIST_FULL + list * ITEMS + at), ph, 70 + list));
+        d = items[list * ITEMS + at];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(C::LIST_EMPTY + list * ITEMS + at));
+        return ok && !d.last;
+    };
+
     // The register limits stand at the head of the roles: where they cannot be told apart the compiler takes the lower one.
-    if (warp >= kFirstSoftmax) {
+    if (none) {
+    } else if (warp >= kFirstSoftmax) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
         // ------------------------------ softmax, results ------------------------------
         const int s = (warp - kFirstSoftmax) >> 2, quad = warp & 3, row = quad * 32 + lane;  // this thread's row of its stream
         const uint32_t lanes = (uint32_t)(quad * 32) << 16;
         const uint32_t s_addr = tmem + C::S_COL + 128 * s + lanes, o_addr = tmem + C::O_COL + D * s + lanes;
-        uint32_t s_uses = 0, o_uses = 0, merges = 0;
-        for (uint32_t it = 0;; ++it) {
-            const uint32_t st = it % ITEMS;
-            ok = __all_sync(~0u, ok && wait_bar(item_full + 8 * st, (it / ITEMS) & 1u, 78));
-            const Item d = items[st];
-            __syncwarp();
-            if (lane == 0) mbar_arrive(item_empty + 8 * st);
-            if (!ok || d.last) break;
-            const int steps = d.steps[s];
-            const int r = d.r0 + (d.single ? 0 : s * BM) + row;  // packed row of the request
-            const bool live = r < d.r0 + d.rows;
-            const int token = r / p.group, head = d.hk * p.group + (r - token * p.group);
-            const int keys = live ? min(max(d.kv - d.n + token + 1, 0), d.kv) : d.kv;  // rows that are not there need no mask
-            const bool warp_live = d.r0 + (d.single ? 0 : s * BM) + quad * 32 < d.r0 + d.rows;
-
-            if (steps > 0 && !(d.single && s == 1)) {  // queries -> shared memory, two (four) rows per warp instruction
-                const long long off = (long long)(d.start + token) * p.q_token + (long long)head * p.q_head;
-                constexpr int LANES = D / 8, PER = 32 / LANES;
-                if (warp_live) {
-#pragma unroll 8
-                    for (int i = 0; i < 32 / PER; ++i) {
-                        const int from = i * PER + lane / LANES, piece = lane % LANES;
-                        const long long o = __shfl_sync(~0u, off, from);
-                        const bool there = __shfl_sync(~0u, live, from);
-                        uint4 x = make_uint4(0, 0, 0, 0);
-                        if (there) x = *reinterpret_cast<const uint4*>(p.q + o + piece * 8);
-                        x.x ^= p.flip, x.y ^= p.flip, x.z ^= p.flip, x.w ^= p.flip;
-                        const int rr = quad * 32 + from;
-                        sts128(q_smem + s * C::Q_BYTES + (piece / 8) * C::HALF_BYTES + rr * 128 + (((piece % 8) ^ (rr & 7)) << 4), x);
-                    }
+        const int tile_rows = p.tokens * p.group, row_token = row / p.group, row_head = row - row_token * p.group;
+        for (int turn = has_pairs ? 0 : 1; turn < 2; ++turn) {  // the pairs, then the items of this stream alone
+            const int list = turn == 0 ? 0 : 1 + s;
+            if (!ok || places[list].b < 0) break;
+            const uint32_t s_full = bar(C::S_FULL + 2 * turn + s), p_full = bar(C::P_FULL + 2 * turn + s), o_full = bar(C::O_FULL + 2 * turn + s);
+            uint32_t s_ph = 0, o_ph = 0;
+            Item d;
+            for (uint32_t it = 0; take(list, it, d);) {
+                const int steps = d.steps[s], tok0 = d.tok0 + (list == 0 ? s * p.tokens : 0), token = tok0 + row_token;
+                const bool live = row < tile_rows && token < d.n;
+                const bool warp_live = __any_sync(~0u, live);
+                const int keys = live ? min(max(d.kv - d.n + token + 1, 0), d.kv) : 0x7fffffff;  // a row that is not there needs no mask
+                RowState rs{-CUDART_INF_F, 0.f};
+                for (int i = 0; i < steps; ++i) {
+                    ok = __all_sync(~0u, ok && wait_bar(s_full, s_ph, 79));
+                    if (!ok) break;
+                    s_ph ^= 1u;
+                    tc_fence_after();
+                    if (warp_live) softmax_step<D>(rs, s_addr, o_addr, keys - (d.t0 + i) * BN, live, i == 0, p.c);
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(p_full);
                 }
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(q_full + 8 * s);
-            }
-
-            RowState rs{-CUDART_INF_F, 0.f};
-            for (int i = 0; i < steps; ++i) {
-                const int step = d.t0 + (d.single ? 2 * i + s : i);
-                ok = __all_sync(~0u, ok && wait_bar(s_full + 8 * s, s_uses & 1u, 79));
-                if (!ok) break;
-                ++s_uses;
-                tc_fence_after();
-                if (warp_live) softmax_step<D>(rs, s_addr, o_addr, keys - step * BN, i == 0, p.c);
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(p_full + 8 * s);
-            }
-            if (steps > 0) {
-                ok = __all_sync(~0u, ok && wait_bar(o_full + 8 * s, o_uses & 1u, 80));
-                ++o_uses;
-                tc_fence_after();
-            }
-            if (!ok) break;
-            float m = rs.m == -CUDART_INF_F ? -CUDART_INF_F : rs.m * p.c, l = rs.l;
-
-            // Piece j of 16 bytes of this thread's row in the shared memory of a stream's queries (whose products are done): the
-            // bytes of a row stay a row's, so a warp that goes on to the next item's queries disturbs no other.
-            auto row_piece = [&](int tile, int rr, int j) {
-                return q_smem + tile * C::Q_BYTES + (j / 8) * C::HALF_BYTES + rr * 128 + (((j % 8) ^ (rr & 7)) << 4);
-            };
-            if (d.single && d.steps[1] > 0 && warp_live) {
-                // The streams' sums of the same rows: the second stream's come over half by half, through the second tile's place.
-                if (s == 1) {
-                    merge_m[row] = m, merge_l[row] = l;
-#pragma unroll 1
-                    for (int half = 0; half < 2; ++half) {
-#pragma unroll 1
-                        for (int c0 = 0; c0 < D / 2; c0 += 32) {
-                            uint32_t o[32];
-                            tmem_ld32(o_addr + half * (D / 2) + c0, o);
-                            tmem_ld_wait32(o);
-#pragma unroll
-                            for (int j = 0; j < 8; ++j) sts128(row_piece(1, row, c0 / 4 + j), make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]));
-                        }
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(merge_full + 8 * quad);
-                        ok = __all_sync(~0u, ok && wait_bar(merge_empty + 8 * quad, merges & 1u, 81));
-                        ++merges;
-                    }
-                } else {
-                    float wa = 0.f, wb = 0.f;
-#pragma unroll 1
-                    for (int half = 0; half < 2; ++half) {
-                        ok = __all_sync(~0u, ok && wait_bar(merge_full + 8 * quad, merges & 1u, 82));
-                        ++merges;
-                        if (half == 0) {
-                            const float m1 = merge_m[row], top = fmaxf(m, m1);
-                            wa = weight_to(m, top), wb = weight_to(m1, top);
-                            l = l * wa + merge_l[row] * wb;
-                            m = top;
-                        }
-#pragma unroll 1
-                        for (int c0 = 0; c0 < D / 2; c0 += 32) {
-                            uint32_t o[32];
-                            tmem_ld32(o_addr + half * (D / 2) + c0, o);
-                            tmem_ld_wait32(o);
-#pragma unroll
-                            for (int j = 0; j < 8; ++j) {
-                                const uint4 x = lds128(row_piece(1, row, c0 / 4 + j));
-                                o[4 * j] = __float_as_uint(__uint_as_float(o[4 * j]) * wa + __uint_as_float(x.x) * wb);
-                                o[4 * j + 1] = __float_as_uint(__uint_as_float(o[4 * j + 1]) * wa + __uint_as_float(x.y) * wb);
-                                o[4 * j + 2] = __float_as_uint(__uint_as_float(o[4 * j + 2]) * wa + __uint_as_float(x.z) * wb);
-                                o[4 * j + 3] = __float_as_uint(__uint_as_float(o[4 * j + 3]) * wa + __uint_as_float(x.w) * wb);
-                            }
-                            tmem_st32(o_addr + half * (D / 2) + c0, o);
-                        }
-                        tmem_st_wait();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(merge_empty + 8 * quad);
-                    }
+                if (steps > 0) {
+                    ok = __all_sync(~0u, ok && wait_bar(o_full, o_ph, 80));
+                    o_ph ^= 1u;
+                    tc_fence_after();
                 }
                 if (!ok) break;
-            }
-            if (d.single && s == 1) continue;
-
-            const bool none = steps == 0;  // the upper stream's rows see nothing of this piece
-            if (d.slot < 0) {
-                // The row's columns, divided by the sum, go through the shared memory of the stream's queries so that whole lines are stored.
-                if (warp_live) {
+                if (!warp_live) continue;
+                const float l = rs.l;
+                if (d.slot < 0) {
                     const float inv = 1.f / l;
                     const bool empty = l == 0.f;  // no key in sight: zeros
+                    __nv_bfloat16* const dst = p.out + (long long)(d.start + token) * p.o_token + (long long)(d.hk * p.group + row_head) * p.o_head;
+#pragma unroll 1
+                    for (int c0 = 0; c0 < D; c0 += 32) {
+                        uint32_t o[32], w[16];
+                        tmem_ld32(o_addr + c0, o);
+                        tmem_ld_wait32(o);
+#pragma unroll
+                        for (int j = 0; j < 16; ++j)
+                            w[j] = empty ? 0u : pack_bf16x2(__uint_as_float(o[2 * j]) * inv, __uint_as_float(o[2 * j + 1]) * inv);
+                        if (live) store_row32(dst + c0, w, p.wide_stores);
+                    }
+                } else {
+                    const bool nothing = steps == 0;  // the first stream's rows see nothing of this piece
+                    float* const slot = p.partial + (long long)(d.slot + (list == 0 ? 2 * blocks * s : 0)) * p.slot_rows * (D + 2);
+                    const bool mine = row < p.slot_rows;
+                    if (mine) {
+                        slot[p.slot_rows * D + row] = rs.m == -CUDART_INF_F ? -CUDART_INF_F : rs.m * p.c;
+                        slot[p.slot_rows * (D + 1) + row] = l;
+                    }
 #pragma unroll 1
                     for (int c0 = 0; c0 < D; c0 += 32) {
                         uint32_t o[32];
                         tmem_ld32(o_addr + c0, o);
                         tmem_ld_wait32(o);
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            uint32_t w[4];
-#pragma unroll
-                            for (int k = 0; k < 4; ++k)
-                                w[k] = pack_bf16x2(__uint_as_float(o[8 * j + 2 * k]) * inv, __uint_as_float(o[8 * j + 2 * k + 1]) * inv);
-                            sts128(row_piece(s, row, c0 / 8 + j), empty ? make_uint4(0, 0, 0, 0) : make_uint4(w[0], w[1], w[2], w[3]));
+                        for (int j = 0; j < 8; ++j) {
+                            uint4 x = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+                            if (nothing) x = make_uint4(0, 0, 0, 0);
+                            if (mine) reinterpret_cast<uint4*>(slot)[(c0 / 4 + j) * p.slot_rows + row] = x;
                         }
                     }
-                    __syncwarp();
-                    const long long off = (long long)(d.start + token) * p.o_token + (long long)head * p.o_head;
-                    constexpr int LANES = D / 8, PER = 32 / LANES;
-#pragma unroll 4
-                    for (int i = 0; i < 32 / PER; ++i) {
-                        const int from = i * PER + lane / LANES, piece = lane % LANES;
-                        const long long o = __shfl_sync(~0u, off, from);
-                        const bool there = __shfl_sync(~0u, live, from);
-                        const int rr = quad * 32 + from;
-                        const uint4 x = lds128(row_piece(s, rr, piece));
-                        if (there) *reinterpret_cast<uint4*>(p.out + o + piece * 8) = x;
-                    }
-                    __syncwarp();
                 }
-            } else if (warp_live) {
-                float* const slot = p.partial + (long long)d.slot * p.slot_rows * (D + 2);
-                const int at = (d.single ? 0 : s * BM) + row;
-                if (at < p.slot_rows) {
-                    slot[p.slot_rows * D + at] = none ? -CUDART_INF_F : m;
-                    slot[p.slot_rows * (D + 1) + at] = none ? 0.f : l;
-                }
-#pragma unroll 1
-                for (int c0 = 0; c0 < D; c0 += 32) {
-                    uint32_t o[32];
-                    tmem_ld32(o_addr + c0, o);
-                    tmem_ld_wait32(o);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        float4 x = *reinterpret_cast<float4*>(&o[4 * j]);
-                        if (none) x = make_float4(0, 0, 0, 0);
-                        if (at < p.slot_rows) reinterpret_cast<float4*>(slot)[(c0 / 4 + j) * p.slot_rows + at] = x;
-                    }
-                }
+                tc_fence_before();
             }
-            tc_fence_before();
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kControlRegs));
-        if (warp == kItemWarp) {
-            // ------------------------------ items ------------------------------
-            if (lane == 0) {
-                int b = found;
+        if (warp == kCopyWarp0 || warp == kCopyWarp1) {
+            // ------------------------------ items; pages and queries -> shared memory ------------------------------
+            const int s = warp == kCopyWarp1;
+            const int box_rows = min(p.page, HN), boxes = BN / box_rows;
+            // Lane l copies box l / HALVES of a step, columns 64 (l % HALVES).
+            const int box = lane / C::HALVES, half = lane % C::HALVES;
+            auto publish = [&](int list, uint32_t& it, const Item& d) {
+                const uint32_t at = it % ITEMS, ph = (it / ITEMS) & 1u;
+                ++it;
+                ok = __all_sync(~0u, ok && wait_bar(bar(C::LIST_EMPTY + list * ITEMS + at), ph ^ 1u, 73));
+                if (lane == 0) {
+                    items[list * ITEMS + at] = d;
+                    mbar_arrive(bar(C::LIST_FULL + list * ITEMS + at));
+                }
+                __syncwarp();
+            };
+            auto load_queries = [&](int tile, int set, uint32_t& ph, int token, int hk) {
+                const uint32_t full = bar(C::Q_FULL + 2 * set + tile);
+                ok = __all_sync(~0u, ok && wait_bar(bar(C::Q_EMPTY + 2 * set + tile), ph ^ 1u, 74));
+                ph ^= 1u;
+                if (ok && lane == 0) {
+                    mbar_arrive_expect_tx(full, p.tokens * p.group * D * 2);
+                    for (int h = 0; h < C::HALVES; ++h)
+                        tma_load_3d(q_smem + tile * C::Q_BYTES + h * (BM * 128), &qmap, 64 * h, hk * p.group, token, full);
+                }
+                __syncwarp();
+            };
+            // The page of this lane's box; where that holds no key of the request one behind the pool: zeros without a read.
+            auto page_at = [&](const Item& d, int step) {
+                const int at = (step * BN + box * box_rows) >> p.page_shift, held = (d.kv + p.page - 1) >> p.page_shift;
+                int id = p.num_pages;
+                if (box < boxes && at < held) id = p.page_table[(long long)d.b * p.width + at];
+                return (unsigned)id < (unsigned)p.num_pages ? id : p.num_pages;
+            };
+            auto copy_box = [&](const CUtensorMap* map, uint32_t dst, int step, int hk, int id, uint32_t full) {
+                tma_load_4d(dst, map, half * 64, (step * BN + box * box_rows) & (p.page - 1), hk, id, full);
+            };
+            if (has_pairs && s == 0) {
+                uint32_t it = 0, stage = 0, ph = 0;
+                auto load = [&](const CUtensorMap* map, const Item& d, int step, int id) {
+                    ok = __all_sync(~0u, ok && wait_bar(bar(C::PAIR_EMPTY + stage), ph ^ 1u, 75));
+                    if (!ok) return;
+                    const uint32_t full = bar(C::PAIR_FULL + stage);
+                    if (lane == 0) mbar_arrive_expect_tx(full, C::STAGE_BYTES);
+                    __syncwarp();
+                    if (box < boxes) copy_box(map, ring + stage * C::STAGE_BYTES + half * (BN * 128) + box * box_rows * 128, step, d.hk, id, full);
+                    if (++stage == C::STAGES) stage = 0, ph ^= 1u;
+                };
+                const Place w = places[0];
+                int b = w.b;
                 Request q = request_of(p, b);
-                int tiles = tiles_of(q, p.group);
-                const long long per_head = steps_before(q, tiles, p.group);
-                long long rest = u0 - found_before;
+                int tiles = pair_tiles(q, p.tokens);
+                long long rest = w.rest;
+                const long long per_head = pairs_before(q, tiles, p.tokens);
                 int hk = (int)(rest / per_head);
                 rest -= hk * per_head;
-                int lo = 0, hi = tiles - 1;  // the last tile that begins at or before the place
-                while (lo < hi) {
-                    const int mid = (lo + hi + 1) >> 1;
-                    if (steps_before(q, mid, p.group) <= rest) lo = mid; else hi = mid - 1;
+                int tile = 0, hi = tiles - 1;  // the last tile that begins at or before the place
+                while (tile < hi) {
+                    const int mid = (tile + hi + 1) >> 1;
+                    if (pairs_before(q, mid, p.tokens) <= rest) tile = mid; else hi = mid - 1;
                 }
-                int tile = lo, t0 = (int)(rest - steps_before(q, tile, p.group));
-                bool head_written = false;
-                uint32_t it = 0;
-                for (long long u = u0;; ++it) {
-                    const uint32_t st = it % ITEMS;
-                    ok = ok && wait_bar(item_empty + 8 * st, ((it / ITEMS) & 1u) ^ 1u, 70);
-                    Item* d = items + st;
-                    if (u >= u1) {
-                        d->last = 1;
-                        mbar_arrive(item_full + 8 * st);
-                        break;
+                int off = (int)(rest - pairs_before(q, tile, p.tokens));
+                Item d;
+                for (long long u = w.u; ok && u < w.end;) {
+                    d.start = q.start, d.n = q.n, d.kv = q.kv, d.b = b, d.hk = hk, d.tok0 = tile * 2 * p.tokens, d.last = 0;
+                    const int steps = steps_of(keys_of(q, min(d.tok0 + 2 * p.tokens, q.n) - 1)), cost = steps + kItemCost;
+                    const int to = (int)min((long long)cost, off + (w.end - u));
+                    d.t0 = max(off - kItemCost, 0);
+                    const int t1 = max(to - kItemCost, 0);
+                    const bool begins = d.t0 == 0, ends = to == cost;
+                    if (t1 > d.t0) {
+                        d.slot = begins && ends ? -1 : 2 * (int)blockIdx.x + (begins ? 1 : 0);
+                        d.steps[0] = max(min(t1, steps_of(keys_of(q, d.tok0 + p.tokens - 1))) - d.t0, 0);  // its tokens see fewer keys
+                        d.steps[1] = t1 - d.t0;
+                        publish(0, it, d);
+                        if (begins && !ends && lane < 2) {  // the pieces behind this one: one per worker, up to that of the last place
+                            int* h = p.headers + (lane * blocks + blockIdx.x) * HEADER;
+                            const int tok0 = d.tok0 + lane * p.tokens;
+                            h[1] = q.start, h[2] = hk, h[3] = tok0, h[4] = max(min(p.tokens, q.n - tok0), 0) * p.group;
+                            h[0] = (int)((u + (cost - off) - 1) / w.share) - (int)blockIdx.x + 1;
+                        }
+                        const int n = d.steps[1];
+                        int ids[3] = {page_at(d, d.t0), n > 1 ? page_at(d, d.t0 + 1) : 0, 0};  // asked for a step before they are needed
+                        load(&kmap, d, d.t0, ids[0]);
+                        for (int i = 0; ok && i < n; ++i) {  // keys run one step ahead of the values
+                            if (i + 2 < n) ids[2] = page_at(d, d.t0 + i + 2);
+                            if (i + 1 < n) load(&kmap, d, d.t0 + i + 1, ids[1]);
+                            load(&vmap, d, d.t0 + i, ids[0]);
+                            ids[0] = ids[1], ids[1] = ids[2];
+                        }
                     }
-                    const int r0 = tile * TILE_ROWS, r_end = min(r0 + TILE_ROWS, q.n * p.group);
-                    const int steps = steps_of(keys_of(q, r_end - 1, p.group));
-                    const int t1 = (int)min((long long)steps, t0 + (u1 - u));
-                    const bool ends = t1 == steps;
-                    d->last = 0;
-                    d->start = q.start, d->n = q.n, d->kv = q.kv, d->b = b, d->hk = hk, d->r0 = r0, d->rows = r_end - r0, d->t0 = t0;
-                    d->single = r_end - r0 <= BM;
-                    d->slot = t0 == 0 && ends ? -1 : 2 * (int)blockIdx.x + (t0 == 0 ? 1 : 0);
-                    if (d->single) {
-                        d->steps[0] = (t1 - t0 + 1) / 2, d->steps[1] = (t1 - t0) / 2;
-                    } else {
-                        const int first = steps_of(keys_of(q, r0 + BM - 1, p.group));  // the upper stream's rows see fewer keys
-                        d->steps[0] = max(min(t1, first) - t0, 0), d->steps[1] = t1 - t0;
-                    }
-                    mbar_arrive(item_full + 8 * st);
-                    if (t0 == 0 && !ends) {  // begins here and goes on: the pieces behind it lie one per block
-                        const long long behind = u + steps - u1;
-                        header[1] = q.start, header[2] = hk, header[3] = r0, header[4] = r_end - r0;
-                        header[0] = 1 + (int)((behind + share - 1) / share);
-                        head_written = true;
-                    }
-                    u += t1 - t0;
-                    t0 = 0;
+                    u += to - off;
+                    off = 0;
                     if (ends && ++tile == tiles) {
                         tile = 0;
                         if (++hk == p.hkv) {
                             hk = 0;
-                            do {  // u < u1 says that one with rows follows
+                            do {  // u < end says that one with pairs follows
                                 if (++b >= p.batch) break;
                                 q = request_of(p, b);
-                                tiles = tiles_of(q, p.group);
+                                tiles = pair_tiles(q, p.tokens);
                             } while (tiles == 0);
+                            if (b >= p.batch) break;
                         }
                     }
                 }
-                if (!head_written) header[0] = 0;
-            }
-        } else if (warp == kTmaWarp) {
-            // ------------------------------ pages -> ring ------------------------------
-            uint32_t ring_it = 0;
-            const int box_rows = min(p.page, BN), boxes = BN / box_rows;
-            for (uint32_t it = 0;; ++it) {
-                const uint32_t st = it % ITEMS;
-                ok = __all_sync(~0u, ok && wait_bar(item_full + 8 * st, (it / ITEMS) & 1u, 71));
-                const Item d = items[st];
-                __syncwarp();
-                if (lane == 0) mbar_arrive(item_empty + 8 * st);
-                if (!ok || d.last) break;
-                const int steps = d.single ? d.steps[0] + d.steps[1] : d.steps[1];
-                const int* table = p.page_table + (long long)d.b * p.width;
-                const int held = (d.kv + p.page - 1) >> p.page_shift;
-                // Lane l copies box l / HALVES, columns 64 (l % HALVES).  Where a box holds no key of the request the page is one
-                // behind the pool: zeros without a read.
-                const int box = lane / C::HALVES, half = lane % C::HALVES;
-                auto page_at = [&](int step) {
-                    const int at = (step * BN + box * box_rows) >> p.page_shift;
-                    int id = p.num_pages;
-                    if (box < boxes && at < held) id = table[at];
-                    return (unsigned)id < (unsigned)p.num_pages ? id : p.num_pages;
-                };
-                auto load = [&](const CUtensorMap* map, int step, int id) {
-                    const uint32_t s = ring_it % C::STAGES, ph = (ring_it / C::STAGES) & 1u;
-                    ok = __all_sync(~0u, ok && wait_bar(kv_empty + 8 * s, ph ^ 1u, 72));
-                    if (!ok) return;
-                    ++ring_it;
-                    if (lane == 0) mbar_arrive_expect_tx(kv_full + 8 * s, C::STAGE_BYTES);
-                    __syncwarp();
-                    if (box < boxes)
-                        tma_load_4d(ring + s * C::STAGE_BYTES + half * C::HALF_BYTES + box * box_rows * 128, map, half * 64,
-                                    (step * BN + box * box_rows) & (p.page - 1), d.hk, id, kv_full + 8 * s);
-                };
-                // keys run one step ahead of the values, two where the streams alternate
-                const int lead = d.single ? 2 : 1;
-                int ids[3] = {page_at(d.t0), steps > 1 ? page_at(d.t0 + 1) : 0, 0};
-                load(&kmap, d.t0, ids[0]);
-                if (lead == 2 && steps > 1) load(&kmap, d.t0 + 1, ids[1]);
-                for (int i = 0; i < steps; ++i) {
-                    if (i + 2 < steps) ids[2] = page_at(d.t0 + i + 2);
-                    if (lead == 1 && i + 1 < steps) load(&kmap, d.t0 + i + 1, ids[1]);
-                    load(&vmap, d.t0 + i, ids[0]);
-                    if (lead == 2 && i + 2 < steps) load(&kmap, d.t0 + i + 2, ids[2]);
-                    ids[0] = ids[1], ids[1] = ids[2];
+                d.last = 1;
+                publish(0, it, d);
+            } else if (has_pairs) {
+                uint32_t q_ph[2] = {0, 0};
+                Item d;
+                for (uint32_t it = 0; take(0, it, d);) {
+                    if (d.steps[0] > 0) load_queries(0, 0, q_ph[0], d.start + d.tok0, d.hk);
+                    load_queries(1, 0, q_ph[1], d.start + d.tok0 + p.tokens, d.hk);
                 }
             }
-            const uint32_t pending = ring_it < (uint32_t)C::STAGES ? ring_it : (uint32_t)C::STAGES;
-            if (!ok)
-                for (uint32_t j = 0; j < pending; ++j) {  // copies under way still land
-                    const uint32_t i2 = ring_it - 1 - j;
-                    wait_bar(kv_full + 8 * (i2 % C::STAGES), (i2 / C::STAGES) & 1u, 73);
+            const Place w = places[1 + s];
+            if (w.b >= 0) {
+                // The pairs' products have read the ring and the queries: now each stream has a half.
+                if (has_pairs) ok = __all_sync(~0u, ok && wait_bar(bar(C::PAIRS_DONE), 0, 77));
+                const uint32_t own = ring + s * (C::STAGES * C::SLOT_BYTES), first = (uint32_t)(s * C::STAGES);
+                const int id = s * blocks + (int)blockIdx.x;
+                uint32_t it = 0, slot = 0, ph = 0, q_ph = 0;
+                auto load = [&](const CUtensorMap* map, const Item& d, int step, int page_id) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        ok = __all_sync(~0u, ok && wait_bar(bar(C::SLOT_EMPTY + first + slot), ph ^ 1u, 78));
+                        if (!ok) return;
+                        const uint32_t full = bar(C::SLOT_FULL + first + slot);
+                        if (lane == 0) mbar_arrive_expect_tx(full, C::SLOT_BYTES);
+                        __syncwarp();
+                        const int at = box * box_rows - h * HN;  // the box's first row in this slot
+                        if (at >= 0 && at < HN) copy_box(map, own + slot * C::SLOT_BYTES + half * (HN * 128) + at * 128, step, d.hk, page_id, full);
+                            if (++slot == C::STAGES) slot = 0, ph ^= 1u;
+                    }
+                };
+                int b = w.b;
+                Request q = request_of(p, b);
+                int cost = steps_of(q.kv) + kItemCost;
+                int hk = (int)(w.rest / cost), off = (int)(w.rest - (long long)hk * cost);
+                Item d;
+                for (long long u = w.u; ok && u < w.end;) {
+                    const int to = (int)min((long long)cost, off + (w.end - u));
+                    d.t0 = max(off - kItemCost, 0);
+                    const int t1 = max(to - kItemCost, 0);
+                    const bool begins = d.t0 == 0, ends = to == cost;
+                    if (t1 > d.t0) {
+                        d.start = q.start, d.n = q.n, d.kv = q.kv, d.b = b, d.hk = hk, d.last = 0;
+                        d.tok0 = (q.n - 1) / (2 * p.tokens) * (2 * p.tokens);
+                        d.steps[s] = t1 - d.t0, d.steps[s ^ 1] = 0;
+                        d.slot = begins && ends ? -1 : 4 * blocks + 2 * id + (begins ? 1 : 0);
+                        publish(1 + s, it, d);
+                        if (begins && !ends && lane == 0) {
+                            int* h = p.headers + (2 * blocks + id) * HEADER;
+                            h[1] = q.start, h[2] = hk, h[3] = d.tok0, h[4] = (q.n - d.tok0) * p.group;
+                            h[0] = (int)((u + (cost - off) - 1) / w.share) - id + 1;
+                        }
+                        int ids[3] = {page_at(d, d.t0), d.t0 + 1 < t1 ? page_at(d, d.t0 + 1) : 0, 0};  // asked for a step before they are needed
+                        for (int step = d.t0; ok && step < t1; ++step) {
+                            if (step + 2 < t1) ids[2] = page_at(d, step + 2);
+                            load(&kmap, d, step, ids[0]);
+                            if (step == d.t0) load_queries(s, 1, q_ph, d.start + d.tok0, d.hk);
+                            load(&vmap, d, step, ids[0]);
+                            ids[0] = ids[1], ids[1] = ids[2];
+                        }
+                    }
+                    u += to - off;
+                    off = 0;
+                    if (ends && ++hk == p.hkv) {
+                        hk = 0;
+                        do {  // u < end says that one with such an item follows
+                            if (++b >= p.batch) break;
+                            q = request_of(p, b);
+                        } while (!has_single(q, p.tokens));
+                        if (b >= p.batch) break;
+                        cost = steps_of(q.kv) + kItemCost;
+                    }
                 }
-        } else if (warp == kMmaWarp) {
+                d.last = 1;
+                publish(1 + s, it, d);
+            }
+            if (!ok) {  // a wait has given up: copies under way (microseconds) get a millisecond to land
+                const long long t0 = clock64();
+                while (clock64() - t0 < 2000000) {
+                }
+            }
+        } else {
             // ------------------------------ matrix products ------------------------------
-            uint32_t ring_it = 0, q_uses[2] = {0, 0}, p_uses[2] = {0, 0};
-            auto stage = [&](uint32_t i) { return ring + (i % C::STAGES) * C::STAGE_BYTES; };
-            auto wait_stage = [&](uint32_t i) { ok = __all_sync(~0u, ok && wait_bar(kv_full + 8 * (i % C::STAGES), (i / C::STAGES) & 1u, 74)); };
-            auto free_stage = [&](uint32_t i) {
-                if (ok && elect_one()) umma_commit(kv_empty + 8 * (i % C::STAGES));
+            // All lanes walk the loops on values that the compiler knows to be the same in all of them (see elect_one).
+            const int s = warp == kMmaWarp1;
+            const uint64_t q_desc = make_smem_desc(q_smem);
+            uint32_t q_ph[2] = {0, 0}, p_ph[2] = {0, 0};
+            auto wait_in = [&](int barrier, uint32_t ph, int where) { ok = __all_sync(~0u, ok && wait_bar(bar(barrier), ph, where)); };
+            auto commit = [&](int barrier) {
+                if (ok && elect_one()) umma_commit(bar(barrier));
                 __syncwarp();
             };
-            auto wait_q = [&](int s) {
-                ok = __all_sync(~0u, ok && wait_bar(q_full + 8 * s, q_uses[s] & 1u, 75));
-                ++q_uses[s];
+            auto take_uniform = [&](int list, uint32_t& it, Item& d) {
+                Item x;
+                const bool more = take(list, it, x);
+                d.n = __shfl_sync(~0u, x.n, 0), d.kv = __shfl_sync(~0u, x.kv, 0), d.t0 = __shfl_sync(~0u, x.t0, 0);
+                d.steps[0] = __shfl_sync(~0u, x.steps[0], 0), d.steps[1] = __shfl_sync(~0u, x.steps[1], 0);
+                return __all_sync(~0u, more) != 0;
             };
-            auto wait_p = [&](int s) {
-                ok = __all_sync(~0u, ok && wait_bar(p_full + 8 * s, p_uses[s] & 1u, 76));
-                ++p_uses[s];
-                tc_fence_after();
-            };
-            auto scores = [&](int s, int q_tile, uint32_t k_it) {  // S_s = Q K^T
-                if (ok && elect_one()) {
-                    const uint64_t a = make_smem_desc(q_smem + q_tile * C::Q_BYTES), b = make_smem_desc(stage(k_it));
-    #pragma unroll
-                    for (int k = 0; k < D / 16; ++k) {
-                        const uint32_t o = (k / 4) * (C::HALF_BYTES >> 4) + (k % 4) * 2;
-                        umma_bf16(tmem + C::S_COL + 128 * s, a + o, b + o, C::IDESC_S, k > 0);
-                    }
-                    umma_commit(s_full + 8 * s);
+            // Rows of the last page behind the request's tokens hold anything; a zero weight does not make a NaN harmless.
+            // `rows` rows at `at` in shared memory begin with key `key`; the halves of the columns lie rows * 128 bytes apart.
+            auto clean = [&](uint32_t at, int key, int rows, int kv) {
+                const int live = kv - key;
+                if (live >= rows) return;
+                const int from = max(live, 0), to = min((((max(live, 0) + key + p.page - 1) >> p.page_shift) << p.page_shift) - key, rows);
+                if (from >= to) return;
+                for (int i = from * C::HALVES * 8 + lane; i < to * C::HALVES * 8; i += 32) {
+                    const int row = i / (C::HALVES * 8), piece = i % (C::HALVES * 8);
+                    sts128(at + (piece / 8) * (rows * 128) + row * 128 + (piece % 8) * 16, make_uint4(0, 0, 0, 0));
                 }
+                fence_proxy_async_smem();
                 __syncwarp();
             };
-            auto values = [&](int s, uint32_t v_it, bool accumulate, bool end) {  // O_s += P V
-                if (ok && elect_one()) {
-                    const uint64_t b = make_mn_desc(stage(v_it), C::HALF_BYTES);
-    #pragma unroll
-                    for (int k = 0; k < BN / 16; ++k)
-                        umma_bf16_ts(tmem + C::O_COL + D * s, tmem + C::S_COL + 128 * s + 8 * k, b + k * (2048 >> 4), C::IDESC_O, accumulate || k > 0);
-                    if (end) umma_commit(o_full + 8 * s);
-                }
-                __syncwarp();
-            };
-            for (uint32_t it = 0;; ++it) {
-                const uint32_t st = it % ITEMS;
-                ok = __all_sync(~0u, ok && wait_bar(item_full + 8 * st, (it / ITEMS) & 1u, 77));
-                const Item d = items[st];
-                __syncwarp();
-                if (lane == 0) mbar_arrive(item_empty + 8 * st);
-                if (!ok || d.last) break;
-                // Rows of the last page behind the request's tokens hold anything; a zero weight does not make a NaN harmless.
-                auto clean = [&](uint32_t v_it, int step) {
-                    const int live = d.kv - step * BN;
-                    if (live >= BN) return;
-                    const int from = max(live, 0), to = min(((from + p.page - 1) >> p.page_shift) << p.page_shift, BN);
-                    if (from == to) return;
-                    for (int i = from * C::HALVES * 8 + lane; i < to * C::HALVES * 8; i += 32) {
-                        const int row = i / (C::HALVES * 8), piece = i % (C::HALVES * 8);
-                        sts128(stage(v_it) + (piece / 8) * C::HALF_BYTES + row * 128 + (piece % 8) * 16, make_uint4(0, 0, 0, 0));
+            if (has_pairs && s == 0) {
+                struct Stage {
+                    uint32_t at, ph;
+                    __device__ __forceinline__ Stage next() const { return at + 1 == C::STAGES ? Stage{0, ph ^ 1u} : Stage{at + 1, ph}; }
+                };
+                const uint64_t k_desc = make_smem_desc(ring), v_desc = make_mn_desc(ring, BN * 128);
+                Stage next{0, 0};  // the next stage of the ring in the order of the copies
+                auto wait_q = [&](int t) { wait_in(C::Q_FULL + t, q_ph[t], 81), q_ph[t] ^= 1u; };
+                auto wait_p = [&](int t) {
+                    wait_in(C::P_FULL + t, p_ph[t], 82), p_ph[t] ^= 1u;
+                    tc_fence_after();
+                };
+                auto scores = [&](int t, const Stage& g) {  // S = Q K^T of stream t
+                    const uint64_t a = q_desc + (uint64_t)(t * (C::Q_BYTES >> 4)), b = k_desc + (uint64_t)(g.at * (C::STAGE_BYTES >> 4));
+                    if (ok && elect_one()) {
+#pragma unroll
+                        for (int k = 0; k < D / 16; ++k) {
+                            const uint32_t o = (k / 4) * (BM * 128 >> 4) + (k % 4) * 2;
+                            umma_bf16(tmem + C::S_COL + 128 * t, a + o, b + o, C::IDESC_S, k > 0);
+                        }
+                        umma_commit(bar(C::S_FULL + t));
                     }
-                    fence_proxy_async_smem();
                     __syncwarp();
                 };
-                if (d.single) {
-                    const int n = d.steps[0] + d.steps[1];
-                    wait_q(0);
-                    for (int i = 0; i < 2 && i < n; ++i) {
-                        wait_stage(ring_it);
-                        scores(i, 0, ring_it);
-                        free_stage(ring_it++);
+                auto values = [&](int t, const Stage& g, uint32_t accumulate) {  // O += P V
+                    const uint64_t b = v_desc + (uint64_t)(g.at * (C::STAGE_BYTES >> 4));
+                    if (ok && elect_one()) {
+                        umma_bf16_ts(tmem + C::O_COL + D * t, tmem + C::S_COL + 128 * t, b, C::IDESC_O, accumulate);
+#pragma unroll
+                        for (int k = 1; k < BN / 16; ++k)
+                            umma_bf16_ts(tmem + C::O_COL + D * t, tmem + C::S_COL + 128 * t + 8 * k, b + k * (2048 >> 4), C::IDESC_O, 1u);
                     }
-                    for (int i = 0; i < n; ++i) {
-                        const int s = i & 1;
-                        wait_stage(ring_it);
-                        clean(ring_it, d.t0 + i);
-                        wait_p(s);
-                        values(s, ring_it, i > 1, i + 2 >= n);
-                        free_stage(ring_it++);
-                        if (i + 2 < n) {
-                            wait_stage(ring_it);
-                            scores(s, 0, ring_it);
-                            free_stage(ring_it++);
-                        }
-                    }
-                } else {
+                    __syncwarp();
+                };
+                Item d;
+                for (uint32_t it = 0; take_uniform(0, it, d);) {
                     const int n0 = d.steps[0], n1 = d.steps[1];
-                    wait_stage(ring_it);
+                    wait_in(C::PAIR_FULL + next.at, next.ph, 83);
                     if (n0 > 0) {
                         wait_q(0);
-                        scores(0, 0, ring_it);
+                        scores(0, next);
+                        if (n0 == 1) commit(C::Q_EMPTY);
                     }
                     wait_q(1);
-                    scores(1, 1, ring_it);
-                    free_stage(ring_it++);
+                    scores(1, next);
+                    if (n1 == 1) commit(C::Q_EMPTY + 1);
+                    commit(C::PAIR_EMPTY + next.at);
+                    next = next.next();
                     for (int i = 0; i < n1; ++i) {
-                        // next keys at ring_it, these values behind them
+                        // the next keys, and these values behind them
                         const bool more = i + 1 < n1;
-                        const uint32_t k_it = ring_it, v_it = ring_it + (more ? 1 : 0);
-                        ring_it = v_it + 1;
-                        if (more) wait_stage(k_it);
-                        wait_stage(v_it);
-                        clean(v_it, d.t0 + i);
+                        const Stage keys = next, vals = more ? next.next() : next;
+                        next = vals.next();
+                        if (more) wait_in(C::PAIR_FULL + keys.at, keys.ph, 84);
+                        wait_in(C::PAIR_FULL + vals.at, vals.ph, 85);
+                        clean(ring + vals.at * C::STAGE_BYTES, (d.t0 + i) * BN, BN, d.kv);
                         if (i < n0) {
                             wait_p(0);
-                            values(0, v_it, i > 0, i + 1 == n0);
-                            if (i + 1 < n0) scores(0, 0, k_it);
+                            values(0, vals, i > 0);
+                            if (i + 1 < n0) scores(0, keys);
+                            else commit(C::O_FULL);
+                            if (i + 2 == n0) commit(C::Q_EMPTY);
                         }
                         wait_p(1);
-                        values(1, v_it, i > 0, !more);
-                        free_stage(v_it);
+                        values(1, vals, i > 0);
+                        commit(C::PAIR_EMPTY + vals.at);
                         if (more) {
-                            scores(1, 1, k_it);
-                            free_stage(k_it);
+                            scores(1, keys);
+                            commit(C::PAIR_EMPTY + keys.at);
+                        } else {
+                            commit(C::O_FULL + 1);
+                        }
+                        if (i + 2 == n1) commit(C::Q_EMPTY + 1);
+                    }
+                }
+                if (elect_one()) umma_commit(bar(C::PAIRS_DONE));
+                __syncwarp();
+            }
+            if (places[1 + s].b >= 0) {
+                if (has_pairs) wait_in(C::PAIRS_DONE, 0, 86);
+                const uint32_t own = ring + s * (C::STAGES * C::SLOT_BYTES);
+                const int first = s * C::STAGES;
+                const uint64_t k_desc = make_smem_desc(own), v_desc = make_mn_desc(own, HN * 128), a = q_desc + (uint64_t)(s * (C::Q_BYTES >> 4));
+                const uint32_t s_col = tmem + C::S_COL + 128 * s, o_col = tmem + C::O_COL + D * s;
+                uint32_t slot = 0, ph = 0, q_parity = 0, p_parity = 0;
+                auto advance = [&]() {
+                    if (++slot == C::STAGES) slot = 0, ph ^= 1u;
+                };
+                Item d;
+                for (uint32_t it = 0; take_uniform(1 + s, it, d);) {
+                    const int n = d.steps[s];
+                    wait_in(C::Q_FULL + 2 + s, q_parity, 87), q_parity ^= 1u;
+                    for (int i = 0; ok && i < n; ++i) {
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            wait_in(C::SLOT_FULL + first + (int)slot, ph, 88);
+                            const uint64_t b = k_desc + (uint64_t)(slot * (C::SLOT_BYTES >> 4));
+                            if (ok && elect_one()) {
+#pragma unroll
+                                for (int k = 0; k < D / 16; ++k)
+                                    umma_bf16(s_col + HN * h, a + (k / 4) * (BM * 128 >> 4) + (k % 4) * 2, b + (k / 4) * (HN * 128 >> 4) + (k % 4) * 2,
+                                              C::IDESC_S_SLOT, k > 0);
+                                umma_commit(bar(C::SLOT_EMPTY + first + slot));
+                            }
+                            __syncwarp();
+                            advance();
+                        }
+                        commit(C::S_FULL + 2 + s);
+                        if (i + 1 == n) commit(C::Q_EMPTY + 2 + s);
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            wait_in(C::SLOT_FULL + first + (int)slot, ph, 89);
+                            clean(own + slot * C::SLOT_BYTES, (d.t0 + i) * BN + h * HN, HN, d.kv);
+                            if (h == 0) {
+                                wait_in(C::P_FULL + 2 + s, p_parity, 90), p_parity ^= 1u;
+                                tc_fence_after();
+                            }
+                            const uint64_t b = v_desc + (uint64_t)(slot * (C::SLOT_BYTES >> 4));
+                            const uint32_t accumulate = i > 0 || h > 0;
+                            if (ok && elect_one()) {
+                                umma_bf16_ts(o_col, s_col + 32 * h, b, C::IDESC_O, accumulate);
+#pragma unroll
+                                for (int k = 1; k < HN / 16; ++k) umma_bf16_ts(o_col, s_col + 32 * h + 8 * k, b + k * (2048 >> 4), C::IDESC_O, 1u);
+                                umma_commit(bar(C::SLOT_EMPTY + first + slot));
+                            }
+                            __syncwarp();
+                            advance();
                         }
                     }
+                    commit(C::O_FULL + 2 + s);
                 }
             }
             // Every product has ended and every arrival that it owes has been made before the block's memory goes.
-            if (elect_one()) umma_commit(done);
+            if (elect_one()) umma_commit(bar(C::DONE + s));
             __syncwarp();
-            wait_bar(done, 0, 83);
+            wait_bar(bar(C::DONE + s), 0, 91);
         }
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == kMmaWarp) {
+    if (warp == kMmaWarp0) {
         tc_fence_after();
         tmem_dealloc(tmem, 512);
     }
 }
 
-// Joins the pieces of the item that begins in block x of the first kernel, 32 rows of it per block.
+// Joins the pieces of the item that begins at worker x of the first kernel and goes on behind it, 32 rows of it per block.
 template <int D>
 __global__ void __launch_bounds__(256) paged_attention_join_kernel(const Params p) {
     wait_for_preceding_grid();
     const int* header = p.headers + blockIdx.x * HEADER;
-    const int pieces = header[0], start = header[1], hk = header[2], r0 = header[3], rows = header[4];
+    const int pieces = header[0], start = header[1], hk = header[2], tok0 = header[3], rows = header[4];
     const int row = blockIdx.y * 32 + (threadIdx.x & 31);
     if (pieces == 0 || row >= rows) return;
     const long long slot_floats = (long long)p.slot_rows * (D + 2);
@@ -796,8 +865,8 @@ __global__ void __launch_bounds__(256) paged_attention_join_kernel(const Params 
         }
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    const int r = r0 + row, token = r / p.group, head = hk * p.group + (r - token * p.group);
-    __nv_bfloat16* out = p.out + (start + token) * p.o_token + head * p.o_head + (threadIdx.x >> 5) * PER * 4;
+    const int token = row / p.group, head = hk * p.group + (row - token * p.group);
+    __nv_bfloat16* out = p.out + (start + tok0 + token) * p.o_token + head * p.o_head + (threadIdx.x >> 5) * PER * 4;
 #pragma unroll
     for (int j = 0; j < PER; ++j)
         *reinterpret_cast<uint2*>(out + 4 * j) = make_uint2(pack_bf16x2(o[j].x * inv, o[j].y * inv), pack_bf16x2(o[j].z * inv, o[j].w * inv));
@@ -822,26 +891,38 @@ static int sm_count() {
     return counts[dev];
 }
 
-// Rows of a partial result: a tile's, or what the whole call has of one head where that is less.
+// Rows of a partial result: a stream's, or what the whole call has of one head where that is less.
 static int slot_rows_of(int rows, int group) {
     const long long all = ((long long)rows * group + 31) / 32 * 32;
-    return (int)(all < TILE_ROWS ? all : TILE_ROWS);
+    return (int)(all < BM ? all : BM);
 }
 
-static int encode_page_map(CUtensorMap* map, const void* base, const long long* strides, int num_pages, int page, int heads, int D) {
+static int encode_map(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box,
+                      CUtensorMapL2promotion promotion) {
     EncodeTiledFn fn = get_encode_fn();
     if (fn == nullptr) return QB200_ERR_DRIVER;
+    const cuuint32_t unit[4] = {1, 1, 1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), dims, strides, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, promotion, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? QB200_OK : QB200_ERR_DRIVER;
+}
+// The stride of a dimension of one entry is never used, but has to be a valid one.
+static cuuint64_t stride_bytes(long long stride, long long entries, int D) { return (cuuint64_t)(entries > 1 ? stride : D) * 2; }
+
+static int encode_page_map(CUtensorMap* map, const void* base, const long long* strides, int num_pages, int page, int heads, int D) {
     const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)page, (cuuint64_t)heads, (cuuint64_t)num_pages};
-    // the stride of a dimension of one entry is never used, but has to be a valid one
-    const cuuint64_t st[3] = {(cuuint64_t)strides[1] * 2, (cuuint64_t)(heads > 1 ? strides[2] : D) * 2, (cuuint64_t)(num_pages > 1 ? strides[0] : D) * 2};
-    const cuuint32_t box[4] = {64, (cuuint32_t)(page < BN ? page : BN), 1, 1}, unit[4] = {1, 1, 1, 1};
-    return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, st, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE,
-              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
-               ? QB200_OK : QB200_ERR_DRIVER;
+    const cuuint64_t st[3] = {stride_bytes(strides[1], page, D), stride_bytes(strides[2], heads, D), stride_bytes(strides[0], num_pages, D)};
+    const cuuint32_t box[4] = {64, (cuuint32_t)(page < HN ? page : HN), 1, 1};
+    return encode_map(map, base, 4, dims, st, box, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
+}
+static int encode_query_map(CUtensorMap* map, const void* base, const long long* strides, int rows, int heads, int group, int D) {
+    const cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)heads, (cuuint64_t)rows};
+    const cuuint64_t st[2] = {stride_bytes(strides[1], heads, D), stride_bytes(strides[0], rows, D)};
+    const cuuint32_t box[3] = {64, (cuuint32_t)group, (cuuint32_t)(BM / group)};
+    return encode_map(map, base, 3, dims, st, box, CU_TENSOR_MAP_L2_PROMOTION_L2_128B);
 }
 
 template <int D>
-static int launch(Params p, const CUtensorMap& kmap, const CUtensorMap& vmap, int blocks, cudaStream_t stream) {
+static int launch(const Params& p, const CUtensorMap& qmap, const CUtensorMap& kmap, const CUtensorMap& vmap, int blocks, cudaStream_t stream) {
     static bool prepared[kMaxDevices];  // of the device, once; a second thread that does it again does no harm
     const int dev = current_device();
     if (dev < 0) return QB200_ERR_CUDA;
@@ -849,11 +930,11 @@ static int launch(Params p, const CUtensorMap& kmap, const CUtensorMap& vmap, in
         if (cudaFuncSetAttribute(paged_attention_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::SMEM) != cudaSuccess) return QB200_ERR_CUDA;
         prepared[dev] = true;
     }
-    paged_attention_kernel<D><<<blocks, kThreads, Cfg<D>::SMEM, stream>>>(p, kmap, vmap);
+    paged_attention_kernel<D><<<blocks, kThreads, Cfg<D>::SMEM, stream>>>(p, qmap, kmap, vmap);
     const int st = launch_status();
     if (st != QB200_OK) return st;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(blocks, (p.slot_rows + 31) / 32);
+    cfg.gridDim = dim3(4 * blocks, p.slot_rows / 32);
     cfg.blockDim = dim3(256);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
@@ -875,7 +956,7 @@ using namespace qb;
 extern "C" int paged_attention_workspace(int rows, int batch, int n_head, int n_kv_head, int head_dim) {
     if (rows <= 0 || batch <= 0 || n_head <= 0 || n_kv_head <= 0 || n_head % n_kv_head != 0 || head_dim <= 0 || head_dim > 128) return 0;
     const long long sms = pa::sm_count();
-    return (int)(sms * (2ll * pa::slot_rows_of(rows, n_head / n_kv_head) * (head_dim + 2) * 4 + pa::HEADER * 4));
+    return (int)(sms * (8ll * pa::slot_rows_of(rows, n_head / n_kv_head) * (head_dim + 2) * 4 + 4 * pa::HEADER * 4));
 }
 
 extern "C" int paged_attention_cuda_bf16(void* out, const long long* out_strides, const void* q, const long long* q_strides,
@@ -883,36 +964,35 @@ extern "C" int paged_attention_cuda_bf16(void* out, const long long* out_strides
                                          const long long* v_strides, const int* page_table, const int* kv_lens, const int* cu_new,
                                          void* workspace, float scale, int rows, int batch, int width, int n_head, int n_kv_head,
                                          int head_dim, int num_pages, int page_size, cudaStream_t stream) {
-    if (rows < 0 || batch < 0 || width < 0 || n_head <= 0 || n_kv_head <= 0 || num_pages < 0 || page_size <= 0) return QB200_ERR_INVALID_ARGUMENT;
+    if (rows < 0 || batch < 0 || width < 0 || n_head <= 0 || n_kv_head <= 0 || num_pages < 0 || page_size <= 0 || !(scale >= 0.f)) return QB200_ERR_INVALID_ARGUMENT;
     if (rows == 0 || batch == 0) return QB200_OK;
     if (!out || !out_strides || !q || !q_strides || !k_strides || !v_strides || !kv_lens || !cu_new || !workspace || (width && !page_table) ||
         !k_cache || !v_cache || num_pages == 0)
         return QB200_ERR_INVALID_ARGUMENT;
-    if ((head_dim != 64 && head_dim != 128) || n_head % n_kv_head != 0 || (page_size & (page_size - 1)) != 0 || page_size < 16 || page_size > 1024 ||
-        !aligned16(out) || !aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(workspace))
+    if ((head_dim != 64 && head_dim != 128) || n_head % n_kv_head != 0 || n_head / n_kv_head > pa::BM || (page_size & (page_size - 1)) != 0 ||
+        page_size < 16 || page_size > 1024 || (long long)width * page_size > 0x3fffffffll || rows > (1 << 29) || !aligned16(out) || !aligned16(q) ||
+        !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(workspace))
         return QB200_ERR_UNSUPPORTED;
-    const int group = n_head / n_kv_head;
-    if ((long long)rows * group > (1ll << 30) || (long long)width * page_size * group > 0x7fffffffll) return QB200_ERR_UNSUPPORTED;
     for (int i = 0; i < 3; ++i)
         if (k_strides[i] % 8 || v_strides[i] % 8 || (i < 2 && (q_strides[i] % 8 || out_strides[i] % 8))) return QB200_ERR_UNSUPPORTED;
-    const int sms = pa::sm_count();
+    const int group = n_head / n_kv_head, sms = pa::sm_count();
     if (sms == 0) return QB200_ERR_CUDA;
-    CUtensorMap kmap, vmap;
-    int st = pa::encode_page_map(&kmap, k_cache, k_strides, num_pages, page_size, n_kv_head, head_dim);
+    CUtensorMap qmap, kmap, vmap;
+    int st = pa::encode_query_map(&qmap, q, q_strides, rows, n_head, group, head_dim);
+    if (st == QB200_OK) st = pa::encode_page_map(&kmap, k_cache, k_strides, num_pages, page_size, n_kv_head, head_dim);
     if (st == QB200_OK) st = pa::encode_page_map(&vmap, v_cache, v_strides, num_pages, page_size, n_kv_head, head_dim);
     if (st != QB200_OK) return st;
     pa::Params p{};
     p.out = static_cast<__nv_bfloat16*>(out);
-    p.q = static_cast<const __nv_bfloat16*>(q);
     p.page_table = page_table, p.kv_lens = kv_lens, p.cu = cu_new;
     p.slot_rows = pa::slot_rows_of(rows, group);
     p.partial = static_cast<float*>(workspace);
-    p.headers = reinterpret_cast<int*>(p.partial + sms * 2ll * p.slot_rows * (head_dim + 2));
-    p.o_token = out_strides[0], p.o_head = out_strides[1], p.q_token = q_strides[0], p.q_head = q_strides[1];
-    p.flip = scale < 0 ? 0x80008000u : 0u;
-    p.c = fmaxf(fabsf(scale) * 1.4426950408889634f, 1.17549435e-38f);  // above zero: what is masked stays at minus infinity
-    p.rows = rows, p.batch = batch, p.width = width, p.hkv = n_kv_head, p.group = group, p.num_pages = num_pages, p.page = page_size;
+    p.headers = reinterpret_cast<int*>(p.partial + sms * 8ll * p.slot_rows * (head_dim + 2));
+    p.o_token = out_strides[0], p.o_head = out_strides[1];
+    p.wide_stores = reinterpret_cast<uintptr_t>(out) % 32 == 0 && p.o_token % 16 == 0 && p.o_head % 16 == 0;
+    p.c = fmaxf(scale * 1.4426950408889634f, 1.17549435e-38f);  // above zero: what is masked stays at minus infinity
+    p.rows = rows, p.batch = batch, p.width = width, p.hkv = n_kv_head, p.group = group, p.tokens = pa::BM / group;
+    p.num_pages = num_pages, p.page = page_size;
     for (p.page_shift = 0; (1 << p.page_shift) < page_size; ++p.page_shift) {}
-    p.min_steps = 1;
-    return head_dim == 64 ? pa::launch<64>(p, kmap, vmap, sms, stream) : pa::launch<128>(p, kmap, vmap, sms, stream);
+    return head_dim == 64 ? pa::launch<64>(p, qmap, kmap, vmap, sms, stream) : pa::launch<128>(p, qmap, kmap, vmap, sms, stream);
 }
