@@ -82,8 +82,10 @@ class Attention(nn.Module):
         self.c_attn = nn.Linear(cfg.n_embd, 3 * cfg.n_embd, bias=False)
         self.c_proj = nn.Linear(cfg.n_embd, cfg.n_embd, bias=False)
 
-    def forward(self, x, table):
+    def forward(self, x, table, pages=None):
         B, T, C = x.shape
+        if pages is not None:  # packed tokens of many requests over a paged cache
+            return self.c_proj(pages.attend(self.c_attn(x).view(B * T, 3 * C), table, self.n_head).view(B, T, C))
         q, k, v = self.c_attn(x).split(self.n_embd, dim=2)
         q, k = apply_rope(q.view(B, T, self.n_head, -1), k.view(B, T, self.n_head, -1), table)
         v = v.view(B, T, self.n_head, -1)
@@ -108,13 +110,13 @@ class Block(nn.Module):
         self.ln_1, self.attn = RMSNorm(cfg.n_embd, cfg.rmsnorm_eps), Attention(cfg)
         self.ln_2, self.mlp = RMSNorm(cfg.n_embd, cfg.rmsnorm_eps), MLP(cfg)
 
-    def forward(self, x, table):
+    def forward(self, x, table, pages=None):
         if getattr(self, "fused", False):
-            return self.forward_fused(x, table)
-        x = x + self.attn(self.ln_1(x), table)
+            return self.forward_fused(x, table, pages)
+        x = x + self.attn(self.ln_1(x), table, pages)
         return x + self.mlp(self.ln_2(x))
 
-    def forward_fused(self, x, table):
+    def forward_fused(self, x, table, pages=None):
         """The same block with every quantiser fused into the producer of its input: RMSNorm -> quantise is one kernel
         (its result feeds c_attn, and w1 and w2 share one quantisation; the second one adds the residual, too),
         SiLU(w1 x) * w2 x -> quantise is one kernel, and q and k are rotated where the projection has left them.
@@ -131,15 +133,19 @@ class Block(nn.Module):
         q = quest.producer_hadamard_quantize(quest.PRODUCE_RMSNORM, flat, norm_weight=self.ln_1.weight, eps=self.ln_1.eps,
                                              block=HADAMARD_BLOCK, **ws(C, 3 * C))
         qkv = att.c_attn.forward_quantized(*q)
-        if kernels_may_replace(qkv, table) and rope_in_place_ok(qkv, table, T, att.n_head):
-            quest.rope_inplace(qkv, table, T, 2 * C)
-            qh, kh, vh = qkv.view(B, T, 3, att.n_head, -1).unbind(2)
+        if pages is not None:
+            y = pages.attend(qkv, table, att.n_head).view(B, T, C)
         else:
-            qh, kh, vh = qkv.view(B, T, 3 * C).split(C, dim=2)
-            qh, kh = apply_rope(qh.view(B, T, att.n_head, -1), kh.view(B, T, att.n_head, -1), table)
-            vh = vh.view(B, T, att.n_head, -1)
-        y = F.scaled_dot_product_attention(qh.transpose(1, 2), kh.transpose(1, 2), vh.transpose(1, 2), is_causal=True)
-        y = att.c_proj(y.transpose(1, 2).contiguous().view(B, T, C)).view(-1, C)
+            if kernels_may_replace(qkv, table) and rope_in_place_ok(qkv, table, T, att.n_head):
+                quest.rope_inplace(qkv, table, T, 2 * C)
+                qh, kh, vh = qkv.view(B, T, 3, att.n_head, -1).unbind(2)
+            else:
+                qh, kh, vh = qkv.view(B, T, 3 * C).split(C, dim=2)
+                qh, kh = apply_rope(qh.view(B, T, att.n_head, -1), kh.view(B, T, att.n_head, -1), table)
+                vh = vh.view(B, T, att.n_head, -1)
+            y = F.scaled_dot_product_attention(qh.transpose(1, 2), kh.transpose(1, 2), vh.transpose(1, 2), is_causal=True)
+            y = y.transpose(1, 2).contiguous().view(B, T, C)
+        y = att.c_proj(y).view(-1, C)
         if kernels_may_replace(flat, y):
             flat, q = quest.add_rmsnorm_hadamard_quantize(flat, y, norm_weight=self.ln_2.weight, eps=self.ln_2.eps,
                                                           block=HADAMARD_BLOCK, **ws(C, ffn))
@@ -176,10 +182,12 @@ class Decoder(nn.Module):
             if p.dim() > 1:
                 nn.init.normal_(p, mean=0.0, std=0.02)
 
-    def forward(self, idx: torch.Tensor) -> torch.Tensor:
+    def forward(self, idx: torch.Tensor, pages=None) -> torch.Tensor:
+        """Hidden states of idx (B, T).  ``pages`` (a list with one ``serving.LayerPages`` per layer): idx (1, T) holds packed
+        tokens of many requests, which attend over the paged cache."""
         x = self.transformer.wte(idx)
-        for blk in self.transformer.h:
-            x = blk(x, self.rope)
+        for i, blk in enumerate(self.transformer.h):
+            x = blk(x, self.rope, None if pages is None else pages[i])
         return self.transformer.ln_f(x)
 
 

@@ -1,0 +1,127 @@
+"""Decoding with the Llama-style decoder of ``prefill.py`` over a paged cache.
+
+``PagedCache`` owns the pages of every layer and the bookkeeping on the device; ``extend`` runs the new tokens of all requests
+(prompts, chunks of prompts, single tokens, drafts, in any mixture) through the model in one packed batch; ``generate`` is the
+greedy loop and ``verify`` one step of speculative decoding.  The reference stops at one forward pass without logits
+(gemm-quest/benchmarks/bench_e2e.py:98-121); its decoder has no cache.
+"""
+from __future__ import annotations
+
+import torch
+
+import quest_b200 as quest
+from .paged import PageStep
+from .prefill import Decoder, DecoderConfig
+
+
+class LayerPages:
+    """One layer's pages during one step: what its attention needs in place of dense keys and values."""
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, page_table: torch.Tensor, step: PageStep):
+        self.k, self.v, self.page_table, self.step = k, v, page_table, step
+
+    def attend(self, qkv: torch.Tensor, table: torch.Tensor, n_head: int) -> torch.Tensor:
+        """qkv [rows, 3 n_head head_dim], not rotated yet -> attention [rows, n_head, head_dim]; keys and values go to the pages.
+        Rows that belong to no request come out as zeros."""
+        head_dim = self.k.size(3)
+        rows = qkv.size(0)
+        q = quest.rope_paged_append(qkv, table, self.step.positions, self.step.slots, self.k, self.v, n_head)
+        out = torch.zeros(rows, n_head, head_dim, dtype=qkv.dtype, device=qkv.device)
+        return quest.paged_attention(q, self.k, self.v, self.page_table, self.step.kv_lens, self.step.cu_new, out=out)
+
+
+class PagedCache:
+    """Pages of all layers of a model for up to ``max_requests`` requests of up to ``max_length`` tokens; ``num_pages`` pages of
+    ``page_size`` tokens are shared by them.  ``lens`` [max_requests] are the tokens held, on the device."""
+
+    def __init__(self, cfg: DecoderConfig, num_pages: int, max_requests: int, max_length: int = None, page_size: int = 64, device="cuda"):
+        head_dim = cfg.n_embd // cfg.n_head
+        max_length = cfg.sequence_length if max_length is None else max_length
+        assert page_size <= max_length <= cfg.sequence_length, "whole pages, up to the end of the rotary table"
+        self.page_size, self.num_pages = page_size, num_pages
+        self.k, self.v = ([torch.zeros(num_pages, page_size, cfg.n_head, head_dim, dtype=torch.bfloat16, device=device)
+                           for _ in range(cfg.n_layer)] for _ in range(2))
+        # whole pages would let a request grow beyond max_length by part of a page: the table has only full ones
+        self.page_table = torch.zeros(max_requests, max(1, max_length // page_size), dtype=torch.int32, device=device)
+        self.free_pages = torch.arange(num_pages, dtype=torch.int32, device=device)
+        self.free_count = torch.full((1,), num_pages, dtype=torch.int32, device=device)
+        self.lens = torch.zeros(max_requests, dtype=torch.int32, device=device)
+
+    def assign(self, new_lens: torch.Tensor, num_tokens: int) -> PageStep:
+        """Room for ``new_lens[b]`` more tokens of every request; requests without room are refused (``page_assign``)."""
+        step = quest.page_assign(self.page_table, self.free_pages, self.free_count, self.lens, new_lens, num_tokens, self.page_size)
+        self.lens.copy_(step.lens)
+        self.free_count.copy_(step.free_count)
+        return step
+
+    def shorten(self, keep_lens: torch.Tensor) -> None:
+        """Request b keeps its first ``keep_lens[b]`` tokens (0: it has finished and its place can be used again)."""
+        keep = torch.minimum(keep_lens, self.lens)
+        self.free_count.copy_(quest.page_release(self.page_table, self.free_pages, self.free_count, self.lens, keep, self.page_size))
+        self.lens.copy_(keep)
+
+    def layers(self, step: PageStep) -> list[LayerPages]:
+        return [LayerPages(k, v, self.page_table, step) for k, v in zip(self.k, self.v)]
+
+
+@torch.inference_mode()
+def extend(model: Decoder, cache: PagedCache, tokens: torch.Tensor, new_lens: torch.Tensor) -> tuple[torch.Tensor, PageStep]:
+    """Runs ``tokens`` [rows], the new tokens of the requests packed one after the other (``new_lens`` [max_requests] int32 of
+    them; rows behind the last are padding), through the model.  Returns (hidden states [rows, n_embd], step).  Nothing is
+    read on the host: a step of fixed size can be captured in a graph and replayed."""
+    step = cache.assign(new_lens, tokens.numel())
+    return model(tokens.view(1, -1), cache.layers(step))[0], step
+
+
+def last_rows(step: PageStep) -> torch.Tensor:
+    """Row of each request's last new token (0 where it has none)."""
+    return (step.cu_new[1:] - 1).clamp(min=0).long()
+
+
+@torch.inference_mode()
+def generate(model: Decoder, cache: PagedCache, prompts: list[torch.Tensor], max_new: int) -> torch.Tensor:
+    """Greedy continuation of the prompts (1-D token ids, at most ``max_requests``): [len(prompts), max_new].  The requests take the
+    first places of the cache, which must be free, and give their pages back at the end."""
+    slots, n = cache.lens.numel(), len(prompts)
+    device = cache.lens.device
+    if n > slots or any(p.numel() == 0 for p in prompts):
+        raise ValueError("more prompts than places, or an empty prompt")
+    longest = max(p.numel() for p in prompts) + max_new
+    if longest > cache.page_table.size(1) * cache.page_size or sum(-(-(p.numel() + max_new) // cache.page_size) for p in prompts) > cache.num_pages:
+        raise ValueError("the cache has too few pages for these prompts and their continuation")
+    if bool((cache.lens[:n] != 0).any()):
+        raise ValueError("places of the cache are in use")
+    new = torch.zeros(slots, dtype=torch.int32, device=device)
+    new[:n] = torch.tensor([p.numel() for p in prompts], dtype=torch.int32, device=device)
+    hidden, step = extend(model, cache, torch.cat([p.to(device) for p in prompts]), new)
+    new[:n] = 1
+    result = []
+    for i in range(max_new):
+        token = model.lm_head(hidden[last_rows(step)[:n]]).argmax(dim=-1)
+        result.append(token)
+        if i + 1 < max_new:
+            hidden, step = extend(model, cache, token, new)
+    keep = cache.lens.clone()
+    keep[:n] = 0
+    cache.shorten(keep)
+    return torch.stack(result, dim=1) if result else torch.empty(n, 0, dtype=torch.long, device=device)
+
+
+@torch.inference_mode()
+def verify(model: Decoder, cache: PagedCache, tokens: torch.Tensor, drafts: torch.Tensor, uniforms: torch.Tensor,
+           draft_probs: torch.Tensor = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """One step of speculative decoding for all places of the cache: ``tokens`` [R], the last token of each request, which is not
+    in the cache yet, and ``drafts`` [R, K] drafted behind it run through the model in one pass, drafts that the target refuses are taken
+    out of the cache again.  ``uniforms`` [R, K + 1] fp32 in [0, 1); ``draft_probs`` [R, K, vocab] fp32.  Returns (new tokens
+    [R, K + 1], -1 behind the last one; drafts kept [R]); the last new token is the next call's ``tokens``."""
+    requests, count = drafts.shape
+    device = cache.lens.device
+    before = cache.lens.clone()
+    new = torch.full((requests,), count + 1, dtype=torch.int32, device=device)
+    hidden, _ = extend(model, cache, torch.cat([tokens[:, None], drafts], dim=1).view(-1), new)
+    probs = torch.softmax(model.lm_head(hidden).float(), dim=-1)
+    cu = torch.arange(0, (requests + 1) * count, max(count, 1), dtype=torch.int32, device=device)[:requests + 1] if count else torch.zeros(requests + 1, dtype=torch.int32, device=device)
+    result, kept = quest.verify_drafts(probs, drafts.reshape(-1), cu, uniforms.reshape(-1), count,
+                                       draft_probs=None if draft_probs is None else draft_probs.reshape(requests * count, -1))
+    cache.shorten(before + 1 + kept)
+    return result, kept

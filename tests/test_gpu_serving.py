@@ -1,0 +1,203 @@
+"""The decoder over a paged cache: against its own forward pass over whole sequences, and the loops around it."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from quest_b200 import serving
+from quest_b200.prefill import Decoder, DecoderConfig, swap_linears
+
+pytestmark = pytest.mark.gpu
+
+CFG = DecoderConfig(n_embd=512, n_layer=2, n_head=4, ffn=768, vocab_size=300, sequence_length=256)
+
+
+def make_model(mode, seed=0):
+    with torch.random.fork_rng(devices=[0]):
+        torch.manual_seed(seed)
+        with torch.device("cuda"):
+            model = Decoder(CFG).to(torch.bfloat16).eval()
+            for p in model.parameters():  # livelier than the initialisation for training, so that attention matters
+                if p.dim() > 1:
+                    p.data.mul_(3)
+    return swap_linears(model, mode) if mode != "bf16" else model
+
+
+def prompts_of(lengths, seed=1):
+    g = torch.Generator().manual_seed(seed)
+    return [torch.randint(0, CFG.vocab_size, (n,), generator=g) for n in lengths]
+
+
+def relative(a, b):
+    return ((a.double() - b.double()).norm() / b.double().norm()).item()
+
+
+@pytest.mark.parametrize("page_size", [16, 64])
+def test_paged_forward_equals_the_forward_of_whole_sequences(page_size):
+    """bf16 linears: both passes round at the same places but for the attention (its probabilities to bf16) and the rotary
+    embedding; each bf16 rounding is 2^-9 of a value on average, and two layers have about ten of them in line."""
+    model = make_model("bf16")
+    prompts = prompts_of([1, 17, 128, 200])
+    cache = serving.PagedCache(CFG, 64, 5, page_size=page_size)
+    new = torch.tensor([p.numel() for p in prompts] + [0], dtype=torch.int32, device="cuda")
+    with torch.inference_mode():
+        hidden, step = serving.extend(model, cache, torch.cat(prompts).cuda(), new)
+        whole = [model(p.cuda()[None])[0] for p in prompts]
+    assert step.kv_lens.tolist() == [1, 17, 128, 200, 0] and cache.lens.tolist() == [1, 17, 128, 200, 0]
+    for b, w in enumerate(whole):
+        assert relative(hidden[step.cu_new[b]:step.cu_new[b + 1]], w) < 10 * 2 ** -9
+
+
+@pytest.mark.parametrize("mode", ["bf16", "int4", "int4_fused"])
+def test_chunks_and_single_tokens_equal_one_pass_over_the_cache(mode):
+    """The same tokens in one step, or as chunks and single tokens: rows of the linears do not depend on one another, the attention
+    sums in another order.  With int4 activations a value at a border can change its code, so only the bulk is compared."""
+    model = make_model(mode)
+    prompts = prompts_of([90, 33])
+    whole = serving.PagedCache(CFG, 16, 2, page_size=16)
+    new = torch.tensor([90, 33], dtype=torch.int32, device="cuda")
+    hidden, step = serving.extend(model, whole, torch.cat(prompts).cuda(), new)
+    parts = serving.PagedCache(CFG, 16, 2, page_size=16)
+    got = [[], []]
+    at = [0, 0]
+    for counts in ([50, 1], [1, 20], [38, 0], [1, 12]):
+        x = torch.cat([p[a:a + c] for p, a, c in zip(prompts, at, counts)]).cuda()
+        h, s = serving.extend(model, parts, x, torch.tensor(counts, dtype=torch.int32, device="cuda"))
+        for b in range(2):
+            got[b].append(h[s.cu_new[b]:s.cu_new[b + 1]])
+            at[b] += counts[b]
+    assert parts.lens.tolist() == [90, 33] == whole.lens.tolist() and parts.free_count.item() == whole.free_count.item()
+    for b in range(2):
+        a, w = torch.cat(got[b]), hidden[step.cu_new[b]:step.cu_new[b + 1]]
+        assert relative(a, w) < (10 * 2 ** -9 if mode == "bf16" else 0.35)
+
+
+@pytest.mark.parametrize("mode", ["bf16", "int4_fused"])
+def test_padding_rows_are_zero_and_change_nothing(mode):
+    model = make_model(mode)
+    prompt = prompts_of([40])[0].cuda()
+    new = torch.tensor([40, 0], dtype=torch.int32, device="cuda")
+    a, _ = serving.extend(model, serving.PagedCache(CFG, 8, 2, page_size=16), prompt, new)
+    b, _ = serving.extend(model, serving.PagedCache(CFG, 8, 2, page_size=16), torch.cat([prompt, prompt[:9]]), new)
+    assert torch.isfinite(b).all()
+    if mode == "bf16":
+        assert relative(b[:40], a) < 10 * 2 ** -9
+
+
+def test_generate_equals_the_loop_without_a_cache():
+    """Greedy tokens of the same model by whole forward passes; where its two best logits are closer than the rounding of bf16
+    may move them, the sequence may part, so each step's choice is compared under the tokens chosen by generate."""
+    model = make_model("bf16")
+    prompts = prompts_of([3, 30, 64])
+    cache = serving.PagedCache(CFG, 24, 4, page_size=16)
+    got = serving.generate(model, cache, prompts, 20)
+    assert got.shape == (3, 20) and cache.free_count.item() == 24 and cache.lens.tolist() == [0] * 4
+    with torch.inference_mode():
+        for b, p in enumerate(prompts):
+            sequence = torch.cat([p.cuda(), got[b]])
+            logits = model.lm_head(model(sequence[None])[0]).float()[p.numel() - 1:-1]
+            chosen = logits.gather(1, got[b][:, None])[:, 0]
+            assert (logits.amax(dim=1) - chosen <= 20 * 2 ** -9 * logits.abs().amax(dim=1)).all()
+    again = serving.generate(model, cache, prompts, 20)  # pages are used again, in another order
+    assert torch.equal(again, got)
+
+
+def test_generate_refuses_what_does_not_fit():
+    model = make_model("bf16")
+    cache = serving.PagedCache(CFG, 4, 2, page_size=16)
+    with pytest.raises(ValueError):
+        serving.generate(model, cache, prompts_of([1, 1, 1]), 1)
+    with pytest.raises(ValueError):
+        serving.generate(model, cache, prompts_of([40, 40]), 1)
+    with pytest.raises(ValueError):
+        serving.generate(model, cache, [torch.empty(0, dtype=torch.long)], 1)
+    with pytest.raises(AssertionError):
+        serving.PagedCache(CFG, 4, 2, max_length=257)
+
+
+def test_decoding_step_in_a_graph():
+    """A captured step replayed token after token gives what eager steps give."""
+    model = make_model("int4_fused")
+    prompts = prompts_of([20, 35])
+    new = torch.tensor([20, 35], dtype=torch.int32, device="cuda")
+    one = torch.ones(2, dtype=torch.int32, device="cuda")
+    tokens = prompts_of([2], seed=5)[0].cuda()
+    feed = [prompts_of([2], seed=s)[0].cuda() for s in range(6, 12)]
+
+    def run(graphed):
+        cache = serving.PagedCache(CFG, 16, 2, page_size=16)
+        serving.extend(model, cache, torch.cat(prompts).cuda(), new)
+        held = torch.empty_like(tokens)
+        if graphed:
+            side = torch.cuda.Stream()
+            side.wait_stream(torch.cuda.current_stream())
+            state = [t.clone() for t in (cache.lens, cache.free_count, cache.page_table)]
+            with torch.cuda.stream(side):
+                held.copy_(tokens)
+                serving.extend(model, cache, held, one)
+            torch.cuda.current_stream().wait_stream(side)
+            for t, x in zip((cache.lens, cache.free_count, cache.page_table), state):
+                t.copy_(x)
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                hidden, _ = serving.extend(model, cache, held, one)
+        out = []
+        for x in feed:
+            held.copy_(x)
+            if graphed:
+                graph.replay()
+                out.append(hidden.clone())
+            else:
+                out.append(serving.extend(model, cache, held, one)[0])
+        return torch.stack(out), cache.lens.tolist()
+
+    eager, lens = run(False)
+    graphed, lens_g = run(True)
+    assert lens == lens_g == [26, 41] and torch.equal(eager, graphed)
+
+
+@pytest.mark.parametrize("count", [0, 1, 4])
+def test_verify_takes_refused_drafts_out_again(count):
+    """Drafts that are the target's own greedy tokens under a sharpened model are kept, others refused; the cache afterwards holds
+    exactly the kept ones, whatever was written."""
+    model = make_model("bf16")
+    model.lm_head.weight.data.mul_(200)  # nearly all probability on one token
+    prompts = prompts_of([10, 25])
+    cache = serving.PagedCache(CFG, 16, 2, page_size=16)
+    serving.extend(model, cache, torch.cat(prompts).cuda(), torch.tensor([10, 25], dtype=torch.int32, device="cuda"))
+    reference = serving.PagedCache(CFG, 16, 2, page_size=16)
+    last = torch.tensor([7, 11], device="cuda")
+    chain = serving.generate(model, reference, [torch.cat([p, t.cpu()[None]]) for p, t in zip(prompts, last)], max(count, 1))
+    drafts = chain[:, :count].clone()
+    if count:
+        drafts[1, count // 2] = (drafts[1, count // 2] + 1) % CFG.vocab_size  # the second request's drafts go wrong there
+    u = torch.full((2, count + 1), 0.5, device="cuda")
+    free = cache.free_count.item()
+    tokens, kept = serving.verify(model, cache, last, drafts, u)
+    assert kept.tolist() == ([count, count // 2] if count else [0, 0])
+    assert cache.lens.tolist() == [10 + 1 + kept[0].item(), 25 + 1 + kept[1].item()]
+    held = sum(-(-n // 16) for n in cache.lens.tolist())
+    assert cache.free_count.item() == 16 - held and free >= cache.free_count.item()
+    assert sorted(cache.free_pages[:16 - held].tolist() + cache.page_table[0, :-(-cache.lens[0].item() // 16)].tolist()
+                  + cache.page_table[1, :-(-cache.lens[1].item() // 16)].tolist()) == list(range(16))
+    if count:
+        assert tokens[0, :count].tolist() == drafts[0].tolist() and tokens[1, kept[1].item()].item() == chain[1, count // 2].item()
+    # the next step attends over the kept tokens: the same as a cache that never saw the refused ones
+    clean = serving.PagedCache(CFG, 16, 2, page_size=16)
+    sequences = [torch.cat([p.cuda(), last[b:b + 1], drafts[b, :kept[b]]]) for b, p in enumerate(prompts)]
+    serving.extend(model, clean, torch.cat(sequences), torch.tensor([s.numel() for s in sequences], dtype=torch.int32, device="cuda"))
+    one = torch.ones(2, dtype=torch.int32, device="cuda")
+    a, _ = serving.extend(model, cache, last, one)
+    b, _ = serving.extend(model, clean, last, one)
+    assert relative(a, b) < 10 * 2 ** -9
+
+
+def test_requests_without_pages_are_refused_and_recover():
+    model = make_model("bf16")
+    cache = serving.PagedCache(CFG, 3, 2, page_size=16)
+    _, step = serving.extend(model, cache, prompts_of([60])[0].cuda(), torch.tensor([30, 30], dtype=torch.int32, device="cuda"))
+    assert step.kv_lens.tolist() == [30, 0] and cache.lens.tolist() == [30, 0] and cache.free_count.item() == 1
+    cache.shorten(torch.zeros(2, dtype=torch.int32, device="cuda"))
+    assert cache.free_count.item() == 3
+    _, step = serving.extend(model, cache, prompts_of([30])[0].cuda(), torch.tensor([0, 30], dtype=torch.int32, device="cuda"))
+    assert step.kv_lens.tolist() == [0, 30]
