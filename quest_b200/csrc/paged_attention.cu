@@ -30,7 +30,7 @@ constexpr int BM = 128, BN = 128, HN = BN / 2;  // rows of a stream, keys of a s
 constexpr int kThreads = 384;
 constexpr int kCopyWarp0 = 0, kMmaWarp0 = 1, kMmaWarp1 = 2, kCopyWarp1 = 3, kFirstSoftmax = 4;
 constexpr int ITEMS = 4;                            // descriptors in flight on each list
-constexpr int kControlRegs = 88, kSoftmaxRegs = 208;  // 128 x 88 + 256 x 208 = 384 x 168, what the block is launched with
+constexpr int kControlRegs = 72, kSoftmaxRegs = 216;  // 128 x 72 + 256 x 216 = 384 x 168, what the block is launched with
 static_assert(128 * kControlRegs + 256 * kSoftmaxRegs <= kThreads * 168, "register shares exceed the launch");
 constexpr int kItemCost = 1;                        // steps that an item's queries and result are worth in the lines
 
@@ -41,10 +41,9 @@ struct Cfg {
     static constexpr int STAGE_BYTES = 2 * SLOT_BYTES;    // that of a pair stages of 128
     static constexpr int STAGES = D == 128 ? 5 : 10;      // stages of the pair's ring = slots of each stream's
     static constexpr int HALVES = D / 64;
-    // barriers: pair ring, slots; queries, scores, probabilities (of half a step), outputs, each of the pair's streams and of single
-    // ones; three lists; ends
+    // barriers: pair ring, slots; queries, scores, probabilities, outputs (of the pair's streams, of single ones); three lists; ends
     static constexpr int PAIR_FULL = 0, PAIR_EMPTY = PAIR_FULL + STAGES, SLOT_FULL = PAIR_EMPTY + STAGES, SLOT_EMPTY = SLOT_FULL + 2 * STAGES,
-                         Q_FULL = SLOT_EMPTY + 2 * STAGES, Q_EMPTY = Q_FULL + 4, S_FULL = Q_EMPTY + 4, P_FULL = S_FULL + 4, O_FULL = P_FULL + 8,
+                         Q_FULL = SLOT_EMPTY + 2 * STAGES, Q_EMPTY = Q_FULL + 4, S_FULL = Q_EMPTY + 4, P_FULL = S_FULL + 4, O_FULL = P_FULL + 4,
                          LIST_FULL = O_FULL + 4, LIST_EMPTY = LIST_FULL + 3 * ITEMS, PAIRS_DONE = LIST_EMPTY + 3 * ITEMS, DONE = PAIRS_DONE + 1,
                          NUM_BARS = DONE + 2;
     static constexpr int SMEM = 1024 + 2 * Q_BYTES + STAGES * STAGE_BYTES + NUM_BARS * 8 + 16 + 3 * ITEMS * 64;
@@ -63,7 +62,7 @@ struct Params {
     int* headers;     // 4 per block: for each worker the item that begins there and goes on
     long long o_token, o_head;
     float c;          // scale log2(e)
-    int rows, batch, width, hkv, group, tokens /* of a stream's tile */, num_pages, page, page_shift, slot_rows, wide_stores;
+    int rows, batch, width, hkv, group, tokens /* of a stream's tile */, half_tokens /* of half a tile */, num_pages, page, page_shift, slot_rows, wide_stores;
 };
 
 // One item, or the piece of it that a worker (the pair, or a single stream) has.
@@ -219,14 +218,6 @@ __device__ __forceinline__ void store_row32(__nv_bfloat16* dst, const uint32_t (
     }
 }
 
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};"
-        ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
-          "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
-        : "memory");
-}
-
 // What the softmax warps of a stream keep of an item: the reference maximum and the sum of the thread's row.
 struct RowState {
     float m, l;  // m in units of the scores; -inf: nothing seen
@@ -234,8 +225,7 @@ struct RowState {
 
 // One step of a row: scores in tensor memory -> probabilities over them.  `seen` keys of this step are visible to the row.
 template <int D>
-__device__ __forceinline__ void softmax_step(RowState& st, const uint32_t s_addr, const uint32_t o_addr, const int seen, const bool live, const bool first, const float c,
-                                             const uint32_t p_full) {
+__device__ __forceinline__ void softmax_step(RowState& st, const uint32_t s_addr, const uint32_t o_addr, const int seen, const bool live, const bool first, const float c) {
     uint32_t s[4][32];
 #pragma unroll
     for (int i = 0; i < 4; ++i) tmem_ld32(s_addr + 32 * i, s[i]);
@@ -278,34 +268,24 @@ __device__ __forceinline__ void softmax_step(RowState& st, const uint32_t s_addr
     const uint64_t c2 = pack2(c, c), off2 = pack2(off, off);
     uint64_t sum[2] = {0, 0};
 #pragma unroll
-    for (int part = 0; part < 4; ++part) {
-        uint32_t pk[16];
+    for (int half = 0; half < 2; ++half) {
+        uint32_t pk[32];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const uint64_t x = fma2(pack2(__uint_as_float(s[part][2 * i]), __uint_as_float(s[part][2 * i + 1])), c2, off2);
+        for (int i = 0; i < 32; ++i) {
+            const int e = half * 64 + 2 * i;
+            const uint64_t x = fma2(pack2(__uint_as_float(s[e / 32][e % 32]), __uint_as_float(s[e / 32][e % 32 + 1])), c2, off2);
             float x0, x1;
             unpack2(x, x0, x1);
             x0 = ex2(x0), x1 = ex2(x1);
             sum[i & 1] = add2(sum[i & 1], pack2(x0, x1));
             pk[i] = pack_bf16x2(x0, x1);
         }
-        // The product over the first 64 keys begins while the rest is worked on; its probabilities have arrived in tensor memory by
-        // the time that the third quarter is computed, so the wait costs nothing.
-        if (part == 2) {
-            tmem_st_wait();
-            tc_fence_before();
-            __syncwarp();
-            if ((threadIdx.x & 31) == 0) mbar_arrive(p_full);
-        }
-        tmem_st16(s_addr + part * 16, pk);
+        tmem_st32(s_addr + half * 32, pk);
     }
-    tmem_st_wait();
-    tc_fence_before();
-    __syncwarp();
-    if ((threadIdx.x & 31) == 0) mbar_arrive(p_full + 8);
     float a, b;
     unpack2(add2(sum[0], sum[1]), a, b);
     st.l += a + b;
+    tmem_st_wait();
 }
 
 // A worker's place in a line: from u to end, beginning in request b `rest` places behind the request's first.
@@ -317,7 +297,7 @@ struct Place {
 
 template <int D>
 __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Params p, const __grid_constant__ CUtensorMap qmap,
-                                                                      const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
+                                                                      const __grid_constant__ CUtensorMap hqmap, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
     using C = Cfg<D>;
     extern __shared__ uint8_t raw[];
     const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
@@ -333,11 +313,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
     if (warp == kMmaWarp0) {
         tmem_alloc(smem_u32(tmem_slot), 512);
         tmem_relinquish();
-    } else if (warp == kCopyWarp0 && lane == 0) {
-        tma_prefetch_desc(&qmap), tma_prefetch_desc(&kmap), tma_prefetch_desc(&vmap);
-        for (int i = 0; i < C::NUM_BARS; ++i) {
+    } else if (warp == kCopyWarp0) {
+        if (lane == 0) tma_prefetch_desc(&qmap), tma_prefetch_desc(&hqmap), tma_prefetch_desc(&kmap), tma_prefetch_desc(&vmap);
+        for (int i = lane; i < C::NUM_BARS; i += 32) {
             int count = 1;
-            if (i >= C::P_FULL && i < C::P_FULL + 8) count = 4;                   // four warps of a stream
+            if (i >= C::P_FULL && i < C::P_FULL + 4) count = 4;                   // four warps of a stream
             if (i >= C::LIST_EMPTY && i < C::LIST_EMPTY + ITEMS) count = 10;      // MMA warp, copier of the queries, eight softmax warps
             if (i >= C::LIST_EMPTY + ITEMS && i < C::LIST_EMPTY + 3 * ITEMS) count = 5;  // MMA warp, four softmax warps
             mbar_init(bar(i), count);
@@ -424,19 +404,22 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
     } else if (warp >= kFirstSoftmax) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
         // ------------------------------ softmax, results ------------------------------
-        const int s = (warp - kFirstSoftmax) >> 2, quad = warp & 3, row = quad * 32 + lane;  // this thread's row of its stream
+        const int s = (warp - kFirstSoftmax) >> 2, quad = warp & 3, lane_row = quad * 32 + lane;  // this thread's row of its stream
         const uint32_t lanes = (uint32_t)(quad * 32) << 16;
         const uint32_t s_addr = tmem + C::S_COL + 128 * s + lanes, o_addr = tmem + C::O_COL + D * s + lanes;
-        const int tile_rows = p.tokens * p.group, row_token = row / p.group, row_head = row - row_token * p.group;
+        const int tile_rows = p.tokens * p.group;
         for (int turn = has_pairs ? 0 : 1; turn < 2; ++turn) {  // the pairs, then the items of this stream alone
             const int list = turn == 0 ? 0 : 1 + s;
             if (!ok || places[list].b < 0) break;
-            const uint32_t s_full = bar(C::S_FULL + 2 * turn + s), p_full = bar(C::P_FULL + 4 * turn + 2 * s), o_full = bar(C::O_FULL + 2 * turn + s);
+            const uint32_t s_full = bar(C::S_FULL + 2 * turn + s), p_full = bar(C::P_FULL + 2 * turn + s), o_full = bar(C::O_FULL + 2 * turn + s);
             uint32_t s_ph = 0, o_ph = 0;
             Item d;
             for (uint32_t it = 0; take(list, it, d);) {
-                const int steps = d.steps[s], tok0 = d.tok0 + (list == 0 ? s * p.tokens : 0), token = tok0 + row_token;
-                const bool live = row < tile_rows && token < d.n;
+                const int steps = d.steps[s], tok0 = d.tok0 + (list == 0 ? s * p.tokens : 0);
+                // Where few rows are there the second stream's lie in the other two quadrants: its warps run on other parts of the SM.
+                const int row = lane_row - (list > 0 && s == 1 && d.n - tok0 <= p.half_tokens ? BM / 2 : 0);
+                const int row_token = row >= 0 ? row / p.group : 0, row_head = row - row_token * p.group, token = tok0 + row_token;
+                const bool live = row >= 0 && row < tile_rows && token < d.n;
                 const bool warp_live = __any_sync(~0u, live);
                 const int keys = live ? min(max(d.kv - d.n + token + 1, 0), d.kv) : 0x7fffffff;  // a row that is not there needs no mask
                 RowState rs{-CUDART_INF_F, 0.f};
@@ -445,11 +428,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
                     if (!ok) break;
                     s_ph ^= 1u;
                     tc_fence_after();
-                    if (warp_live) {
-                        softmax_step<D>(rs, s_addr, o_addr, keys - (d.t0 + i) * BN, live, i == 0, p.c, p_full);
-                    } else if (lane == 0) {
-                        mbar_arrive(p_full), mbar_arrive(p_full + 8);
-                    }
+                    if (warp_live) softmax_step<D>(rs, s_addr, o_addr, keys - (d.t0 + i) * BN, live, i == 0, p.c);
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(p_full);
                 }
                 if (steps > 0) {
                     ok = __all_sync(~0u, ok && wait_bar(o_full, o_ph, 80));
@@ -476,7 +458,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
                 } else {
                     const bool nothing = steps == 0;  // the first stream's rows see nothing of this piece
                     float* const slot = p.partial + (long long)(d.slot + (list == 0 ? 2 * blocks * s : 0)) * p.slot_rows * (D + 2);
-                    const bool mine = row < p.slot_rows;
+                    const bool mine = row >= 0 && row < p.slot_rows;
                     if (mine) {
                         slot[p.slot_rows * D + row] = rs.m == -CUDART_INF_F ? -CUDART_INF_F : rs.m * p.c;
                         slot[p.slot_rows * (D + 1) + row] = l;
@@ -515,14 +497,15 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
                 }
                 __syncwarp();
             };
-            auto load_queries = [&](int tile, int set, uint32_t& ph, int token, int hk) {
+            auto load_queries = [&](int tile, int set, uint32_t& ph, int token, int hk, bool upper) {
                 const uint32_t full = bar(C::Q_FULL + 2 * set + tile);
                 ok = __all_sync(~0u, ok && wait_bar(bar(C::Q_EMPTY + 2 * set + tile), ph ^ 1u, 74));
                 ph ^= 1u;
                 if (ok && lane == 0) {
-                    mbar_arrive_expect_tx(full, p.tokens * p.group * D * 2);
+                    mbar_arrive_expect_tx(full, (upper ? p.half_tokens : p.tokens) * p.group * D * 2);
                     for (int h = 0; h < C::HALVES; ++h)
-                        tma_load_3d(q_smem + tile * C::Q_BYTES + h * (BM * 128), &qmap, 64 * h, hk * p.group, token, full);
+                        tma_load_3d(q_smem + tile * C::Q_BYTES + h * (BM * 128) + (upper ? BM / 2 * 128 : 0), upper ? &hqmap : &qmap, 64 * h,
+                                    hk * p.group, token, full);
                 }
                 __syncwarp();
             };
@@ -611,8 +594,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
                 uint32_t q_ph[2] = {0, 0};
                 Item d;
                 for (uint32_t it = 0; take(0, it, d);) {
-                    if (d.steps[0] > 0) load_queries(0, 0, q_ph[0], d.start + d.tok0, d.hk);
-                    load_queries(1, 0, q_ph[1], d.start + d.tok0 + p.tokens, d.hk);
+                    if (d.steps[0] > 0) load_queries(0, 0, q_ph[0], d.start + d.tok0, d.hk, false);
+                    load_queries(1, 0, q_ph[1], d.start + d.tok0 + p.tokens, d.hk, false);
                 }
             }
             const Place w = places[1 + s];
@@ -660,7 +643,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
                         for (int step = d.t0; ok && step < t1; ++step) {
                             if (step + 2 < t1) ids[2] = page_at(d, step + 2);
                             load(&kmap, d, step, ids[0]);
-                            if (step == d.t0) load_queries(s, 1, q_ph, d.start + d.tok0, d.hk);
+                            if (step == d.t0) load_queries(s, 1, q_ph, d.start + d.tok0, d.hk, s == 1 && d.n - d.tok0 <= p.half_tokens);
                             load(&vmap, d, step, ids[0]);
                             ids[0] = ids[1], ids[1] = ids[2];
                         }
@@ -690,6 +673,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
             // All lanes walk the loops on values that the compiler knows to be the same in all of them (see elect_one).
             const int s = warp == kMmaWarp1;
             const uint64_t q_desc = make_smem_desc(q_smem);
+            uint32_t q_ph[2] = {0, 0}, p_ph[2] = {0, 0};
             auto wait_in = [&](int barrier, uint32_t ph, int where) { ok = __all_sync(~0u, ok && wait_bar(bar(barrier), ph, where)); };
             auto commit = [&](int barrier) {
                 if (ok && elect_one()) umma_commit(bar(barrier));
@@ -698,8 +682,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
             auto take_uniform = [&](int list, uint32_t& it, Item& d) {
                 Item x;
                 const bool more = take(list, it, x);
-                d.kv = __reduce_max_sync(~0u, x.kv), d.t0 = __reduce_max_sync(~0u, x.t0);
-                d.steps[0] = __reduce_max_sync(~0u, x.steps[0]), d.steps[1] = __reduce_max_sync(~0u, x.steps[1]);
+                d.n = __shfl_sync(~0u, x.n, 0), d.kv = __shfl_sync(~0u, x.kv, 0), d.t0 = __shfl_sync(~0u, x.t0, 0);
+                d.steps[0] = __shfl_sync(~0u, x.steps[0], 0), d.steps[1] = __shfl_sync(~0u, x.steps[1], 0);
                 return __all_sync(~0u, more) != 0;
             };
             // Rows of the last page behind the request's tokens hold anything; a zero weight does not make a NaN harmless.
@@ -716,30 +700,19 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
                 fence_proxy_async_smem();
                 __syncwarp();
             };
-            // O += P V of stream t over 64 keys: their probabilities are there first, those of the step's second half while this runs.
-            auto values = [&](int t, int p_full, uint32_t p_ph, int half, uint64_t b, uint32_t accumulate) {
-                wait_in(p_full, p_ph, 82);
-                tc_fence_after();
-                const uint32_t o_col = tmem + C::O_COL + D * t, p_col = tmem + C::S_COL + 128 * t + 32 * half;
-                if (ok && elect_one()) {
-                    umma_bf16_ts(o_col, p_col, b, C::IDESC_O, accumulate);
-#pragma unroll
-                    for (int k = 1; k < HN / 16; ++k) umma_bf16_ts(o_col, p_col + 8 * k, b + k * (2048 >> 4), C::IDESC_O, 1u);
-                }
-                __syncwarp();
-            };
             if (has_pairs && s == 0) {
-                // One warp issues for both streams, each time the values of a step and the scores of the next one: issued by a warp
-                // of their own the streams' products ran interleaved and all of them late (chunk of 4096 behind 28672: 4.2 against 3.4 ms).
                 struct Stage {
                     uint32_t at, ph;
                     __device__ __forceinline__ Stage next() const { return at + 1 == C::STAGES ? Stage{0, ph ^ 1u} : Stage{at + 1, ph}; }
                 };
                 const uint64_t k_desc = make_smem_desc(ring), v_desc = make_mn_desc(ring, BN * 128);
                 Stage next{0, 0};  // the next stage of the ring in the order of the copies
-                uint32_t q_ph[2] = {0, 0}, p_ph[2] = {0, 0};
-                auto wait_stage = [&](const Stage& g) { wait_in(C::PAIR_FULL + g.at, g.ph, 83); };
-                auto scores = [&](int t, const Stage& g, bool last) {  // S = Q K^T of stream t; the last of an item frees its queries
+                auto wait_q = [&](int t) { wait_in(C::Q_FULL + t, q_ph[t], 81), q_ph[t] ^= 1u; };
+                auto wait_p = [&](int t) {
+                    wait_in(C::P_FULL + t, p_ph[t], 82), p_ph[t] ^= 1u;
+                    tc_fence_after();
+                };
+                auto scores = [&](int t, const Stage& g) {  // S = Q K^T of stream t
                     const uint64_t a = q_desc + (uint64_t)(t * (C::Q_BYTES >> 4)), b = k_desc + (uint64_t)(g.at * (C::STAGE_BYTES >> 4));
                     if (ok && elect_one()) {
 #pragma unroll
@@ -750,50 +723,56 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
                         umma_commit(bar(C::S_FULL + t));
                     }
                     __syncwarp();
-                    if (last) commit(C::Q_EMPTY + t);
                 };
-                auto first_scores = [&](int t, const Stage& g, int n) {
-                    wait_in(C::Q_FULL + t, q_ph[t], 81), q_ph[t] ^= 1u;
-                    scores(t, g, n == 1);
-                };
-                auto step_values = [&](int t, const Stage& g, bool accumulate) {
+                auto values = [&](int t, const Stage& g, uint32_t accumulate) {  // O += P V
                     const uint64_t b = v_desc + (uint64_t)(g.at * (C::STAGE_BYTES >> 4));
-                    values(t, C::P_FULL + 2 * t, p_ph[t], 0, b, accumulate);
-                    values(t, C::P_FULL + 2 * t + 1, p_ph[t], 1, b + (HN * 128 >> 4), 1u);
-                    p_ph[t] ^= 1u;
+                    if (ok && elect_one()) {
+                        umma_bf16_ts(tmem + C::O_COL + D * t, tmem + C::S_COL + 128 * t, b, C::IDESC_O, accumulate);
+#pragma unroll
+                        for (int k = 1; k < BN / 16; ++k)
+                            umma_bf16_ts(tmem + C::O_COL + D * t, tmem + C::S_COL + 128 * t + 8 * k, b + k * (2048 >> 4), C::IDESC_O, 1u);
+                    }
+                    __syncwarp();
                 };
                 Item d;
-                uint32_t it = 0;
-                bool more_items = take_uniform(0, it, d);
-                if (more_items) {  // the place can be too small for a step
-                    wait_stage(next);
-                    if (d.steps[0] > 0) first_scores(0, next, d.steps[0]);
-                    first_scores(1, next, d.steps[1]);
+                for (uint32_t it = 0; take_uniform(0, it, d);) {
+                    const int n0 = d.steps[0], n1 = d.steps[1];
+                    wait_in(C::PAIR_FULL + next.at, next.ph, 83);
+                    if (n0 > 0) {
+                        wait_q(0);
+                        scores(0, next);
+                        if (n0 == 1) commit(C::Q_EMPTY);
+                    }
+                    wait_q(1);
+                    scores(1, next);
+                    if (n1 == 1) commit(C::Q_EMPTY + 1);
                     commit(C::PAIR_EMPTY + next.at);
                     next = next.next();
-                }
-                while (ok && more_items) {
-                    const int n0 = d.steps[0], n1 = d.steps[1], t0 = d.t0, kv = d.kv;
-                    for (int i = 0; ok && i < n1; ++i) {
-                        // the next keys (of the next item behind this one's last step), and these values before or behind them
+                    for (int i = 0; i < n1; ++i) {
+                        // the next keys, and these values behind them
                         const bool more = i + 1 < n1;
-                        const Stage keys = more ? next : next.next(), vals = more ? next.next() : next;
-                        next = next.next().next();
-                        wait_stage(vals);
-                        clean(ring + vals.at * C::STAGE_BYTES, (t0 + i) * BN, BN, kv);
-                        if (i < n0) step_values(0, vals, i > 0);
-                        if (i + 1 == n0) commit(C::O_FULL);
-                        if (!more) more_items = take_uniform(0, it, d);
-                        const bool go_on = more || more_items;
-                        if (go_on) wait_stage(keys);
-                        if (more && i + 1 < n0) scores(0, keys, i + 2 == n0);
-                        if (!more && more_items && d.steps[0] > 0) first_scores(0, keys, d.steps[0]);
-                        step_values(1, vals, i > 0);
+                        const Stage keys = next, vals = more ? next.next() : next;
+                        next = vals.next();
+                        if (more) wait_in(C::PAIR_FULL + keys.at, keys.ph, 84);
+                        wait_in(C::PAIR_FULL + vals.at, vals.ph, 85);
+                        clean(ring + vals.at * C::STAGE_BYTES, (d.t0 + i) * BN, BN, d.kv);
+                        if (i < n0) {
+                            wait_p(0);
+                            values(0, vals, i > 0);
+                            if (i + 1 < n0) scores(0, keys);
+                            else commit(C::O_FULL);
+                            if (i + 2 == n0) commit(C::Q_EMPTY);
+                        }
+                        wait_p(1);
+                        values(1, vals, i > 0);
                         commit(C::PAIR_EMPTY + vals.at);
-                        if (more) scores(1, keys, i + 2 == n1);
-                        else commit(C::O_FULL + 1);
-                        if (!more && more_items) first_scores(1, keys, d.steps[1]);
-                        if (go_on) commit(C::PAIR_EMPTY + keys.at);
+                        if (more) {
+                            scores(1, keys);
+                            commit(C::PAIR_EMPTY + keys.at);
+                        } else {
+                            commit(C::O_FULL + 1);
+                        }
+                        if (i + 2 == n1) commit(C::Q_EMPTY + 1);
                     }
                 }
                 if (elect_one()) umma_commit(bar(C::PAIRS_DONE));
@@ -803,8 +782,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
                 if (has_pairs) wait_in(C::PAIRS_DONE, 0, 86);
                 const uint32_t own = ring + s * (C::STAGES * C::SLOT_BYTES);
                 const int first = s * C::STAGES;
-                const uint64_t k_desc = make_smem_desc(own), v_desc = make_mn_desc(own, HN * 128), q_tile = q_desc + (uint64_t)(s * (C::Q_BYTES >> 4));
-                const uint32_t s_col = tmem + C::S_COL + 128 * s;
+                const uint64_t k_desc = make_smem_desc(own), v_desc = make_mn_desc(own, HN * 128), a = q_desc + (uint64_t)(s * (C::Q_BYTES >> 4));
+                const uint32_t s_col = tmem + C::S_COL + 128 * s, o_col = tmem + C::O_COL + D * s;
                 uint32_t slot = 0, ph = 0, q_parity = 0, p_parity = 0;
                 auto advance = [&]() {
                     if (++slot == C::STAGES) slot = 0, ph ^= 1u;
@@ -821,7 +800,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
                             if (ok && elect_one()) {
 #pragma unroll
                                 for (int k = 0; k < D / 16; ++k)
-                                    umma_bf16(s_col + HN * h, q_tile + (k / 4) * (BM * 128 >> 4) + (k % 4) * 2, b + (k / 4) * (HN * 128 >> 4) + (k % 4) * 2,
+                                    umma_bf16(s_col + HN * h, a + (k / 4) * (BM * 128 >> 4) + (k % 4) * 2, b + (k / 4) * (HN * 128 >> 4) + (k % 4) * 2,
                                               C::IDESC_S_SLOT, k > 0);
                                 umma_commit(bar(C::SLOT_EMPTY + first + slot));
                             }
@@ -834,11 +813,21 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
                         for (int h = 0; h < 2; ++h) {
                             wait_in(C::SLOT_FULL + first + (int)slot, ph, 89);
                             clean(own + slot * C::SLOT_BYTES, (d.t0 + i) * BN + h * HN, HN, d.kv);
-                            values(s, C::P_FULL + 4 + 2 * s + h, p_parity, h, v_desc + (uint64_t)(slot * (C::SLOT_BYTES >> 4)), i > 0 || h > 0);
-                            commit(C::SLOT_EMPTY + first + (int)slot);
+                            if (h == 0) {
+                                wait_in(C::P_FULL + 2 + s, p_parity, 90), p_parity ^= 1u;
+                                tc_fence_after();
+                            }
+                            const uint64_t b = v_desc + (uint64_t)(slot * (C::SLOT_BYTES >> 4));
+                            const uint32_t accumulate = i > 0 || h > 0;
+                            if (ok && elect_one()) {
+                                umma_bf16_ts(o_col, s_col + 32 * h, b, C::IDESC_O, accumulate);
+#pragma unroll
+                                for (int k = 1; k < HN / 16; ++k) umma_bf16_ts(o_col, s_col + 32 * h + 8 * k, b + k * (2048 >> 4), C::IDESC_O, 1u);
+                                umma_commit(bar(C::SLOT_EMPTY + first + slot));
+                            }
+                            __syncwarp();
                             advance();
                         }
-                        p_parity ^= 1u;
                     }
                     commit(C::O_FULL + 2 + s);
                 }
@@ -857,62 +846,75 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
     }
 }
 
-// Joins the pieces of the item that begins at worker x of the first kernel and goes on behind it.  A thread has 16 bytes (WIDE times)
-// of a row and reads the pieces JOIN / WIDE at a time, so that an item cut over all blocks costs a few latencies and not one per piece.
-// ROWS rows at once: 8 where a head has few rows in all, 32 (of which a thread has WIDE pieces) where tiles are full.
-constexpr int JOIN = 8;
-template <int D, int ROWS, int WIDE>
-__global__ void __launch_bounds__(ROWS * D / 4 / WIDE) paged_attention_join_kernel(const Params p) {
+// Joins the pieces of the item that begins at worker x of the first kernel and goes on behind it: 32 rows and four pieces of four
+// columns each per warp, or eight rows at once where there are few.  A thread reads the results of several workers at a time, so
+// that an item cut over all blocks costs a few latencies and not one per block.
+template <int D, int WIDE, int AT_ONCE>
+__device__ __forceinline__ void join_row(const Params& p, const float* tail, int pieces, int row, const int (&at)[WIDE], __nv_bfloat16* dst) {
+    const long long slot_floats = (long long)p.slot_rows * (D + 2);
+    float top = -CUDART_INF_F, l = 0;
+    float4 o[WIDE];
+#pragma unroll
+    for (int k = 0; k < WIDE; ++k) o[k] = make_float4(0, 0, 0, 0);
+    for (int i0 = 0; i0 < pieces; i0 += AT_ONCE) {
+        float m[AT_ONCE], s[AT_ONCE];
+        float4 x[AT_ONCE][WIDE];
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; ++j) {
+            const int i = i0 + j;
+            const float* slot = tail + (2ll * i - (i == 0 ? 0 : 1)) * slot_floats;  // the first piece is a tail, the others are heads
+            const bool there = i < pieces;
+            m[j] = there ? slot[p.slot_rows * D + row] : -CUDART_INF_F;
+            s[j] = there ? slot[p.slot_rows * (D + 1) + row] : 0.f;
+#pragma unroll
+            for (int k = 0; k < WIDE; ++k) x[j][k] = there ? reinterpret_cast<const float4*>(slot)[at[k]] : make_float4(0, 0, 0, 0);
+        }
+        float up = top;
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; ++j) up = fmaxf(up, m[j]);
+        const float w0 = weight_to(top, up);
+        top = up;
+        l *= w0;
+#pragma unroll
+        for (int k = 0; k < WIDE; ++k) o[k].x *= w0, o[k].y *= w0, o[k].z *= w0, o[k].w *= w0;
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; ++j) {
+            const float w = weight_to(m[j], up);
+            l += w * s[j];
+#pragma unroll
+            for (int k = 0; k < WIDE; ++k) o[k].x += w * x[j][k].x, o[k].y += w * x[j][k].y, o[k].z += w * x[j][k].z, o[k].w += w * x[j][k].w;
+        }
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int k = 0; k < WIDE; ++k)
+        *reinterpret_cast<uint2*>(dst + 4 * k) = make_uint2(pack_bf16x2(o[k].x * inv, o[k].y * inv), pack_bf16x2(o[k].z * inv, o[k].w * inv));
+}
+
+template <int D>
+__global__ void __launch_bounds__(2 * D) paged_attention_join_kernel(const Params p) {
     wait_for_preceding_grid();
     const int* header = p.headers + blockIdx.x * HEADER;
     const int4 h = *reinterpret_cast<const int4*>(header);
     const int pieces = h.x, start = h.y, hk = h.z, tok0 = h.w, rows = header[4];
     if (pieces == 0) return;
-    const long long slot_floats = (long long)p.slot_rows * (D + 2);
-    const float* const tail = p.partial + (2ll * blockIdx.x + 1) * slot_floats;  // the first piece; the others lie two slots apart
-    const int chunk = threadIdx.x / ROWS * WIDE;
-    constexpr int AT_ONCE = JOIN / WIDE;
-    for (int row = blockIdx.y * ROWS + threadIdx.x % ROWS; row < rows; row += gridDim.y * ROWS) {
-        float top = -CUDART_INF_F, l = 0;
-        float4 o[WIDE];
-#pragma unroll
-        for (int k = 0; k < WIDE; ++k) o[k] = make_float4(0, 0, 0, 0);
-        for (int i0 = 0; i0 < pieces; i0 += AT_ONCE) {
-            float m[AT_ONCE], s[AT_ONCE];
-            float4 x[AT_ONCE][WIDE];
-#pragma unroll
-            for (int j = 0; j < AT_ONCE; ++j) {
-                const int i = i0 + j;
-                const float* slot = tail + (2ll * i - (i == 0 ? 0 : 1)) * slot_floats;
-                const bool there = i < pieces;
-                m[j] = there ? slot[p.slot_rows * D + row] : -CUDART_INF_F;
-                s[j] = there ? slot[p.slot_rows * (D + 1) + row] : 0.f;
-#pragma unroll
-                for (int k = 0; k < WIDE; ++k)
-                    x[j][k] = there ? reinterpret_cast<const float4*>(slot)[(chunk + k) * p.slot_rows + row] : make_float4(0, 0, 0, 0);
-            }
-            float up = top;
-#pragma unroll
-            for (int j = 0; j < AT_ONCE; ++j) up = fmaxf(up, m[j]);
-            const float w0 = weight_to(top, up);
-            top = up;
-            l *= w0;
-#pragma unroll
-            for (int k = 0; k < WIDE; ++k) o[k].x *= w0, o[k].y *= w0, o[k].z *= w0, o[k].w *= w0;
-#pragma unroll
-            for (int j = 0; j < AT_ONCE; ++j) {
-                const float w = weight_to(m[j], up);
-                l += w * s[j];
-#pragma unroll
-                for (int k = 0; k < WIDE; ++k) o[k].x += w * x[j][k].x, o[k].y += w * x[j][k].y, o[k].z += w * x[j][k].z, o[k].w += w * x[j][k].w;
-            }
-        }
-        const float inv = l == 0.f ? 0.f : 1.f / l;
+    const float* const tail = p.partial + (2ll * blockIdx.x + 1) * p.slot_rows * (D + 2);
+    auto out_of = [&](int row) {
         const int token = row / p.group, head = hk * p.group + (row - token * p.group);
-        __nv_bfloat16* const dst = p.out + (long long)(start + tok0 + token) * p.o_token + (long long)head * p.o_head + chunk * 4;
-#pragma unroll
-        for (int k = 0; k < WIDE; ++k)
-            *reinterpret_cast<uint2*>(dst + 4 * k) = make_uint2(pack_bf16x2(o[k].x * inv, o[k].y * inv), pack_bf16x2(o[k].z * inv, o[k].w * inv));
+        return p.out + (long long)(start + tok0 + token) * p.o_token + (long long)head * p.o_head;
+    };
+    if (rows > 32) {
+        const int chunk = threadIdx.x / 32 * 4;
+        for (int row = blockIdx.y * 32 + threadIdx.x % 32; row < rows; row += gridDim.y * 32) {
+            const int at[4] = {chunk * p.slot_rows + row, (chunk + 1) * p.slot_rows + row, (chunk + 2) * p.slot_rows + row, (chunk + 3) * p.slot_rows + row};
+            join_row<D, 4, 2>(p, tail, pieces, row, at, out_of(row) + 4 * chunk);
+        }
+    } else {
+        const int chunk = threadIdx.x / 8;
+        for (int row = blockIdx.y * 8 + threadIdx.x % 8; row < rows; row += gridDim.y * 8) {
+            const int at[1] = {chunk * p.slot_rows + row};
+            join_row<D, 1, 8>(p, tail, pieces, row, at, out_of(row) + 4 * chunk);
+        }
     }
 }
 
@@ -958,15 +960,15 @@ static int encode_page_map(CUtensorMap* map, const void* base, const long long* 
     const cuuint32_t box[4] = {64, (cuuint32_t)(page < HN ? page : HN), 1, 1};
     return encode_map(map, base, 4, dims, st, box, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
 }
-static int encode_query_map(CUtensorMap* map, const void* base, const long long* strides, int rows, int heads, int group, int D) {
+static int encode_query_map(CUtensorMap* map, const void* base, const long long* strides, int rows, int heads, int group, int tokens, int D) {
     const cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)heads, (cuuint64_t)rows};
     const cuuint64_t st[2] = {stride_bytes(strides[1], heads, D), stride_bytes(strides[0], rows, D)};
-    const cuuint32_t box[3] = {64, (cuuint32_t)group, (cuuint32_t)(BM / group)};
+    const cuuint32_t box[3] = {64, (cuuint32_t)group, (cuuint32_t)tokens};
     return encode_map(map, base, 3, dims, st, box, CU_TENSOR_MAP_L2_PROMOTION_L2_128B);
 }
 
 template <int D>
-static int launch(const Params& p, const CUtensorMap& qmap, const CUtensorMap& kmap, const CUtensorMap& vmap, int blocks, cudaStream_t stream) {
+static int launch(const Params& p, const CUtensorMap& qmap, const CUtensorMap& hqmap, const CUtensorMap& kmap, const CUtensorMap& vmap, int blocks, cudaStream_t stream) {
     static bool prepared[kMaxDevices];  // of the device, once; a second thread that does it again does no harm
     const int dev = current_device();
     if (dev < 0) return QB200_ERR_CUDA;
@@ -974,20 +976,19 @@ static int launch(const Params& p, const CUtensorMap& qmap, const CUtensorMap& k
         if (cudaFuncSetAttribute(paged_attention_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::SMEM) != cudaSuccess) return QB200_ERR_CUDA;
         prepared[dev] = true;
     }
-    paged_attention_kernel<D><<<blocks, kThreads, Cfg<D>::SMEM, stream>>>(p, qmap, kmap, vmap);
+    paged_attention_kernel<D><<<blocks, kThreads, Cfg<D>::SMEM, stream>>>(p, qmap, hqmap, kmap, vmap);
     const int st = launch_status();
     if (st != QB200_OK) return st;
     cudaLaunchConfig_t cfg = {};
-    const bool few = p.slot_rows <= 32;
-    cfg.gridDim = dim3(4 * blocks, few ? p.slot_rows / 8 : p.slot_rows / 32);
-    cfg.blockDim = dim3(few ? 8 * D / 4 : 32 * D / 16);
+    cfg.gridDim = dim3(4 * blocks, p.slot_rows / 32);
+    cfg.blockDim = dim3(2 * D);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cuda_status(few ? cudaLaunchKernelEx(&cfg, paged_attention_join_kernel<D, 8, 1>, p) : cudaLaunchKernelEx(&cfg, paged_attention_join_kernel<D, 32, 4>, p));
+    return cuda_status(cudaLaunchKernelEx(&cfg, paged_attention_join_kernel<D>, p));
 }
 
 }  // namespace pa
@@ -1022,8 +1023,10 @@ extern "C" int paged_attention_cuda_bf16(void* out, const long long* out_strides
         if (k_strides[i] % 8 || v_strides[i] % 8 || (i < 2 && (q_strides[i] % 8 || out_strides[i] % 8))) return QB200_ERR_UNSUPPORTED;
     const int group = n_head / n_kv_head, sms = pa::sm_count();
     if (sms == 0) return QB200_ERR_CUDA;
-    CUtensorMap qmap, kmap, vmap;
-    int st = pa::encode_query_map(&qmap, q, q_strides, rows, n_head, group, head_dim);
+    CUtensorMap qmap, hqmap, kmap, vmap;
+    const int tokens = pa::BM / group, half_tokens = pa::BM / 2 / group;  // 0: no tile has so few rows
+    int st = pa::encode_query_map(&qmap, q, q_strides, rows, n_head, group, tokens, head_dim);
+    if (st == QB200_OK) st = pa::encode_query_map(&hqmap, q, q_strides, rows, n_head, group, half_tokens > 0 ? half_tokens : tokens, head_dim);
     if (st == QB200_OK) st = pa::encode_page_map(&kmap, k_cache, k_strides, num_pages, page_size, n_kv_head, head_dim);
     if (st == QB200_OK) st = pa::encode_page_map(&vmap, v_cache, v_strides, num_pages, page_size, n_kv_head, head_dim);
     if (st != QB200_OK) return st;
@@ -1036,8 +1039,8 @@ extern "C" int paged_attention_cuda_bf16(void* out, const long long* out_strides
     p.o_token = out_strides[0], p.o_head = out_strides[1];
     p.wide_stores = reinterpret_cast<uintptr_t>(out) % 32 == 0 && p.o_token % 16 == 0 && p.o_head % 16 == 0;
     p.c = fmaxf(scale * 1.4426950408889634f, 1.17549435e-38f);  // above zero: what is masked stays at minus infinity
-    p.rows = rows, p.batch = batch, p.width = width, p.hkv = n_kv_head, p.group = group, p.tokens = pa::BM / group;
+    p.rows = rows, p.batch = batch, p.width = width, p.hkv = n_kv_head, p.group = group, p.tokens = tokens, p.half_tokens = half_tokens;
     p.num_pages = num_pages, p.page = page_size;
     for (p.page_shift = 0; (1 << p.page_shift) < page_size; ++p.page_shift) {}
-    return head_dim == 64 ? pa::launch<64>(p, qmap, kmap, vmap, sms, stream) : pa::launch<128>(p, qmap, kmap, vmap, sms, stream);
+    return head_dim == 64 ? pa::launch<64>(p, qmap, hqmap, kmap, vmap, sms, stream) : pa::launch<128>(p, qmap, hqmap, kmap, vmap, sms, stream);
 }
