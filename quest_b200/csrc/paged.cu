@@ -221,17 +221,14 @@ struct VerifyParams {
     int batch, n_tokens, vocab, most;
 };
 
-constexpr int kVerifyThreads = 256, kVerifyCluster = 8, kSegment = 256;
-constexpr int kMaxSegments = 4096;  // of one block: a vocabulary of up to 8 Mi entries
+constexpr int kVerifyThreads = 256, kVerifyWarps = kVerifyThreads / 32, kVerifyCluster = 8, kSegment = 256;
 
-__device__ __forceinline__ double as_double(float v) { return v; }
-__device__ __forceinline__ double as_double(__nv_bfloat16 v) { return __bfloat162float(v); }
-// A weight: what is not positive (a NaN among it) counts as nothing.
-__device__ __forceinline__ double weight_of(double p, double q) { const double w = p - q; return w > 0 ? w : 0; }
+__device__ __forceinline__ float as_float(float v) { return v; }
+__device__ __forceinline__ float as_float(__nv_bfloat16 v) { return __bfloat162float(v); }
 
 // Eight neighbouring entries of a row of probabilities, zeros behind its end.
 template <typename T, bool VEC>
-__device__ __forceinline__ void load8(double (&x)[8], const T* row, int at, int vocab) {
+__device__ __forceinline__ void load8(float (&x)[8], const T* row, int at, int vocab) {
     if (VEC && at + 8 <= vocab) {
         if (sizeof(T) == 4) {
             const uint4 a = __ldg(reinterpret_cast<const uint4*>(row + at)), b = __ldg(reinterpret_cast<const uint4*>(row + at) + 1);
@@ -247,21 +244,33 @@ __device__ __forceinline__ void load8(double (&x)[8], const T* row, int at, int 
         return;
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = at + j < vocab ? as_double(row[at + j]) : 0;
+    for (int j = 0; j < 8; ++j) x[j] = at + j < vocab ? as_float(row[at + j]) : 0;
+}
+
+// Sum of eight weights max(p - q, 0), which decides between tokens and so has to be as good as one in 64 bits, without 64-bit
+// arithmetic per entry (converting every entry made the kernel four times slower than its reads: 55 us where two rows of 131072
+// bf16 for 200 requests take 12): the difference is split into d + e exactly, d into a multiple of 2^-16, whose sums are exact in
+// fp32, and a rest below 2^-17, whose sums lose less than 2^-38; two conversions for eight entries.
+__device__ __forceinline__ double sum8(const float (&p)[8], const float (&q)[8]) {
+    float high = 0, low = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float d = __fsub_rn(p[j], q[j]), e = __fsub_rn(__fsub_rn(p[j], d), q[j]);  // d + e = p - q where p > q >= 0
+        const float h = __fsub_rn(__fadd_rn(d, 192.f), 192.f), r = __fadd_rn(__fsub_rn(d, h), e);
+        if (d > 0) high = __fadd_rn(high, h), low = __fadd_rn(low, r);  // what is not positive (a NaN among it) counts as nothing
+    }
+    return (double)high + (double)low;
 }
 
 // Rejection sampling against a draft, one cluster of eight blocks per request.  Draft i is kept while u_i q_i(x_i) < p_i(x_i);
 // the next token is drawn from max(p - q, 0) of the first refused row, or from the row behind the last draft, by inverting the
-// running sum at u times the total.  Every block takes an eighth of the vocabulary and sums segments of 256 entries in 64 bits
-// (sums decide which token it is: in 32 bits the border between two tokens would depend on the order); the totals go round the
-// cluster, and the block that holds the border reads that one segment again.  So a row is read once; without clusters a
-// request would have a single SM's bandwidth (V 131072, two fp32 rows: 1 MB) or a second launch.
+// running sum at u times the total.  Every warp of the cluster sums a stretch of the vocabulary; the totals go round the cluster, and
+// the block that holds the border reads the stretch of that warp again, a segment of 256 entries per warp.  So a row is read once;
+// without clusters a request would have a single SM's bandwidth or a second launch.
 template <typename T, bool VEC>
 __global__ void __cluster_dims__(kVerifyCluster, 1, 1) __launch_bounds__(kVerifyThreads) verify_drafts_kernel(const VerifyParams p) {
-    extern __shared__ double seg_sum[];
-    __shared__ int s_refused;
-    __shared__ double s_total;
-    __shared__ int s_last;  // last entry of this block with a weight, -1: none
+    __shared__ int s_refused, s_last, s_hit, s_fall;  // s_last: last entry of this block with a weight, -1: none
+    __shared__ double s_warp[kVerifyWarps], s_total;
     cg::cluster_group cluster = cg::this_cluster();
     const int b = blockIdx.x / kVerifyCluster, rank = blockIdx.x % kVerifyCluster;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -275,8 +284,8 @@ __global__ void __cluster_dims__(kVerifyCluster, 1, 1) __launch_bounds__(kVerify
         const long long x = p.tokens[c0 + i];
         bool good = false;
         if (x >= 0 && x < p.vocab) {
-            const double q = p.draft == nullptr ? 1.0 : as_double(draft[(long long)i * p.vocab + x]);
-            good = (double)p.u[c0 + b + i] * q < as_double(target[(long long)i * p.vocab + x]);
+            const double q = p.draft == nullptr ? 1.0 : (double)as_float(draft[(long long)i * p.vocab + x]);
+            good = (double)p.u[c0 + b + i] * q < (double)as_float(target[(long long)i * p.vocab + x]);
         }
         if (!good) atomicMin(&s_refused, i);
     }
@@ -288,68 +297,56 @@ __global__ void __cluster_dims__(kVerifyCluster, 1, 1) __launch_bounds__(kVerify
     const long long hot = refused && p.draft == nullptr ? p.tokens[c0 + kept] : -1;  // a draft without probabilities: all on its token
 
     const int segments = (p.vocab + kSegment - 1) / kSegment;
-    const int share = (segments + kVerifyCluster - 1) / kVerifyCluster;
-    const int seg0 = min(rank * share, segments), seg1 = min(seg0 + share, segments);
+    const int share = (segments + kVerifyCluster * kVerifyWarps - 1) / (kVerifyCluster * kVerifyWarps);  // of a warp
+    const int seg0 = min((rank * kVerifyWarps + warp) * share, segments), seg1 = min(seg0 + share, segments);
     bool residual = refused;
-    double total = 0, before = 0;
-    int last = -1;
-    auto weights = [&](double (&w)[8], int at) {
-        load8<T, VEC>(w, prow, at, p.vocab);
+    auto load = [&](float (&x)[8], float (&q)[8], int at) {
+        load8<T, VEC>(x, prow, at, p.vocab);
         if (residual && p.draft != nullptr) {
-            double q[8];
             load8<T, VEC>(q, qrow, at, p.vocab);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) w[j] = weight_of(w[j], q[j]);
         } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) w[j] = residual && at + j == hot ? 0 : weight_of(w[j], 0);
+            for (int j = 0; j < 8; ++j) {
+                q[j] = 0;
+                if (residual && at + j == hot) x[j] = 0;
+            }
         }
     };
+    double total = 0, before = 0;  // of all blocks, of those before this one
+    int last = -1;
     while (true) {
-        if (threadIdx.x == 0) s_total = 0, s_last = -1;
+        if (threadIdx.x == 0) s_last = -1;
         __syncthreads();
-        for (int s = seg0 + warp; s < seg1; s += kVerifyThreads / 32) {
-            double w[8];
+        double sum = 0;
+        int mine = -1;
+#pragma unroll 4
+        for (int s = seg0; s < seg1; ++s) {
+            float x[8], q[8];
             const int at = s * kSegment + lane * 8;
-            weights(w, at);
-            double sum = 0;
-            int mine = -1;
+            load(x, q, at);
+            const double add = sum8(x, q);
+            sum += add;
+            if (add > 0) mine = at;
+        }
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                sum += w[j];
-                if (w[j] > 0) mine = at + j;
-            }
-#pragma unroll
-            for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
-            mine = __reduce_max_sync(~0u, mine);
-            if (lane == 0) {
-                seg_sum[s - seg0] = sum;
-                if (mine >= 0) atomicMax(&s_last, mine);
-            }
+        for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
+        mine = __reduce_max_sync(~0u, mine);
+        if (lane == 0) {
+            s_warp[warp] = sum;
+            if (mine >= 0) atomicMax(&s_last, mine);
         }
         __syncthreads();
-        if (warp == 0) {  // running sums of the segments
-            double carry = 0;
-            for (int s = 0; s < seg1 - seg0; s += 32) {
-                double v = s + lane < seg1 - seg0 ? seg_sum[s + lane] : 0;
-#pragma unroll
-                for (int d = 1; d < 32; d <<= 1) {
-                    const double o = __shfl_up_sync(~0u, v, d);
-                    if (lane >= d) v += o;
-                }
-                v += carry;
-                if (s + lane < seg1 - seg0) seg_sum[s + lane] = v;
-                carry = __shfl_sync(~0u, v, min(31, seg1 - seg0 - s - 1));  // the very value of the last segment
-            }
-            if (lane == 0) s_total = carry;
+        if (threadIdx.x == 0) {
+            double t = 0;
+            for (int w = 0; w < kVerifyWarps; ++w) t += s_warp[w];
+            s_total = t;
         }
         cluster.sync();
         total = before = 0;
         last = -1;
         for (int r = 0; r < kVerifyCluster; ++r) {
-            const double t = *cluster.map_shared_rank(&s_total, r);
             if (r == rank) before = total;
-            total += t;
+            total += *cluster.map_shared_rank(&s_total, r);
             last = max(last, *cluster.map_shared_rank(&s_last, r));
         }
         cluster.sync();  // nobody leaves or starts over while another block reads
@@ -363,49 +360,70 @@ __global__ void __cluster_dims__(kVerifyCluster, 1, 1) __launch_bounds__(kVerify
             if (i != kept) p.out[(long long)b * (p.most + 1) + i] = i < kept ? p.tokens[c0 + i] : -1;
         if (threadIdx.x == 0) p.accepted[b] = kept;
     }
-    if (warp != 0) return;
     long long* slot = p.out + (long long)b * (p.most + 1) + kept;
-    const bool beyond = !(aim < total);  // u that rounds to one, or no weight at all
-    if (beyond) {
-        if (rank == 0 && lane == 0) *slot = last < 0 ? 0 : last;
+    // The block whose part holds the aim; where u rounds to one the one with the last weight, and without any weight the first.
+    const bool beyond = !(aim < total);
+    const int per_block = share * kVerifyWarps * kSegment;
+    if (beyond ? rank != (last < 0 ? 0 : last / per_block) : !(before <= aim && aim < before + s_total)) return;
+    if (beyond && last < 0) {
+        if (threadIdx.x == 0) *slot = 0;
         return;
     }
-    const int mine = seg1 - seg0;
-    if (mine == 0 || !(before <= aim && aim < before + seg_sum[mine - 1])) return;
-    int lo = 0, hi = mine - 1;  // first segment whose running sum passes the aim
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (before + seg_sum[mid] > aim) hi = mid; else lo = mid + 1;
+    // ---- the warp's stretch, then the segment, then the entry
+    int w = 0;
+    double base = before;
+    if (beyond) {
+        w = (last - rank * per_block) / (share * kSegment);
+    } else {
+        while (w + 1 < kVerifyWarps && !(base + s_warp[w] > aim)) base += s_warp[w++];
     }
-    int hit = 0x7fffffff, fall = -1;
-    for (;; ++lo) {
-        const double base = before + (lo == 0 ? 0 : seg_sum[lo - 1]);
-        double w[8];
-        const int at = (seg0 + lo) * kSegment + lane * 8;
-        weights(w, at);
-        double sum = 0;
+    const int first = (rank * kVerifyWarps + w) * share, end = min(first + share, segments);
+    if (threadIdx.x == 0) s_hit = 0x7fffffff, s_fall = -1;
+    for (int s = first; s < end; s += kVerifyWarps) {
+        float x[8], q[8];
+        double v[8], sum = 0;
+        const int at = (s + warp) * kSegment + lane * 8;
+        load(x, q, s + warp < end ? at : p.vocab);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) sum += w[j];
+        for (int j = 0; j < 8; ++j) {
+            v[j] = (double)x[j] - (double)q[j];
+            v[j] = v[j] > 0 ? v[j] : 0;
+            sum += v[j];
+        }
         double run = sum;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
             const double o = __shfl_up_sync(~0u, run, d);
             if (lane >= d) run += o;
         }
-        run += base - sum;
+        __syncthreads();  // the round before has been read
+        if (lane == 31) s_warp[warp] = run;
+        __syncthreads();
+        double mine = base;
+        for (int k = 0; k < kVerifyWarps; ++k) {
+            if (k == warp) mine = base;
+            base += s_warp[k];
+        }
+        run += mine - sum;
+        int hit = 0x7fffffff, fall = -1;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            run += w[j];
-            if (w[j] > 0) {
+            run += v[j];
+            if (v[j] > 0) {
                 if (run > aim) hit = min(hit, at + j);
                 fall = at + j;
             }
         }
         hit = __reduce_min_sync(~0u, hit);
         fall = __reduce_max_sync(~0u, fall);
-        if (fall >= 0 || lo + 1 >= mine) break;  // the sums' rounding can point at a segment without weights: the next one
+        if (lane == 0) {
+            if (hit != 0x7fffffff) atomicMin(&s_hit, hit);
+            if (fall >= 0) atomicMax(&s_fall, fall);
+        }
     }
-    if (lane == 0) *slot = hit != 0x7fffffff ? hit : fall >= 0 ? fall : last;  // ... or behind a segment's last weight: that one
+    __syncthreads();
+    // Behind the stretch's last weight by the rounding of the sums (or of u): that weight.
+    if (threadIdx.x == 0) *slot = !beyond && s_hit != 0x7fffffff ? s_hit : s_fall >= 0 ? s_fall : last;
 }
 
 }  // namespace qb
@@ -478,8 +496,7 @@ extern "C" int rope_paged_append_cuda_bf16(const void* qkv, long long ld, const 
 
 template <typename T, bool VEC>
 static int launch_verify(const VerifyParams& p, cudaStream_t stream) {
-    const int segments = (p.vocab + kSegment - 1) / kSegment, share = (segments + kVerifyCluster - 1) / kVerifyCluster;
-    verify_drafts_kernel<T, VEC><<<(unsigned)p.batch * kVerifyCluster, kVerifyThreads, sizeof(double) * share, stream>>>(p);
+    verify_drafts_kernel<T, VEC><<<(unsigned)p.batch * kVerifyCluster, kVerifyThreads, 0, stream>>>(p);
     return launch_status();
 }
 
@@ -489,7 +506,7 @@ extern "C" int verify_drafts_cuda(const void* target_probs, const void* draft_pr
     if (batch < 0 || n_drafts < 0 || vocab <= 0 || max_drafts < 0) return QB200_ERR_INVALID_ARGUMENT;
     if (batch == 0) return QB200_OK;
     if (!target_probs || !cu_drafts || !uniforms || !tokens || !accepted || (n_drafts && !draft_tokens)) return QB200_ERR_INVALID_ARGUMENT;
-    if (vocab > kMaxSegments * kVerifyCluster * kSegment || batch > (1 << 27)) return QB200_ERR_UNSUPPORTED;
+    if (vocab > (1 << 23) || batch > (1 << 27)) return QB200_ERR_UNSUPPORTED;
     VerifyParams p{target_probs, draft_probs, draft_tokens, cu_drafts, uniforms, tokens, accepted, batch, n_drafts, vocab, max_drafts};
     const bool vec = vocab % 8 == 0 && aligned16(target_probs) && aligned16(draft_probs);
     if (probs_are_bf16) return vec ? launch_verify<__nv_bfloat16, true>(p, stream) : launch_verify<__nv_bfloat16, false>(p, stream);

@@ -9,22 +9,32 @@ host, so a step can be captured in a CUDA graph and replayed while the requests 
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import NamedTuple
 
 import torch
 
 from . import _lib
 
-_Strides2, _Strides3 = ctypes.c_longlong * 2, ctypes.c_longlong * 3
+_Strides6, _Strides10 = ctypes.c_longlong * 6, ctypes.c_longlong * 10
 
 
-def _call(name: str, device: torch.device, *args) -> None:
+def _device(*tensors: torch.Tensor) -> int:
+    """The CUDA device that all of them are on."""
+    device = tensors[0].get_device()
+    for t in tensors:
+        if not t.is_cuda or t.get_device() != device:
+            _lib.require_cuda(*tensors)
+    return device
+
+
+def _call(name: str, device: int, *args) -> None:
     fn = getattr(_lib.load(), name)
-    if torch._C._cuda_getDevice() == device.index:
-        status = fn(*args, torch._C._cuda_getCurrentRawStream(device.index))
+    if torch._C._cuda_getDevice() == device:
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(device))
     else:
         with torch.cuda.device(device):
-            status = fn(*args, torch._C._cuda_getCurrentRawStream(device.index))
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(device))
     if status:
         _lib.check(status, name)
 
@@ -41,7 +51,7 @@ class PageStep(NamedTuple):
 
 def _check_i32(*tensors: torch.Tensor) -> None:
     for t in tensors:
-        assert t.dtype == torch.int32 and t.is_contiguous()
+        assert t.dtype is torch.int32 and t.is_contiguous()
 
 
 def page_assign(
@@ -65,10 +75,10 @@ def page_assign(
     assert page_table.dim() == 2 and free_pages.dim() == 1 and free_count.numel() == 1 and page_size > 0 and num_tokens >= 0
     batch, width = page_table.shape
     assert cached_lens.shape == (batch,) and new_lens.shape == (batch,)
-    dev = _lib.require_cuda(page_table, free_pages, free_count, cached_lens, new_lens)
-    cu, kv_lens, lens, positions, left = torch.empty(3 * batch + num_tokens + 2, dtype=torch.int32, device=dev).split(
-        (batch + 1, batch, batch, num_tokens, 1))
-    slots = torch.empty(num_tokens, dtype=torch.int64, device=dev)
+    dev = _device(page_table, free_pages, free_count, cached_lens, new_lens)
+    cu, kv_lens, lens, positions, left = torch.split_with_sizes(page_table.new_empty(3 * batch + num_tokens + 2),
+                                                                (batch + 1, batch, batch, num_tokens, 1))
+    slots = page_table.new_empty(num_tokens, dtype=torch.int64)
     _call("page_assign_cuda", dev, page_table.data_ptr(), free_pages.data_ptr(), free_count.data_ptr(), cached_lens.data_ptr(),
           new_lens.data_ptr(), cu.data_ptr(), kv_lens.data_ptr(), lens.data_ptr(), slots.data_ptr(), positions.data_ptr(),
           left.data_ptr(), batch, width, free_pages.numel(), num_tokens, page_size)
@@ -90,8 +100,8 @@ def page_release(
     assert page_table.dim() == 2 and free_pages.dim() == 1 and free_count.numel() == 1 and page_size > 0
     batch, width = page_table.shape
     assert lens.shape == (batch,) and keep_lens.shape == (batch,)
-    dev = _lib.require_cuda(page_table, free_pages, free_count, lens, keep_lens)
-    left = torch.empty(1, dtype=torch.int32, device=dev)
+    dev = _device(page_table, free_pages, free_count, lens, keep_lens)
+    left = free_count.new_empty(1)
     _call("page_release_cuda", dev, page_table.data_ptr(), free_pages.data_ptr(), free_count.data_ptr(), lens.data_ptr(),
           keep_lens.data_ptr(), left.data_ptr(), batch, width, free_pages.numel(), page_size)
     return left
@@ -125,14 +135,22 @@ def rope_paged_append(
     _check_i32(positions)
     assert slots.dtype == torch.int64 and slots.is_contiguous() and positions.shape == (rows,) and slots.shape == (rows,)
     if q_out is None:
-        q_out = torch.empty(rows, n_head, head_dim, dtype=qkv.dtype, device=qkv.device)
+        q_out = qkv.new_empty((rows, n_head, head_dim))
     assert q_out.shape == (rows, n_head, head_dim) and q_out.dtype == torch.bfloat16 and q_out.is_contiguous()
-    dev = _lib.require_cuda(qkv, table, positions, slots, k_cache, v_cache, q_out)
+    dev = _device(qkv, table, positions, slots, k_cache, v_cache, q_out)
+    strides = _Strides6(*k_cache.stride()[:3], *v_cache.stride()[:3])
+    at = ctypes.addressof(strides)
     _call("rope_paged_append_cuda_bf16", dev, qkv.data_ptr(), max(qkv.stride(0), qkv.size(1)), table.data_ptr(),
-          int(table.dtype == torch.bfloat16), positions.data_ptr(), slots.data_ptr(), k_cache.data_ptr(), _Strides3(*k_cache.stride()[:3]),
-          v_cache.data_ptr(), _Strides3(*v_cache.stride()[:3]), q_out.data_ptr(), rows, n_head, n_kv_head, head_dim, table.size(0),
-          num_pages, page_size)
+          table.dtype is torch.bfloat16, positions.data_ptr(), slots.data_ptr(), k_cache.data_ptr(), at, v_cache.data_ptr(), at + 24,
+          q_out.data_ptr(), rows, n_head, n_kv_head, head_dim, table.size(0), num_pages, page_size)
     return q_out
+
+
+@functools.lru_cache(maxsize=4096)
+def _workspace(device: int, rows: int, group: int, head_dim: int) -> int:
+    """Size of the workspace of an attention call in bf16 elements."""
+    with torch.cuda.device(device):
+        return _lib.load().paged_attention_workspace(rows, 1, group, 1, head_dim) // 2
 
 
 def paged_attention(
@@ -162,16 +180,15 @@ def paged_attention(
     batch, width = page_table.shape
     assert kv_lens.shape == (batch,) and cu_new.shape == (batch + 1,)
     if out is None:
-        out = torch.empty(rows, n_head, head_dim, dtype=q.dtype, device=q.device)
+        out = q.new_empty((rows, n_head, head_dim))
     assert out.shape == q.shape and out.dtype == torch.bfloat16 and out.stride(2) == 1
-    dev = _lib.require_cuda(q, k_cache, v_cache, page_table, kv_lens, cu_new, out)
-    lib = _lib.load()
-    need = lib.paged_attention_workspace(rows, batch, n_head, n_kv_head, head_dim)
-    workspace = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
-    _call("paged_attention_cuda_bf16", dev, out.data_ptr(), _Strides2(*out.stride()[:2]), q.data_ptr(), _Strides2(*q.stride()[:2]),
-          k_cache.data_ptr(), _Strides3(*k_cache.stride()[:3]), v_cache.data_ptr(), _Strides3(*v_cache.stride()[:3]),
-          page_table.data_ptr(), kv_lens.data_ptr(), cu_new.data_ptr(), None if workspace is None else workspace.data_ptr(),
-          head_dim ** -0.5 if scale is None else float(scale), rows, batch, width, n_head, n_kv_head, head_dim, num_pages, page_size)
+    dev = _device(q, k_cache, v_cache, page_table, kv_lens, cu_new, out)
+    workspace = q.new_empty(_workspace(dev, rows, n_head // n_kv_head if n_kv_head else 0, head_dim))
+    strides = _Strides10(*out.stride()[:2], *q.stride()[:2], *k_cache.stride()[:3], *v_cache.stride()[:3])
+    at = ctypes.addressof(strides)
+    _call("paged_attention_cuda_bf16", dev, out.data_ptr(), at, q.data_ptr(), at + 16, k_cache.data_ptr(), at + 32, v_cache.data_ptr(), at + 56,
+          page_table.data_ptr(), kv_lens.data_ptr(), cu_new.data_ptr(), workspace.data_ptr(), head_dim ** -0.5 if scale is None else float(scale),
+          rows, batch, width, n_head, n_kv_head, head_dim, num_pages, page_size)
     return out
 
 
@@ -199,11 +216,11 @@ def verify_drafts(
     assert cu_drafts.dim() == 1 and batch >= 0 and max_drafts >= 0 and target_probs.size(0) == n + batch
     assert uniforms.dtype == torch.float32 and uniforms.is_contiguous() and uniforms.shape == (n + batch,)
     assert draft_probs is None or (draft_probs.dtype == target_probs.dtype and draft_probs.shape == (n, vocab) and draft_probs.is_contiguous())
-    dev = _lib.require_cuda(target_probs, draft_tokens, cu_drafts, uniforms, draft_probs)
-    tokens = torch.empty(batch, max_drafts + 1, dtype=torch.int64, device=dev)
-    accepted = torch.empty(batch, dtype=torch.int32, device=dev)
+    dev = _device(target_probs, draft_tokens, cu_drafts, uniforms, *(() if draft_probs is None else (draft_probs,)))
+    tokens = draft_tokens.new_empty((batch, max_drafts + 1))
+    accepted = cu_drafts.new_empty(batch)
     # an empty draft_probs (no request has drafts) has no address and stands for nothing
-    _call("verify_drafts_cuda", dev, target_probs.data_ptr(), _lib.ptr(draft_probs), int(target_probs.dtype == torch.bfloat16),
+    _call("verify_drafts_cuda", dev, target_probs.data_ptr(), _lib.ptr(draft_probs), target_probs.dtype is torch.bfloat16,
           draft_tokens.data_ptr(), cu_drafts.data_ptr(), uniforms.data_ptr(), tokens.data_ptr(), accepted.data_ptr(), batch, n, vocab,
           max_drafts)
     return tokens, accepted
