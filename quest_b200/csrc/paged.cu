@@ -221,58 +221,105 @@ struct VerifyParams {
     int batch, n_tokens, vocab, most;
 };
 
-constexpr int kVerifyThreads = 256, kVerifyWarps = kVerifyThreads / 32, kVerifyCluster = 8, kSegment = 256;
+constexpr int kVerifyThreads = 256, kVerifyWarps = kVerifyThreads / 32, kSegment = 256;
 
 __device__ __forceinline__ float as_float(float v) { return v; }
 __device__ __forceinline__ float as_float(__nv_bfloat16 v) { return __bfloat162float(v); }
 
-// Eight neighbouring entries of a row of probabilities, zeros behind its end.
+// Eight neighbouring entries of a row of probabilities as they are read, zeros behind its end.
+template <typename T>
+struct Raw8 {
+    uint4 w[sizeof(T) / 2];
+};
 template <typename T, bool VEC>
-__device__ __forceinline__ void load8(float (&x)[8], const T* row, int at, int vocab) {
+__device__ __forceinline__ Raw8<T> read8(const T* row, int at, int vocab) {
+    Raw8<T> r;
     if (VEC && at + 8 <= vocab) {
-        if (sizeof(T) == 4) {
-            const uint4 a = __ldg(reinterpret_cast<const uint4*>(row + at)), b = __ldg(reinterpret_cast<const uint4*>(row + at) + 1);
-            const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = __uint_as_float(w[j]);
-        } else {
-            const uint4 a = __ldg(reinterpret_cast<const uint4*>(row + at));
-            const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) x[2 * j] = bf16lo_to_f32(w[j]), x[2 * j + 1] = bf16hi_to_f32(w[j]);
-        }
-        return;
+        for (int j = 0; j < (int)sizeof(T) / 2; ++j) r.w[j] = ld_stream16(reinterpret_cast<const uint4*>(row + at) + j);
+        return r;
     }
+    float x[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) x[j] = at + j < vocab ? as_float(row[at + j]) : 0;
-}
-
-// Sum of eight weights max(p - q, 0), which decides between tokens and so has to be as good as one in 64 bits, without 64-bit
-// arithmetic per entry (converting every entry made the kernel four times slower than its reads: 55 us where two rows of 131072
-// bf16 for 200 requests take 12): the difference is split into d + e exactly, d into a multiple of 2^-16, whose sums are exact in
-// fp32, and a rest below 2^-17, whose sums lose less than 2^-38; two conversions for eight entries.
-__device__ __forceinline__ double sum8(const float (&p)[8], const float (&q)[8]) {
-    float high = 0, low = 0;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const float d = __fsub_rn(p[j], q[j]), e = __fsub_rn(__fsub_rn(p[j], d), q[j]);  // d + e = p - q where p > q >= 0
-        const float h = __fsub_rn(__fadd_rn(d, 192.f), 192.f), r = __fadd_rn(__fsub_rn(d, h), e);
-        if (d > 0) high = __fadd_rn(high, h), low = __fadd_rn(low, r);  // what is not positive (a NaN among it) counts as nothing
+    if (sizeof(T) == 4) {
+        r.w[0] = make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+        r.w[sizeof(T) / 2 - 1] = make_uint4(__float_as_uint(x[4]), __float_as_uint(x[5]), __float_as_uint(x[6]), __float_as_uint(x[7]));
+    } else {
+        r.w[0] = make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
     }
-    return (double)high + (double)low;
+    return r;
+}
+template <typename T>
+__device__ __forceinline__ void values8(const Raw8<T>& r, float (&x)[8]) {
+    if (sizeof(T) == 4) {
+        const uint4 a = r.w[0], b = r.w[sizeof(T) / 2 - 1];
+        const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = __uint_as_float(w[j]);
+    } else {
+        const uint32_t w[4] = {r.w[0].x, r.w[0].y, r.w[0].z, r.w[0].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[2 * j] = bf16lo_to_f32(w[j]), x[2 * j + 1] = bf16hi_to_f32(w[j]);
+    }
 }
 
-// Rejection sampling against a draft, one cluster of eight blocks per request.  Draft i is kept while u_i q_i(x_i) < p_i(x_i);
+__device__ __forceinline__ uint64_t pair_of(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void of_pair(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t sub_pair(uint64_t a, uint64_t b) {  // one rounding, as a subtraction
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(b), "l"(0xbf800000bf800000ull), "l"(a));
+    return r;
+}
+
+// Sum of eight weights max(p - q, 0).  It decides between tokens, so it has to be as good as one in 64 bits, but 64-bit arithmetic
+// per entry cost more than reading it: the difference d is split into a multiple of 2^-16, whose sums are exact in fp32, and a
+// rest below 2^-17, whose sums lose less than 2^-38; two conversions for eight entries.  For fp32 the rounding of d itself is added back
+// (d + e = p - q exactly where p > q >= 0); the difference of two bf16 numbers has none unless one is 2^16 times the other.
+template <bool EXACT>
+__device__ __forceinline__ double sum8(const float (&p)[8], const float (&q)[8]) {
+    uint64_t high = 0, low = 0;
+    const uint64_t magic = pair_of(192.f, 192.f);
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+        const uint64_t p2 = pair_of(p[j], p[j + 1]), q2 = pair_of(q[j], q[j + 1]), d2 = sub_pair(p2, q2);
+        float d0, d1;
+        of_pair(d2, d0, d1);
+        const float w0 = fmaxf(d0, 0.f), w1 = fmaxf(d1, 0.f);  // what is not positive (a NaN among it) counts as nothing
+        const uint64_t w2 = pair_of(w0, w1), h = sub_pair(add_pair(w2, magic), magic);
+        uint64_t r = sub_pair(w2, h);
+        if (EXACT) {
+            float e0, e1;
+            of_pair(sub_pair(sub_pair(p2, d2), q2), e0, e1);
+            r = add_pair(r, pair_of(d0 > 0 ? e0 : 0.f, d1 > 0 ? e1 : 0.f));
+        }
+        high = add_pair(high, h), low = add_pair(low, r);
+    }
+    float a, b, c, d;
+    of_pair(high, a, b), of_pair(low, c, d);
+    return (double)(a + b) + (double)(c + d);
+}
+
+// Rejection sampling against a draft, one cluster of blocks per request.  Draft i is kept while u_i q_i(x_i) < p_i(x_i);
 // the next token is drawn from max(p - q, 0) of the first refused row, or from the row behind the last draft, by inverting the
 // running sum at u times the total.  Every warp of the cluster sums a stretch of the vocabulary; the totals go round the cluster, and
 // the block that holds the border reads the stretch of that warp again, a segment of 256 entries per warp.  So a row is read once;
 // without clusters a request would have a single SM's bandwidth or a second launch.
 template <typename T, bool VEC>
-__global__ void __cluster_dims__(kVerifyCluster, 1, 1) __launch_bounds__(kVerifyThreads) verify_drafts_kernel(const VerifyParams p) {
+__global__ void __launch_bounds__(kVerifyThreads, 3) verify_drafts_kernel(const VerifyParams p) {
     __shared__ int s_refused, s_last, s_hit, s_fall;  // s_last: last entry of this block with a weight, -1: none
     __shared__ double s_warp[kVerifyWarps], s_total;
     cg::cluster_group cluster = cg::this_cluster();
-    const int b = blockIdx.x / kVerifyCluster, rank = blockIdx.x % kVerifyCluster;
+    const int blocks = (int)cluster.num_blocks(), b = blockIdx.x / blocks, rank = blockIdx.x % blocks;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int c0 = min(max(p.cu[b], 0), p.n_tokens), c1 = min(max(p.cu[b + 1], c0), p.n_tokens);
     const int drafts = min(c1 - c0, p.most);
@@ -297,13 +344,14 @@ __global__ void __cluster_dims__(kVerifyCluster, 1, 1) __launch_bounds__(kVerify
     const long long hot = refused && p.draft == nullptr ? p.tokens[c0 + kept] : -1;  // a draft without probabilities: all on its token
 
     const int segments = (p.vocab + kSegment - 1) / kSegment;
-    const int share = (segments + kVerifyCluster * kVerifyWarps - 1) / (kVerifyCluster * kVerifyWarps);  // of a warp
+    const int share = (segments + blocks * kVerifyWarps - 1) / (blocks * kVerifyWarps);  // of a warp
     const int seg0 = min((rank * kVerifyWarps + warp) * share, segments), seg1 = min(seg0 + share, segments);
     bool residual = refused;
-    auto load = [&](float (&x)[8], float (&q)[8], int at) {
-        load8<T, VEC>(x, prow, at, p.vocab);
-        if (residual && p.draft != nullptr) {
-            load8<T, VEC>(q, qrow, at, p.vocab);
+    const bool both = p.draft != nullptr;
+    auto unpack = [&](const Raw8<T>& a, const Raw8<T>& b, int at, float (&x)[8], float (&q)[8]) {
+        values8(a, x);
+        if (residual && both) {
+            values8(b, q);
         } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
@@ -312,6 +360,7 @@ __global__ void __cluster_dims__(kVerifyCluster, 1, 1) __launch_bounds__(kVerify
             }
         }
     };
+    constexpr int AHEAD = 8 / sizeof(T);  // segments whose reads are under way at once
     double total = 0, before = 0;  // of all blocks, of those before this one
     int last = -1;
     while (true) {
@@ -319,14 +368,23 @@ __global__ void __cluster_dims__(kVerifyCluster, 1, 1) __launch_bounds__(kVerify
         __syncthreads();
         double sum = 0;
         int mine = -1;
-#pragma unroll 4
-        for (int s = seg0; s < seg1; ++s) {
-            float x[8], q[8];
-            const int at = s * kSegment + lane * 8;
-            load(x, q, at);
-            const double add = sum8(x, q);
-            sum += add;
-            if (add > 0) mine = at;
+        for (int s = seg0; s < seg1; s += AHEAD) {
+            Raw8<T> a[AHEAD], c[AHEAD];
+#pragma unroll
+            for (int k = 0; k < AHEAD; ++k) {
+                const int at = s + k < seg1 ? (s + k) * kSegment + lane * 8 : p.vocab;
+                a[k] = read8<T, VEC>(prow, at, p.vocab);
+                if (residual && both) c[k] = read8<T, VEC>(qrow, at, p.vocab);
+            }
+#pragma unroll
+            for (int k = 0; k < AHEAD; ++k) {
+                float x[8], q[8];
+                const int at = (s + k) * kSegment + lane * 8;
+                unpack(a[k], c[k], at, x, q);
+                const double add = sum8<sizeof(T) == 4>(x, q);
+                sum += add;
+                if (add > 0) mine = at;
+            }
         }
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
@@ -344,7 +402,7 @@ __global__ void __cluster_dims__(kVerifyCluster, 1, 1) __launch_bounds__(kVerify
         cluster.sync();
         total = before = 0;
         last = -1;
-        for (int r = 0; r < kVerifyCluster; ++r) {
+        for (int r = 0; r < blocks; ++r) {
             if (r == rank) before = total;
             total += *cluster.map_shared_rank(&s_total, r);
             last = max(last, *cluster.map_shared_rank(&s_last, r));
@@ -383,7 +441,11 @@ __global__ void __cluster_dims__(kVerifyCluster, 1, 1) __launch_bounds__(kVerify
         float x[8], q[8];
         double v[8], sum = 0;
         const int at = (s + warp) * kSegment + lane * 8;
-        load(x, q, s + warp < end ? at : p.vocab);
+        const int from = s + warp < end ? at : p.vocab;
+        Raw8<T> c;
+        const Raw8<T> a = read8<T, VEC>(prow, from, p.vocab);
+        if (residual && both) c = read8<T, VEC>(qrow, from, p.vocab);
+        unpack(a, c, at, x, q);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             v[j] = (double)x[j] - (double)q[j];
@@ -496,8 +558,13 @@ extern "C" int rope_paged_append_cuda_bf16(const void* qkv, long long ld, const 
 
 template <typename T, bool VEC>
 static int launch_verify(const VerifyParams& p, cudaStream_t stream) {
-    verify_drafts_kernel<T, VEC><<<(unsigned)p.batch * kVerifyCluster, kVerifyThreads, 0, stream>>>(p);
-    return launch_status();
+    // As many blocks per request as are at work at once (three per SM), eight at most: with more, the same chain of reads is waited
+    // for in several rounds (64 requests at 32000: 13.3 us with eight, CL4 with four; at 131072 200 requests: CL2 with two).
+    int cluster = 8;
+    while (cluster > 1 && (long long)p.batch * cluster > 3 * 148) cluster /= 2;
+    const cudaError_t e = launch_kernel_cluster(false, cluster, verify_drafts_kernel<T, VEC>, (long long)p.batch * cluster, kVerifyThreads, 0, stream, p);
+    const int st = launch_status();
+    return e == cudaSuccess ? st : QB200_ERR_CUDA;
 }
 
 extern "C" int verify_drafts_cuda(const void* target_probs, const void* draft_probs, int probs_are_bf16, const long long* draft_tokens,
