@@ -57,6 +57,8 @@ struct Cfg {
 
 struct Params {
     __nv_bfloat16* out;
+    const __nv_bfloat16 *q, *k, *v;  // read here only by visible_row
+    long long q_token, q_head, k_page, k_token, k_head, v_page, v_token, v_head;
     const int *page_table, *kv_lens, *cu;
     float* partial;   // 8 slots per block of slot_rows x (D + 2) floats: for each worker a piece that began before it, one that goes on
     int* headers;     // 4 per block: for each worker the item that begins there and goes on
@@ -288,6 +290,32 @@ __device__ __forceinline__ void softmax_step(RowState& st, const uint32_t s_addr
     tmem_st_wait();
 }
 
+// The sum over keys from .. to - 1 of exp2(c q.k - off) v for one row, by a warp; a lane has D / 32 columns.  For rows whose tile holds
+// keys that they do not see and whose values are not finite: there the product's zero weights give NaN.
+template <int D>
+__device__ __forceinline__ void visible_row(const Params& p, const Item& d, int token, int head, int from, int to, float off, int lane, float (&o)[D / 32]) {
+    constexpr int E = D / 32;
+    float q[E];
+    const __nv_bfloat16* src = p.q + (long long)(d.start + token) * p.q_token + (long long)head * p.q_head + lane * E;
+#pragma unroll
+    for (int e = 0; e < E; ++e) q[e] = __bfloat162float(src[e]), o[e] = 0;
+#pragma unroll 1
+    for (int j = from; j < to; ++j) {
+        const int id = p.page_table[(long long)d.b * p.width + (j >> p.page_shift)], at = j & (p.page - 1);
+        const bool there = (unsigned)id < (unsigned)p.num_pages;
+        const __nv_bfloat16* k = p.k + (there ? id : 0) * p.k_page + at * p.k_token + d.hk * p.k_head + lane * E;
+        const __nv_bfloat16* v = p.v + (there ? id : 0) * p.v_page + at * p.v_token + d.hk * p.v_head + lane * E;
+        float s = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) s += there ? q[e] * __bfloat162float(k[e]) : 0.f;
+#pragma unroll
+        for (int k2 = 16; k2 > 0; k2 >>= 1) s += __shfl_xor_sync(~0u, s, k2);
+        const float x = ex2(fmaf(s, p.c, -off));
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] += there ? x * __bfloat162float(v[e]) : 0.f;
+    }
+}
+
 // A worker's place in a line: from u to end, beginning in request b `rest` places behind the request's first.
 struct Place {
     long long u, end, rest, share;
@@ -441,6 +469,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
                 if (!ok) break;
                 if (!warp_live) continue;
                 const float l = rs.l;
+                // Values that are not finite at keys which a row does not see (later tokens of its chunk) must not reach it.
+                const int stop = min((d.t0 + steps) * BN, d.kv);
+                const bool hidden = __any_sync(~0u, live && keys < stop);
+                float check[4] = {0, 0, 0, 0};  // NaN where a column is not finite
                 if (d.slot < 0) {
                     const float inv = 1.f / l;
                     const bool empty = l == 0.f;  // no key in sight: zeros
@@ -453,14 +485,18 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
 #pragma unroll
                         for (int j = 0; j < 16; ++j)
                             w[j] = empty ? 0u : pack_bf16x2(__uint_as_float(o[2 * j]) * inv, __uint_as_float(o[2 * j + 1]) * inv);
+                        if (hidden) {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) check[j % 4] = fmaf(__uint_as_float(o[j]), 0.f, check[j % 4]);
+                        }
                         if (live) store_row32(dst + c0, w, p.wide_stores);
                     }
                 } else {
-                    const bool nothing = steps == 0;  // the first stream's rows see nothing of this piece
+                    const bool nothing = l == 0.f;  // the row sees nothing of this piece (which may have no step for its stream)
                     float* const slot = p.partial + (long long)(d.slot + (list == 0 ? 2 * blocks * s : 0)) * p.slot_rows * (D + 2);
                     const bool mine = row >= 0 && row < p.slot_rows;
                     if (mine) {
-                        slot[p.slot_rows * D + row] = rs.m == -CUDART_INF_F ? -CUDART_INF_F : rs.m * p.c;
+                        slot[p.slot_rows * D + row] = rs.m == -CUDART_INF_F ? rs.m : rs.m * p.c;
                         slot[p.slot_rows * (D + 1) + row] = l;
                     }
 #pragma unroll 1
@@ -472,8 +508,28 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
                         for (int j = 0; j < 8; ++j) {
                             uint4 x = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
                             if (nothing) x = make_uint4(0, 0, 0, 0);
+                            check[0] = fmaf(__uint_as_float(x.x), 0.f, check[0]), check[1] = fmaf(__uint_as_float(x.y), 0.f, check[1]);
+                            check[2] = fmaf(__uint_as_float(x.z), 0.f, check[2]), check[3] = fmaf(__uint_as_float(x.w), 0.f, check[3]);
                             if (mine) reinterpret_cast<uint4*>(slot)[(c0 / 4 + j) * p.slot_rows + row] = x;
                         }
+                    }
+                }
+                uint32_t bad = __ballot_sync(~0u, hidden && live && !((check[0] + check[1]) + (check[2] + check[3]) == 0.f) && l > 0.f && l < CUDART_INF_F && keys < stop);
+                if (bad != 0) __syncwarp();  // the rows' stores are behind
+                while (bad != 0) {
+                    const int from = __ffs(bad) - 1, r = __shfl_sync(~0u, row, from), t = __shfl_sync(~0u, token, from);
+                    const int h = d.hk * p.group + __shfl_sync(~0u, row_head, from);
+                    const float sum = __shfl_sync(~0u, l, from);
+                    bad &= bad - 1;
+                    float o[D / 32];
+                    visible_row<D>(p, d, t, h, d.t0 * BN, min(__shfl_sync(~0u, keys, from), stop), __shfl_sync(~0u, rs.m, from) * p.c, lane, o);
+#pragma unroll
+                    for (int e = 0; e < D / 32; ++e) {
+                        const int col = lane * (D / 32) + e;
+                        if (d.slot < 0)
+                            p.out[(long long)(d.start + t) * p.o_token + (long long)h * p.o_head + col] = __float2bfloat16(o[e] / sum);
+                        else
+                            p.partial[(long long)(d.slot + (list == 0 ? 2 * blocks * s : 0)) * p.slot_rows * (D + 2) + ((col / 4) * p.slot_rows + r) * 4 + col % 4] = o[e];
                     }
                 }
                 tc_fence_before();
@@ -1032,6 +1088,9 @@ extern "C" int paged_attention_cuda_bf16(void* out, const long long* out_strides
     if (st != QB200_OK) return st;
     pa::Params p{};
     p.out = static_cast<__nv_bfloat16*>(out);
+    p.q = static_cast<const __nv_bfloat16*>(q), p.k = static_cast<const __nv_bfloat16*>(k_cache), p.v = static_cast<const __nv_bfloat16*>(v_cache);
+    p.q_token = q_strides[0], p.q_head = q_strides[1], p.k_page = k_strides[0], p.k_token = k_strides[1], p.k_head = k_strides[2];
+    p.v_page = v_strides[0], p.v_token = v_strides[1], p.v_head = v_strides[2];
     p.page_table = page_table, p.kv_lens = kv_lens, p.cu = cu_new;
     p.slot_rows = pa::slot_rows_of(rows, group);
     p.partial = static_cast<float*>(workspace);

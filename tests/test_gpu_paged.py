@@ -232,6 +232,28 @@ def test_attention_pages_outside_the_pool_read_as_nothing():
     assert ((got.double().cpu() - want).abs() <= (2 ** -8 + 2 ** -10) * size + 2 ** -8 * want.abs() + 1e-30).all()
 
 
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("hq, hkv, kv, new", [(4, 2, 300, 200), (8, 1, 40, 5), (16, 16, 260, 260), (2, 1, 6000, 100), (8, 8, 5000, 3)])
+def test_attention_later_tokens_that_are_not_finite_do_not_reach_earlier_rows(hq, hkv, kv, new, bad):
+    """Keys and values of a chunk's later tokens, not finite in one column or in all: rows in front of them are as without, rows behind
+    them are not finite where they have to be (a weight of zero times an infinity is a NaN in either)."""
+    s = ref.paged_state(kv + new, [kv, 30], [new, 2], hq, hkv, 128 if new % 2 else 64, 16)
+    clean = quest.paged_attention(**s).clone()
+    first = kv - new // 2
+    page = s["k_cache"].size(1)
+    for j in range(first, kv):
+        at = s["page_table"][0, j // page].long()
+        s["v_cache"][at, j % page, :, 3 if j % 2 else slice(None)] = bad
+        if j % 3 == 0:
+            s["k_cache"][at, j % page, 0] = bad
+    got = quest.paged_attention(**s)
+    split = first - (kv - new)  # the chunk's rows in front of the first such token
+    want, size = ref.attention(s["q"][:split], s["k_cache"], s["v_cache"], s["page_table"].cpu(), [first], [0, split], s["q"].size(2) ** -0.5, s["q"][:split])
+    assert torch.isfinite(got[:split]).all() and torch.isfinite(got[new:]).all() and torch.equal(got[new:], clean[new:])
+    assert ((got[:split].double().cpu() - want).abs() <= (2 ** -8 + 2 ** -10) * size + 2 ** -8 * want.abs() + 1e-30).all()
+    assert not torch.isfinite(got[split:new, :, 3]).any()
+
+
 def test_attention_is_the_same_call_after_call():
     s = ref.paged_state(10, [700, 3000, 90], [1, 40, 90], 16, 4, 128, 32)
     first = quest.paged_attention(**s).clone()
