@@ -30,7 +30,7 @@ constexpr int BM = 128, BN = 128, HN = BN / 2;  // rows of a stream, keys of a s
 constexpr int kThreads = 384;
 constexpr int kCopyWarp0 = 0, kMmaWarp0 = 1, kMmaWarp1 = 2, kCopyWarp1 = 3, kFirstSoftmax = 4;
 constexpr int ITEMS = 4;                            // descriptors in flight on each list
-constexpr int kControlRegs = 72, kSoftmaxRegs = 216;  // 128 x 72 + 256 x 216 = 384 x 168, what the block is launched with
+constexpr int kControlRegs = 96, kSoftmaxRegs = 200;  // 128 x 96 + 256 x 200 is what the block is launched with, 384 x 168, or less
 static_assert(128 * kControlRegs + 256 * kSoftmaxRegs <= kThreads * 168, "register shares exceed the launch");
 constexpr int kItemCost = 1;  // steps that an item's queries and result are worth in the lines (0 and 2 left blocks up to 10 % longer at work)
 
@@ -255,7 +255,7 @@ __device__ __forceinline__ void softmax_step(RowState& st, const uint32_t s_addr
         st.m = top;
         st.l *= a;
         if (!first) {
-#pragma unroll
+#pragma unroll 1
             for (int i = 0; i < D / 32; ++i) {
                 uint32_t o[32];
                 tmem_ld32(o_addr + 32 * i, o);
@@ -291,7 +291,8 @@ __device__ __forceinline__ void softmax_step(RowState& st, const uint32_t s_addr
 }
 
 // The sum over keys from .. to - 1 of exp2(c q.k - off) v for one row, by a warp; a lane has D / 32 columns.  For rows whose tile holds
-// keys that they do not see and whose values are not finite: there the product's zero weights give NaN.
+// keys that they do not see and whose values are not finite: there the product's zero weights give NaN.  Eight keys at a time (`from`
+// is a multiple of eight, so they lie in one page): about 60 cycles per key.
 template <int D>
 __device__ __forceinline__ void visible_row(const Params& p, const Item& d, int token, int head, int from, int to, float off, int lane, float (&o)[D / 32]) {
     constexpr int E = D / 32;
@@ -300,19 +301,32 @@ __device__ __forceinline__ void visible_row(const Params& p, const Item& d, int 
 #pragma unroll
     for (int e = 0; e < E; ++e) q[e] = __bfloat162float(src[e]), o[e] = 0;
 #pragma unroll 1
-    for (int j = from; j < to; ++j) {
+    for (int j = from; j < to; j += 8) {
         const int id = p.page_table[(long long)d.b * p.width + (j >> p.page_shift)], at = j & (p.page - 1);
-        const bool there = (unsigned)id < (unsigned)p.num_pages;
+        const bool there = (unsigned)id < (unsigned)p.num_pages;  // a page outside the pool reads as zeros
         const __nv_bfloat16* k = p.k + (there ? id : 0) * p.k_page + at * p.k_token + d.hk * p.k_head + lane * E;
         const __nv_bfloat16* v = p.v + (there ? id : 0) * p.v_page + at * p.v_token + d.hk * p.v_head + lane * E;
-        float s = 0;
+        float s[8], x[8][E];
 #pragma unroll
-        for (int e = 0; e < E; ++e) s += there ? q[e] * __bfloat162float(k[e]) : 0.f;
+        for (int i = 0; i < 8; ++i) {
+            const bool live = there && j + i < to;
+            s[i] = 0;
 #pragma unroll
-        for (int k2 = 16; k2 > 0; k2 >>= 1) s += __shfl_xor_sync(~0u, s, k2);
-        const float x = ex2(fmaf(s, p.c, -off));
+            for (int e = 0; e < E; ++e) {
+                s[i] += live ? q[e] * __bfloat162float(k[i * p.k_token + e]) : 0.f;
+                x[i][e] = live ? __bfloat162float(v[i * p.v_token + e]) : 0.f;
+            }
+        }
 #pragma unroll
-        for (int e = 0; e < E; ++e) o[e] += there ? x * __bfloat162float(v[e]) : 0.f;
+        for (int n = 16; n > 0; n >>= 1)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s[i] += __shfl_xor_sync(~0u, s[i], n);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float w = ex2(fmaf(s[i], p.c, -off));  // times zero behind the last key
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] += w * x[i][e];
+        }
     }
 }
 
@@ -729,12 +743,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
             // All lanes walk the loops on values that the compiler knows to be the same in all of them (see elect_one).
             const int s = warp == kMmaWarp1;
             const uint64_t q_desc = make_smem_desc(q_smem);
-            uint32_t q_ph[2] = {0, 0}, p_ph[2] = {0, 0};
             auto wait_in = [&](int barrier, uint32_t ph, int where) { ok = __all_sync(~0u, ok && wait_bar(bar(barrier), ph, where)); };
-            auto commit = [&](int barrier) {
-                if (ok && elect_one()) umma_commit(bar(barrier));
-                __syncwarp();
-            };
             auto take_uniform = [&](int list, uint32_t& it, Item& d) {
                 Item x;
                 const bool more = take(list, it, x);
@@ -763,12 +772,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
                 };
                 const uint64_t k_desc = make_smem_desc(ring), v_desc = make_mn_desc(ring, BN * 128);
                 Stage next{0, 0};  // the next stage of the ring in the order of the copies
+                uint32_t q_ph[2] = {0, 0}, p_ph[2] = {0, 0};
                 auto wait_q = [&](int t) { wait_in(C::Q_FULL + t, q_ph[t], 81), q_ph[t] ^= 1u; };
                 auto wait_p = [&](int t) {
                     wait_in(C::P_FULL + t, p_ph[t], 82), p_ph[t] ^= 1u;
                     tc_fence_after();
                 };
-                auto scores = [&](int t, const Stage& g) {  // S = Q K^T of stream t
+                // S = Q K^T of stream t; `frees`: the stage has been read, `last`: so have the item's queries
+                auto scores = [&](int t, const Stage& g, bool frees, bool last) {
                     const uint64_t a = q_desc + (uint64_t)(t * (C::Q_BYTES >> 4)), b = k_desc + (uint64_t)(g.at * (C::STAGE_BYTES >> 4));
                     if (ok && elect_one()) {
 #pragma unroll
@@ -777,16 +788,22 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
                             umma_bf16(tmem + C::S_COL + 128 * t, a + o, b + o, C::IDESC_S, k > 0);
                         }
                         umma_commit(bar(C::S_FULL + t));
+                        if (frees) umma_commit(bar(C::PAIR_EMPTY + g.at));
+                        if (last) umma_commit(bar(C::Q_EMPTY + t));
                     }
                     __syncwarp();
                 };
-                auto values = [&](int t, const Stage& g, uint32_t accumulate) {  // O += P V
+                // O += P V of stream t; `ends`: the item has no more of them
+                auto values = [&](int t, const Stage& g, bool accumulate, bool frees, bool ends) {
                     const uint64_t b = v_desc + (uint64_t)(g.at * (C::STAGE_BYTES >> 4));
+                    wait_p(t);
                     if (ok && elect_one()) {
                         umma_bf16_ts(tmem + C::O_COL + D * t, tmem + C::S_COL + 128 * t, b, C::IDESC_O, accumulate);
 #pragma unroll
                         for (int k = 1; k < BN / 16; ++k)
                             umma_bf16_ts(tmem + C::O_COL + D * t, tmem + C::S_COL + 128 * t + 8 * k, b + k * (2048 >> 4), C::IDESC_O, 1u);
+                        if (frees) umma_commit(bar(C::PAIR_EMPTY + g.at));
+                        if (ends) umma_commit(bar(C::O_FULL + t));
                     }
                     __syncwarp();
                 };
@@ -796,13 +813,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
                     wait_in(C::PAIR_FULL + next.at, next.ph, 83);
                     if (n0 > 0) {
                         wait_q(0);
-                        scores(0, next);
-                        if (n0 == 1) commit(C::Q_EMPTY);
+                        scores(0, next, false, n0 == 1);
                     }
                     wait_q(1);
-                    scores(1, next);
-                    if (n1 == 1) commit(C::Q_EMPTY + 1);
-                    commit(C::PAIR_EMPTY + next.at);
+                    scores(1, next, true, n1 == 1);
                     next = next.next();
                     for (int i = 0; i < n1; ++i) {
                         // the next keys, and these values behind them
@@ -812,23 +826,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
                         if (more) wait_in(C::PAIR_FULL + keys.at, keys.ph, 84);
                         wait_in(C::PAIR_FULL + vals.at, vals.ph, 85);
                         clean(ring + vals.at * C::STAGE_BYTES, (d.t0 + i) * BN, BN, d.kv);
-                        if (i < n0) {
-                            wait_p(0);
-                            values(0, vals, i > 0);
-                            if (i + 1 < n0) scores(0, keys);
-                            else commit(C::O_FULL);
-                            if (i + 2 == n0) commit(C::Q_EMPTY);
-                        }
-                        wait_p(1);
-                        values(1, vals, i > 0);
-                        commit(C::PAIR_EMPTY + vals.at);
-                        if (more) {
-                            scores(1, keys);
-                            commit(C::PAIR_EMPTY + keys.at);
-                        } else {
-                            commit(C::O_FULL + 1);
-                        }
-                        if (i + 2 == n1) commit(C::Q_EMPTY + 1);
+                        if (i < n0) values(0, vals, i > 0, false, i + 1 == n0);
+                        if (i + 1 < n0) scores(0, keys, false, i + 2 == n0);
+                        values(1, vals, i > 0, true, !more);
+                        if (more) scores(1, keys, true, i + 2 == n1);
                     }
                 }
                 if (elect_one()) umma_commit(bar(C::PAIRS_DONE));
@@ -859,12 +860,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
                                     umma_bf16(s_col + HN * h, a + (k / 4) * (BM * 128 >> 4) + (k % 4) * 2, b + (k / 4) * (HN * 128 >> 4) + (k % 4) * 2,
                                               C::IDESC_S_SLOT, k > 0);
                                 umma_commit(bar(C::SLOT_EMPTY + first + slot));
+                                if (h == 1) umma_commit(bar(C::S_FULL + 2 + s));
+                                if (h == 1 && i + 1 == n) umma_commit(bar(C::Q_EMPTY + 2 + s));
                             }
                             __syncwarp();
                             advance();
                         }
-                        commit(C::S_FULL + 2 + s);
-                        if (i + 1 == n) commit(C::Q_EMPTY + 2 + s);
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
                             wait_in(C::SLOT_FULL + first + (int)slot, ph, 89);
@@ -880,12 +881,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
 #pragma unroll
                                 for (int k = 1; k < HN / 16; ++k) umma_bf16_ts(o_col, s_col + 32 * h + 8 * k, b + k * (2048 >> 4), C::IDESC_O, 1u);
                                 umma_commit(bar(C::SLOT_EMPTY + first + slot));
+                                if (h == 1 && i + 1 == n) umma_commit(bar(C::O_FULL + 2 + s));
                             }
                             __syncwarp();
                             advance();
                         }
                     }
-                    commit(C::O_FULL + 2 + s);
                 }
             }
             // Every product has ended and every arrival that it owes has been made before the block's memory goes.

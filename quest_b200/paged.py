@@ -140,7 +140,7 @@ def rope_paged_append(
     dev = _device(qkv, table, positions, slots, k_cache, v_cache, q_out)
     strides = _Strides6(*k_cache.stride()[:3], *v_cache.stride()[:3])
     at = ctypes.addressof(strides)
-    _call("rope_paged_append_cuda_bf16", dev, qkv.data_ptr(), max(qkv.stride(0), qkv.size(1)), table.data_ptr(),
+    _call("rope_paged_append_cuda_bf16", dev, qkv.data_ptr(), qkv.stride(0) if rows > 1 else qkv.size(1), table.data_ptr(),
           table.dtype is torch.bfloat16, positions.data_ptr(), slots.data_ptr(), k_cache.data_ptr(), at, v_cache.data_ptr(), at + 24,
           q_out.data_ptr(), rows, n_head, n_kv_head, head_dim, table.size(0), num_pages, page_size)
     return q_out
