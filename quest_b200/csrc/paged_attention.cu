@@ -121,10 +121,6 @@ __device__ __forceinline__ long long pairs_before(const Request& q, int tiles, i
     }
     return sum;
 }
-__device__ __forceinline__ long long pair_places(const Params& p, const Request& q) {
-    const int tiles = pair_tiles(q, p.tokens);
-    return tiles == 0 ? 0 : pairs_before(q, tiles, p.tokens) * p.hkv;
-}
 __device__ __forceinline__ long long single_places(const Params& p, const Request& q) {
     return has_single(q, p.tokens) ? (long long)(steps_of(q.kv) + kItemCost) * p.hkv : 0;
 }
@@ -188,19 +184,17 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
           "r"(r[31]), "r"(taddr)
         : "memory");
 }
-// mbar_wait of tcgen05.cuh without a call: behind one the compiler keeps to the registers of the launch.
-__device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, int where) {
+// A bounded wait (about a second), without a call - behind one the compiler cannot give the roles registers of their own - and
+// short: it stands at some fifty places, and the kernel's time on small calls is the time that its instructions take to arrive.
+constexpr uint32_t kLimitCycles = 2000000000u;
+__device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity) {
     if (mbar_try_wait(bar, parity)) return true;
-    const long long t0 = clock64();
-    while (true) {
-        for (int i = 0; i < 64; ++i)
-            if (mbar_try_wait(bar, parity)) return true;
-        const long long waited = clock64() - t0;
-        if (waited > kWaitLimitFloor && waited > *reinterpret_cast<volatile long long*>(&g_wait_limit_cycles)) {
-            atomicCAS(&g_device_status, 0, (where << 8) | QB200_ERR_DEVICE_TIMEOUT);
-            return false;
-        }
-    }
+    const uint32_t t0 = (uint32_t)clock();
+#pragma unroll 1
+    do {
+        if (mbar_try_wait(bar, parity)) return true;
+    } while ((uint32_t)clock() - t0 < kLimitCycles);
+    return false;
 }
 
 // Weight of a partial result with maximum m (in log2 units) when the common maximum is `top`.
@@ -290,49 +284,60 @@ __device__ __forceinline__ void softmax_step(RowState& st, const uint32_t s_addr
     tmem_st_wait();
 }
 
+// D / 32 neighbouring columns of a row of keys or values.
+template <int D>
+__device__ __forceinline__ void lane_columns(const __nv_bfloat16* src, bool live, float (&x)[D / 32]) {
+    uint2 w = make_uint2(0, 0);
+    if (live) {
+        if (D == 128) w = *reinterpret_cast<const uint2*>(src);
+        else w.x = *reinterpret_cast<const uint32_t*>(src);
+    }
+    x[0] = bf16lo_to_f32(w.x), x[1] = bf16hi_to_f32(w.x);
+    if (D == 128) x[D / 32 - 2] = bf16lo_to_f32(w.y), x[D / 32 - 1] = bf16hi_to_f32(w.y);
+}
+
 // The sum over keys from .. to - 1 of exp2(c q.k - off) v for one row, by a warp; a lane has D / 32 columns.  For rows whose tile holds
-// keys that they do not see and whose values are not finite: there the product's zero weights give NaN.  Eight keys at a time (`from`
-// is a multiple of eight, so they lie in one page): about 60 cycles per key.
+// keys that they do not see and whose values are not finite: there the product's zero weights give NaN.  Four keys at a time (`from`
+// is a multiple of four, so they lie in one page).
 template <int D>
 __device__ __forceinline__ void visible_row(const Params& p, const Item& d, int token, int head, int from, int to, float off, int lane, float (&o)[D / 32]) {
-    constexpr int E = D / 32;
+    constexpr int E = D / 32, KEYS = 4;
     float q[E];
-    const __nv_bfloat16* src = p.q + (long long)(d.start + token) * p.q_token + (long long)head * p.q_head + lane * E;
+    lane_columns<D>(p.q + (long long)(d.start + token) * p.q_token + (long long)head * p.q_head + lane * E, true, q);
 #pragma unroll
-    for (int e = 0; e < E; ++e) q[e] = __bfloat162float(src[e]), o[e] = 0;
+    for (int e = 0; e < E; ++e) o[e] = 0;
 #pragma unroll 1
-    for (int j = from; j < to; j += 8) {
+    for (int j = from; j < to; j += KEYS) {
         const int id = p.page_table[(long long)d.b * p.width + (j >> p.page_shift)], at = j & (p.page - 1);
         const bool there = (unsigned)id < (unsigned)p.num_pages;  // a page outside the pool reads as zeros
         const __nv_bfloat16* k = p.k + (there ? id : 0) * p.k_page + at * p.k_token + d.hk * p.k_head + lane * E;
         const __nv_bfloat16* v = p.v + (there ? id : 0) * p.v_page + at * p.v_token + d.hk * p.v_head + lane * E;
-        float s[8], x[8][E];
+        float s[KEYS], x[KEYS][E];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const bool live = there && j + i < to;
+        for (int i = 0; i < KEYS; ++i) {
+            float y[E];
+            lane_columns<D>(k + i * p.k_token, there && j + i < to, y);
+            lane_columns<D>(v + i * p.v_token, there && j + i < to, x[i]);
             s[i] = 0;
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                s[i] += live ? q[e] * __bfloat162float(k[i * p.k_token + e]) : 0.f;
-                x[i][e] = live ? __bfloat162float(v[i * p.v_token + e]) : 0.f;
-            }
+            for (int e = 0; e < E; ++e) s[i] = fmaf(q[e], y[e], s[i]);
         }
 #pragma unroll
         for (int n = 16; n > 0; n >>= 1)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) s[i] += __shfl_xor_sync(~0u, s[i], n);
+            for (int i = 0; i < KEYS; ++i) s[i] += __shfl_xor_sync(~0u, s[i], n);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float w = ex2(fmaf(s[i], p.c, -off));  // times zero behind the last key
+        for (int i = 0; i < KEYS; ++i) {
+            const float w = j + i < to ? ex2(fmaf(s[i], p.c, -off)) : 0.f;
 #pragma unroll
-            for (int e = 0; e < E; ++e) o[e] += w * x[i][e];
+            for (int e = 0; e < E; ++e) o[e] = fmaf(w, x[i][e], o[e]);
         }
     }
 }
 
 // A worker's place in a line: from u to end, beginning in request b `rest` places behind the request's first.
 struct Place {
-    long long u, end, rest, share;
+    long long u, end, rest, share, per_head;  // per_head: places of the request's pairs and one head
     int b;
     Request q;  // request b
 };
@@ -360,7 +365,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
         for (int i = lane; i < C::NUM_BARS; i += 32) {
             int count = 1;
             if (i >= C::P_FULL && i < C::P_FULL + 4) count = 4;                   // four warps of a stream
-            if (i >= C::LIST_EMPTY && i < C::LIST_EMPTY + ITEMS) count = 10;      // MMA warp, copier of the queries, eight softmax warps
+            if (i >= C::LIST_EMPTY && i < C::LIST_EMPTY + ITEMS) count = 11;      // MMA warps, copier of the queries, eight softmax warps
             if (i >= C::LIST_EMPTY + ITEMS && i < C::LIST_EMPTY + 3 * ITEMS) count = 5;  // MMA warp, four softmax warps
             mbar_init(bar(i), count);
         }
@@ -372,11 +377,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
 
     // ---- the lines: all requests' sums, and the requests in which this block's pieces begin
     Request mine;
-    long long places_of[2], run[2], carry[2] = {0, 0};  // of this thread's request; up to and with it; of all rounds so far
+    long long per_head, places_of[2], run[2], carry[2] = {0, 0};  // of this thread's request; up to and with it; of all rounds so far
     auto sum_round = [&](int b) {
         mine = Request{0, 0, 0};
         if (b < p.batch) mine = request_of(p, b);
-        places_of[0] = run[0] = pair_places(p, mine), places_of[1] = run[1] = single_places(p, mine);
+        per_head = pairs_before(mine, pair_tiles(mine, p.tokens), p.tokens);
+        places_of[0] = run[0] = per_head * p.hkv, places_of[1] = run[1] = single_places(p, mine);
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
 #pragma unroll
@@ -401,24 +407,27 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
             carry[k] += all;
         }
     };
-    for (int b0 = 0; b0 < p.batch; b0 += kThreads) sum_round(b0 + (int)threadIdx.x);
-    const long long total[2] = {carry[0], carry[1]};
-    const long long share[2] = {max((total[0] + blocks - 1) / blocks, 1ll), max((total[1] + 2 * blocks - 1) / (2 * blocks), 1ll)};
+    long long total[2], share[2];
     auto find = [&](int b) {
 #pragma unroll
         for (int w = 0; w < 3; ++w) {
             const int k = w > 0;
             const long long u = share[k] * (w == 2 ? blocks + (int)blockIdx.x : (int)blockIdx.x), before = run[k] - places_of[k];
-            if (u >= before && u < run[k]) places[w] = Place{u, min(u + share[k], total[k]), u - before, share[k], b, mine};
+            if (u >= before && u < run[k]) places[w] = Place{u, min(u + share[k], total[k]), u - before, share[k], per_head, b, mine};
         }
     };
-    if (p.batch <= kThreads) {
-        find((int)threadIdx.x);
-    } else {  // the sums again, now that the places are known
-        carry[0] = carry[1] = 0;
+    for (int pass = 0; pass < 2; ++pass) {  // the totals, then the places
         for (int b0 = 0; b0 < p.batch; b0 += kThreads) {
             sum_round(b0 + (int)threadIdx.x);
-            find(b0 + (int)threadIdx.x);
+            if (pass == 1) find(b0 + (int)threadIdx.x);
+        }
+        if (pass == 0) {
+            total[0] = carry[0], total[1] = carry[1], carry[0] = carry[1] = 0;
+            share[0] = max((total[0] + blocks - 1) / blocks, 1ll), share[1] = max((total[1] + 2 * blocks - 1) / (2 * blocks), 1ll);
+            if (p.batch <= kThreads) {  // this thread's sums are still at hand
+                find((int)threadIdx.x);
+                break;
+            }
         }
     }
     tc_fence_before();
@@ -434,7 +443,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
     auto take = [&](int list, uint32_t& it, Item& d) {
         const uint32_t at = it % ITEMS, ph = (it / ITEMS) & 1u;
         ++it;
-        ok = __all_sync(~0u, ok && wait_bar(bar(C::LIST_FULL + list * ITEMS + at), ph, 70 + list));
+        ok = __all_sync(~0u, ok && wait_bar(bar(C::LIST_FULL + list * ITEMS + at), ph));
         d = items[list * ITEMS + at];
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(C::LIST_EMPTY + list * ITEMS + at));
@@ -466,7 +475,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
                 const int keys = live ? min(max(d.kv - d.n + token + 1, 0), d.kv) : 0x7fffffff;  // a row that is not there needs no mask
                 RowState rs{-CUDART_INF_F, 0.f};
                 for (int i = 0; i < steps; ++i) {
-                    ok = __all_sync(~0u, ok && wait_bar(s_full, s_ph, 79));
+                    ok = __all_sync(~0u, ok && wait_bar(s_full, s_ph));
                     if (!ok) break;
                     s_ph ^= 1u;
                     tc_fence_after();
@@ -476,7 +485,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
                     if (lane == 0) mbar_arrive(p_full);
                 }
                 if (steps > 0) {
-                    ok = __all_sync(~0u, ok && wait_bar(o_full, o_ph, 80));
+                    ok = __all_sync(~0u, ok && wait_bar(o_full, o_ph));
                     o_ph ^= 1u;
                     tc_fence_after();
                 }
@@ -560,7 +569,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
             auto publish = [&](int list, uint32_t& it, const Item& d) {
                 const uint32_t at = it % ITEMS, ph = (it / ITEMS) & 1u;
                 ++it;
-                ok = __all_sync(~0u, ok && wait_bar(bar(C::LIST_EMPTY + list * ITEMS + at), ph ^ 1u, 73));
+                ok = __all_sync(~0u, ok && wait_bar(bar(C::LIST_EMPTY + list * ITEMS + at), ph ^ 1u));
                 if (lane == 0) {
                     items[list * ITEMS + at] = d;
                     mbar_arrive(bar(C::LIST_FULL + list * ITEMS + at));
@@ -569,7 +578,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
             };
             auto load_queries = [&](int tile, int set, uint32_t& ph, int token, int hk, bool upper) {
                 const uint32_t full = bar(C::Q_FULL + 2 * set + tile);
-                ok = __all_sync(~0u, ok && wait_bar(bar(C::Q_EMPTY + 2 * set + tile), ph ^ 1u, 74));
+                ok = __all_sync(~0u, ok && wait_bar(bar(C::Q_EMPTY + 2 * set + tile), ph ^ 1u));
                 ph ^= 1u;
                 if (ok && lane == 0) {
                     mbar_arrive_expect_tx(full, (upper ? p.half_tokens : p.tokens) * p.group * D * 2);
@@ -592,7 +601,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
             if (has_pairs && s == 0) {
                 uint32_t it = 0, stage = 0, ph = 0;
                 auto load = [&](const CUtensorMap* map, const Item& d, int step, int id) {
-                    ok = __all_sync(~0u, ok && wait_bar(bar(C::PAIR_EMPTY + stage), ph ^ 1u, 75));
+                    ok = __all_sync(~0u, ok && wait_bar(bar(C::PAIR_EMPTY + stage), ph ^ 1u));
                     if (!ok) return;
                     const uint32_t full = bar(C::PAIR_FULL + stage);
                     if (lane == 0) mbar_arrive_expect_tx(full, C::STAGE_BYTES);
@@ -605,15 +614,16 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
                 Request q = w.q;
                 int tiles = pair_tiles(q, p.tokens);
                 long long rest = w.rest;
-                const long long per_head = pairs_before(q, tiles, p.tokens);
-                int hk = (int)(rest / per_head);
-                rest -= hk * per_head;
+                int hk = (int)(rest / w.per_head);
+                rest -= hk * w.per_head;
                 int tile = 0, hi = tiles - 1;  // the last tile that begins at or before the place
+                long long begin = 0;
                 while (tile < hi) {
                     const int mid = (tile + hi + 1) >> 1;
-                    if (pairs_before(q, mid, p.tokens) <= rest) tile = mid; else hi = mid - 1;
+                    const long long at = pairs_before(q, mid, p.tokens);
+                    if (at <= rest) tile = mid, begin = at; else hi = mid - 1;
                 }
-                int off = (int)(rest - pairs_before(q, tile, p.tokens));
+                int off = (int)(rest - begin);
                 Item d;
                 for (long long u = w.u; ok && u < w.end;) {
                     d.start = q.start, d.n = q.n, d.kv = q.kv, d.b = b, d.hk = hk, d.tok0 = tile * 2 * p.tokens, d.last = 0;
@@ -671,14 +681,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
             const Place w = places[1 + s];
             if (w.b >= 0) {
                 // The pairs' products have read the ring and the queries: now each stream has a half.
-                if (has_pairs) ok = __all_sync(~0u, ok && wait_bar(bar(C::PAIRS_DONE), 0, 77));
+                if (has_pairs) ok = __all_sync(~0u, ok && wait_bar(bar(C::PAIRS_DONE), 0));
                 const uint32_t own = ring + s * (C::STAGES * C::SLOT_BYTES), first = (uint32_t)(s * C::STAGES);
                 const int id = s * blocks + (int)blockIdx.x;
                 uint32_t it = 0, slot = 0, ph = 0, q_ph = 0;
                 auto load = [&](const CUtensorMap* map, const Item& d, int step, int page_id) {
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        ok = __all_sync(~0u, ok && wait_bar(bar(C::SLOT_EMPTY + first + slot), ph ^ 1u, 78));
+                        ok = __all_sync(~0u, ok && wait_bar(bar(C::SLOT_EMPTY + first + slot), ph ^ 1u));
                         if (!ok) return;
                         const uint32_t full = bar(C::SLOT_FULL + first + slot);
                         if (lane == 0) mbar_arrive_expect_tx(full, C::SLOT_BYTES);
@@ -743,7 +753,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
             // All lanes walk the loops on values that the compiler knows to be the same in all of them (see elect_one).
             const int s = warp == kMmaWarp1;
             const uint64_t q_desc = make_smem_desc(q_smem);
-            auto wait_in = [&](int barrier, uint32_t ph, int where) { ok = __all_sync(~0u, ok && wait_bar(bar(barrier), ph, where)); };
+            auto wait_in = [&](int barrier, uint32_t ph) { ok = __all_sync(~0u, ok && wait_bar(bar(barrier), ph)); };
             auto take_uniform = [&](int list, uint32_t& it, Item& d) {
                 Item x;
                 const bool more = take(list, it, x);
@@ -773,9 +783,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
                 const uint64_t k_desc = make_smem_desc(ring), v_desc = make_mn_desc(ring, BN * 128);
                 Stage next{0, 0};  // the next stage of the ring in the order of the copies
                 uint32_t q_ph[2] = {0, 0}, p_ph[2] = {0, 0};
-                auto wait_q = [&](int t) { wait_in(C::Q_FULL + t, q_ph[t], 81), q_ph[t] ^= 1u; };
+                auto wait_q = [&](int t) { wait_in(C::Q_FULL + t, q_ph[t]), q_ph[t] ^= 1u; };
                 auto wait_p = [&](int t) {
-                    wait_in(C::P_FULL + t, p_ph[t], 82), p_ph[t] ^= 1u;
+                    wait_in(C::P_FULL + t, p_ph[t]), p_ph[t] ^= 1u;
                     tc_fence_after();
                 };
                 // S = Q K^T of stream t; `frees`: the stage has been read, `last`: so have the item's queries
@@ -810,7 +820,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
                 Item d;
                 for (uint32_t it = 0; take_uniform(0, it, d);) {
                     const int n0 = d.steps[0], n1 = d.steps[1];
-                    wait_in(C::PAIR_FULL + next.at, next.ph, 83);
+                    wait_in(C::PAIR_FULL + next.at, next.ph);
                     if (n0 > 0) {
                         wait_q(0);
                         scores(0, next, false, n0 == 1);
@@ -823,8 +833,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
                         const bool more = i + 1 < n1;
                         const Stage keys = next, vals = more ? next.next() : next;
                         next = vals.next();
-                        if (more) wait_in(C::PAIR_FULL + keys.at, keys.ph, 84);
-                        wait_in(C::PAIR_FULL + vals.at, vals.ph, 85);
+                        if (more) wait_in(C::PAIR_FULL + keys.at, keys.ph);
+                        wait_in(C::PAIR_FULL + vals.at, vals.ph);
                         clean(ring + vals.at * C::STAGE_BYTES, (d.t0 + i) * BN, BN, d.kv);
                         if (i < n0) values(0, vals, i > 0, false, i + 1 == n0);
                         if (i + 1 < n0) scores(0, keys, false, i + 2 == n0);
@@ -834,9 +844,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
                 }
                 if (elect_one()) umma_commit(bar(C::PAIRS_DONE));
                 __syncwarp();
+            } else if (has_pairs) {  // only follows, so that its wait for the pairs' end is a short one
+                Item d;
+                for (uint32_t it = 0; take(0, it, d);) {
+                }
             }
             if (places[1 + s].b >= 0) {
-                if (has_pairs) wait_in(C::PAIRS_DONE, 0, 86);
+                if (has_pairs) wait_in(C::PAIRS_DONE, 0);
                 const uint32_t own = ring + s * (C::STAGES * C::SLOT_BYTES);
                 const int first = s * C::STAGES;
                 const uint64_t k_desc = make_smem_desc(own), v_desc = make_mn_desc(own, HN * 128), a = q_desc + (uint64_t)(s * (C::Q_BYTES >> 4));
@@ -848,11 +862,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
                 Item d;
                 for (uint32_t it = 0; take_uniform(1 + s, it, d);) {
                     const int n = d.steps[s];
-                    wait_in(C::Q_FULL + 2 + s, q_parity, 87), q_parity ^= 1u;
+                    wait_in(C::Q_FULL + 2 + s, q_parity), q_parity ^= 1u;
                     for (int i = 0; ok && i < n; ++i) {
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            wait_in(C::SLOT_FULL + first + (int)slot, ph, 88);
+                            wait_in(C::SLOT_FULL + first + (int)slot, ph);
                             const uint64_t b = k_desc + (uint64_t)(slot * (C::SLOT_BYTES >> 4));
                             if (ok && elect_one()) {
 #pragma unroll
@@ -868,10 +882,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
                         }
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            wait_in(C::SLOT_FULL + first + (int)slot, ph, 89);
+                            wait_in(C::SLOT_FULL + first + (int)slot, ph);
                             clean(own + slot * C::SLOT_BYTES, (d.t0 + i) * BN + h * HN, HN, d.kv);
                             if (h == 0) {
-                                wait_in(C::P_FULL + 2 + s, p_parity, 90), p_parity ^= 1u;
+                                wait_in(C::P_FULL + 2 + s, p_parity), p_parity ^= 1u;
                                 tc_fence_after();
                             }
                             const uint64_t b = v_desc + (uint64_t)(slot * (C::SLOT_BYTES >> 4));
@@ -892,9 +906,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
             // Every product has ended and every arrival that it owes has been made before the block's memory goes.
             if (elect_one()) umma_commit(bar(C::DONE + s));
             __syncwarp();
-            wait_bar(bar(C::DONE + s), 0, 91);
+            ok = __all_sync(~0u, wait_bar(bar(C::DONE + s), 0)) && ok;
         }
     }
+    if (!ok && lane == 0) atomicCAS(&g_device_status, 0, ((70 + warp) << 8) | QB200_ERR_DEVICE_TIMEOUT);
     tc_fence_before();
     __syncthreads();
     if (warp == kMmaWarp0) {
