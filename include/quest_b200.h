@@ -361,11 +361,13 @@ int rope_paged_append_cuda_bf16(const void* qkv, long long ld, const void* table
  * Attention of new tokens over the pages.  Rows cu_new[b] .. cu_new[b + 1] - 1 of q [rows, n_head, head_dim] are the last tokens of
  * request b, whose kv_lens[b] tokens lie in its pages; row t of n sees the keys 0 .. kv_lens[b] - n + t:
  *   out = softmax(scale * q . k) . v,  query head h over key and value head h / (n_head / n_kv_head).
- * A row that sees no key gives zeros; rows outside every request stay as they were.  Keys and values behind kv_lens[b] are not
- * looked at, whatever they hold.  Strides in elements: q, out (token, head); caches (page, token, head).
- * head_dim 64 or 128; page_size a power of two from 16 to 1024; n_head a multiple of n_kv_head; strides multiples of 8, bases
- * 16-byte aligned (QB200_ERR_UNSUPPORTED otherwise).  workspace: paged_attention_workspace(...) bytes, 16-byte aligned, used by
- * this call alone while it runs.
+ * A row that sees no key gives zeros; rows outside every request stay as they were.  What the pages hold behind kv_lens[b] does
+ * not matter, nor does what a row does not see (later tokens of its chunk that are not finite); a page table entry outside the pool
+ * reads as keys and values of 0.  Strides in elements: q, out (token, head); caches (page, token, head).  Results do not depend on
+ * timing: the same call gives the same bits.
+ * head_dim 64 or 128; page_size a power of two from 16 to 1024; n_head a multiple of n_kv_head, at most 128 times it; width * page_size at
+ * most 2^25; strides multiples of 8, bases 16-byte aligned (QB200_ERR_UNSUPPORTED otherwise); scale not negative.  workspace:
+ * paged_attention_workspace(...) bytes for the current device, 16-byte aligned, used by this call alone while it runs.  Two kernels.
  */
 int paged_attention_cuda_bf16(void* out, const long long* out_strides, const void* q, const long long* q_strides,
                               const void* k_cache, const long long* k_strides, const void* v_cache, const long long* v_strides,

@@ -167,10 +167,11 @@ def paged_attention(
 
     Rows ``cu_new[b] .. cu_new[b + 1] - 1`` of q [rows, n_head, head_dim] bf16 are the last tokens of request b, whose
     ``kv_lens[b]`` tokens (the new ones among them) lie in the pages ``page_table[b]``: one row while decoding, a chunk of a
-    prompt, drafted tokens, or a mixture over the batch.  Query head h reads key and value head h / (n_head / n_kv_head).  Rows
-    that see no key (kv_lens 0: refused by ``page_assign``) give zeros; rows outside every request are not written.  What the
-    pages hold behind a request's tokens does not matter.  head_dim 64 or 128, page_size a power of two from 16 to 1024;
-    q and out may be views (strides in multiples of 8 elements)."""
+    prompt, drafted tokens, or a mixture over the batch.  Query head h reads key and value head h / (n_head / n_kv_head), at most
+    128 of them the same.  Rows that see no key (kv_lens 0: refused by ``page_assign``) give zeros; rows outside every request are
+    not written.  What the pages hold behind a request's tokens does not matter, nor what a row does not see (later tokens of its
+    chunk, whatever they are).  head_dim 64 or 128, page_size a power of two from 16 to 1024; q and out may be views (strides in
+    multiples of 8 elements).  For inference: nothing is recorded for autograd."""
     _check_caches(k_cache, v_cache)
     num_pages, page_size, n_kv_head, head_dim = k_cache.shape
     assert q.dtype == torch.bfloat16 and q.dim() == 3 and q.stride(2) == 1 and q.size(2) == head_dim

@@ -146,3 +146,15 @@ def test_no_cpu_fallback(op):
 def test_arguments_are_checked(op, bad):
     with pytest.raises(AssertionError):
         op(**bad)
+
+
+def test_attention_entry_refuses_scales_and_groups():
+    lib = _lib.load()
+    buf, p = aligned_buffer()
+    two, three = (ctypes.c_longlong * 2)(64 * 256, 64), (ctypes.c_longlong * 3)(1024, 64, 64)
+
+    def call(scale=0.1, hq=2, page=16, width=3):
+        return lib.paged_attention_cuda_bf16(p, two, p, two, p, three, p, three, p, p, p, p, scale, 2, 1, width, hq, 1, 64, 4, page, None)
+
+    assert call(scale=-1.0) == INVALID and call(scale=float("nan")) == INVALID
+    assert call(hq=129) == UNSUPPORTED and call(page=2048) == UNSUPPORTED and call(width=(1 << 21) + 1) == UNSUPPORTED
