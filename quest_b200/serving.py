@@ -56,7 +56,7 @@ class PagedCache:
 
     def shorten(self, keep_lens: torch.Tensor) -> None:
         """Request b keeps its first ``keep_lens[b]`` tokens (0: it has finished and its place can be used again)."""
-        keep = torch.minimum(keep_lens, self.lens)
+        keep = torch.minimum(keep_lens, self.lens).clamp(min=0)
         self.free_count.copy_(quest.page_release(self.page_table, self.free_pages, self.free_count, self.lens, keep, self.page_size))
         self.lens.copy_(keep)
 
@@ -86,11 +86,13 @@ def generate(model: Decoder, cache: PagedCache, prompts: list[torch.Tensor], max
     device = cache.lens.device
     if n > slots or any(p.numel() == 0 for p in prompts):
         raise ValueError("more prompts than places, or an empty prompt")
-    longest = max(p.numel() for p in prompts) + max_new
-    if longest > cache.page_table.size(1) * cache.page_size or sum(-(-(p.numel() + max_new) // cache.page_size) for p in prompts) > cache.num_pages:
-        raise ValueError("the cache has too few pages for these prompts and their continuation")
     if bool((cache.lens[:n] != 0).any()):
         raise ValueError("places of the cache are in use")
+    held = [p.numel() + max(max_new - 1, 0) for p in prompts]  # the last new token is not kept
+    if max(held, default=0) > cache.page_table.size(1) * cache.page_size or sum(-(-h // cache.page_size) for h in held) > int(cache.free_count):
+        raise ValueError("the cache has too few free pages for these prompts and their continuation")
+    if n == 0:
+        return torch.empty(0, max_new, dtype=torch.long, device=device)
     new = torch.zeros(slots, dtype=torch.int32, device=device)
     new[:n] = torch.tensor([p.numel() for p in prompts], dtype=torch.int32, device=device)
     hidden, step = extend(model, cache, torch.cat([p.to(device) for p in prompts]), new)
@@ -109,19 +111,33 @@ def generate(model: Decoder, cache: PagedCache, prompts: list[torch.Tensor], max
 
 @torch.inference_mode()
 def verify(model: Decoder, cache: PagedCache, tokens: torch.Tensor, drafts: torch.Tensor, uniforms: torch.Tensor,
-           draft_probs: torch.Tensor = None) -> tuple[torch.Tensor, torch.Tensor]:
+           draft_probs: torch.Tensor = None, active: torch.Tensor = None) -> tuple[torch.Tensor, torch.Tensor]:
     """One step of speculative decoding for all places of the cache: ``tokens`` [R], the last token of each request, which is not
     in the cache yet, and ``drafts`` [R, K] drafted behind it run through the model in one pass, drafts that the target refuses are taken
     out of the cache again.  ``uniforms`` [R, K + 1] fp32 in [0, 1); ``draft_probs`` [R, K, vocab] fp32.  Returns (new tokens
-    [R, K + 1], -1 behind the last one; drafts kept [R]); the last new token is the next call's ``tokens``."""
+    [R, K + 1], -1 behind the last one; drafts kept [R]); the last new token is the next call's ``tokens``.  Places that are not
+    ``active`` ([R] bool; all are by default) stay as they are, whatever their tokens are; they, and requests for which there are not
+    enough pages, get -1 throughout and 0."""
     requests, count = drafts.shape
-    device = cache.lens.device
+    rows, device = requests * (count + 1), cache.lens.device
     before = cache.lens.clone()
     new = torch.full((requests,), count + 1, dtype=torch.int32, device=device)
-    hidden, _ = extend(model, cache, torch.cat([tokens[:, None], drafts], dim=1).view(-1), new)
+    packed = torch.cat([tokens[:, None], drafts], dim=1).view(-1)
+    if active is not None:  # the active places' tokens move together; place b's begin at its row of the packed batch
+        new = torch.where(active, new, 0)
+        ends = new.cumsum(0)
+        at = ((ends - new)[:, None] + torch.arange(count + 1, device=device)).view(-1)
+        idle = ~active.repeat_interleave(count + 1, output_size=rows)
+        packed = packed.new_zeros(rows + 1).scatter_(0, at.masked_fill(idle, rows), packed)[:rows]
+    hidden, step = extend(model, cache, packed, new)
+    if active is not None:
+        hidden = hidden[at.clamp(max=rows - 1)]
     probs = torch.softmax(model.lm_head(hidden).float(), dim=-1)
-    cu = torch.arange(0, (requests + 1) * count, max(count, 1), dtype=torch.int32, device=device)[:requests + 1] if count else torch.zeros(requests + 1, dtype=torch.int32, device=device)
+    cu = torch.arange(requests + 1, dtype=torch.int32, device=device) * count
     result, kept = quest.verify_drafts(probs, drafts.reshape(-1), cu, uniforms.reshape(-1), count,
                                        draft_probs=None if draft_probs is None else draft_probs.reshape(requests * count, -1))
-    cache.shorten(before + 1 + kept)
-    return result, kept
+    served = step.kv_lens > 0
+    if active is not None:
+        served &= active
+    cache.shorten(torch.where(served, before + 1 + kept, before))
+    return torch.where(served[:, None], result, -1), torch.where(served, kept, 0)

@@ -201,3 +201,60 @@ def test_requests_without_pages_are_refused_and_recover():
     assert cache.free_count.item() == 3
     _, step = serving.extend(model, cache, prompts_of([30])[0].cuda(), torch.tensor([0, 30], dtype=torch.int32, device="cuda"))
     assert step.kv_lens.tolist() == [0, 30]
+
+
+def test_verify_leaves_places_that_are_not_active():
+    """Active places give what a step of them alone gives (rows of a batch do not depend on their places in it, attention sums in
+    the order that the split of the work gives, and the tokens' probabilities are nearly all on one); the others stay as they are."""
+    model = make_model("bf16")
+    model.lm_head.weight.data.mul_(200)
+    prompts, count = prompts_of([10, 20, 25]), 3
+    both, alone = (serving.PagedCache(CFG, 16, n, page_size=16) for n in (4, 2))
+    i32 = dict(dtype=torch.int32, device="cuda")
+    serving.extend(model, both, torch.cat(prompts).cuda(), torch.tensor([10, 20, 0, 25], **i32))
+    serving.extend(model, alone, torch.cat([prompts[0], prompts[2]]).cuda(), torch.tensor([10, 25], **i32))
+    last = torch.tensor([7, 400, -1, 11], device="cuda")  # what stands at the other places is never looked up
+    drafts = torch.randint(0, CFG.vocab_size, (4, count), generator=torch.Generator().manual_seed(3)).cuda()
+    drafts[2] = 10 ** 6
+    chain = serving.generate(model, serving.PagedCache(CFG, 16, 2, page_size=16),
+                             [torch.cat([p, t.cpu()[None]]) for p, t in zip([prompts[0], prompts[2]], last[[0, 3]])], count)
+    drafts[0], drafts[3, :1] = chain[0], chain[1, :1]
+    u = torch.full((4, count + 1), 0.5, device="cuda")
+    active = torch.tensor([True, False, False, True], device="cuda")
+    tokens, kept = serving.verify(model, both, last, drafts, u, active=active)
+    expected, kept_alone = serving.verify(model, alone, last[[0, 3]], drafts[[0, 3]], u[:2])
+    assert torch.equal(tokens[[0, 3]], expected) and kept[[0, 3]].tolist() == kept_alone.tolist() and kept[0].item() == count
+    assert (tokens[[1, 2]] == -1).all() and kept[[1, 2]].tolist() == [0, 0]
+    assert both.lens.tolist() == [11 + kept[0].item(), 20, 0, 26 + kept[3].item()]
+    assert both.free_count.item() == 16 - sum(-(-n // 16) for n in both.lens.tolist())
+
+
+def test_verify_answers_nothing_for_a_request_without_pages():
+    model = make_model("bf16")
+    cache = serving.PagedCache(CFG, 3, 2, page_size=16)
+    serving.extend(model, cache, prompts_of([46])[0].cuda(), torch.tensor([30, 16], dtype=torch.int32, device="cuda"))
+    drafts = torch.zeros(2, 1, dtype=torch.long, device="cuda")
+    tokens, kept = serving.verify(model, cache, torch.tensor([1, 2], device="cuda"), drafts, torch.full((2, 2), 0.5, device="cuda"))
+    assert tokens[0, 0].item() >= 0 and tokens[1].tolist() == [-1, -1] and kept[1].item() == 0
+    assert cache.lens.tolist() == [31 + kept[0].item(), 16] and cache.free_count.item() == 0
+
+
+def test_generate_counts_the_pages_that_are_free():
+    """Pages that another place holds are not there for new prompts; the last new token needs no room."""
+    model = make_model("bf16")
+    cache = serving.PagedCache(CFG, 3, 2, page_size=16)
+    held = torch.tensor([0, 20], dtype=torch.int32, device="cuda")
+    serving.extend(model, cache, prompts_of([20])[0].cuda(), held)
+    with pytest.raises(ValueError):
+        serving.generate(model, cache, prompts_of([10]), 8)
+    assert serving.generate(model, cache, prompts_of([10]), 7).shape == (1, 7)
+    assert cache.lens.tolist() == [0, 20] and cache.free_count.item() == 1
+    assert serving.generate(model, cache, [], 4).shape == (0, 4)
+
+
+def test_shorten_takes_negative_lengths_for_zero():
+    model = make_model("bf16")
+    cache = serving.PagedCache(CFG, 4, 2, page_size=16)
+    serving.extend(model, cache, prompts_of([40])[0].cuda(), torch.tensor([20, 20], dtype=torch.int32, device="cuda"))
+    cache.shorten(torch.tensor([-5, 100], dtype=torch.int32, device="cuda"))
+    assert cache.lens.tolist() == [0, 20] and cache.free_count.item() == 2
