@@ -19,17 +19,16 @@ from . import _lib
 _Strides6, _Strides10 = ctypes.c_longlong * 6, ctypes.c_longlong * 10
 
 
-def _device(*tensors: torch.Tensor) -> int:
-    """The CUDA device that all of them are on."""
-    device = tensors[0].get_device()
-    for t in tensors:
-        if not t.is_cuda or t.get_device() != device:
-            _lib.require_cuda(*tensors)
-    return device
+# These calls are short (a few microseconds on the device), so what Python does around them counts: types are compared by
+# identity, devices by index, and entry points looked up once.
+_i32, _bf16 = torch.int32, torch.bfloat16
+_entries: dict = {}
 
 
 def _call(name: str, device: int, *args) -> None:
-    fn = getattr(_lib.load(), name)
+    fn = _entries.get(name)
+    if fn is None:
+        fn = _entries[name] = getattr(_lib.load(), name)
     if torch._C._cuda_getDevice() == device:
         status = fn(*args, torch._C._cuda_getCurrentRawStream(device))
     else:
@@ -49,11 +48,6 @@ class PageStep(NamedTuple):
     free_count: torch.Tensor  # [1] free pages after the step
 
 
-def _check_i32(*tensors: torch.Tensor) -> None:
-    for t in tensors:
-        assert t.dtype is torch.int32 and t.is_contiguous()
-
-
 def page_assign(
         page_table: torch.Tensor,
         free_pages: torch.Tensor,
@@ -71,11 +65,15 @@ def page_assign(
     Requests are served in order.  One whose rows, table row or pages do not suffice is refused as a whole: it gets no page, its
     rows the slot -1 and its ``kv_lens`` is 0; where rows or pages have run out, so are the later ones that come behind them or need
     a page.  Negative lengths count as 0.  At most 8192 requests."""
-    _check_i32(page_table, free_pages, free_count, cached_lens, new_lens)
+    assert page_table.dtype is free_pages.dtype is free_count.dtype is cached_lens.dtype is new_lens.dtype is _i32
+    assert (page_table.is_contiguous() and free_pages.is_contiguous() and free_count.is_contiguous() and cached_lens.is_contiguous()
+            and new_lens.is_contiguous())
     assert page_table.dim() == 2 and free_pages.dim() == 1 and free_count.numel() == 1 and page_size > 0 and num_tokens >= 0
     batch, width = page_table.shape
-    assert cached_lens.shape == (batch,) and new_lens.shape == (batch,)
-    dev = _device(page_table, free_pages, free_count, cached_lens, new_lens)
+    assert cached_lens.shape == new_lens.shape == (batch,)
+    dev = page_table.get_device()
+    if dev < 0 or not dev == free_pages.get_device() == free_count.get_device() == cached_lens.get_device() == new_lens.get_device():
+        _lib.require_cuda(page_table, free_pages, free_count, cached_lens, new_lens)
     cu, kv_lens, lens, positions, left = torch.split_with_sizes(page_table.new_empty(3 * batch + num_tokens + 2),
                                                                 (batch + 1, batch, batch, num_tokens, 1))
     slots = page_table.new_empty(num_tokens, dtype=torch.int64)
@@ -96,20 +94,19 @@ def page_release(
     """Shortens request b from ``lens[b]`` to ``keep_lens[b]`` tokens (0: it has finished): the pages behind them go to the end of
     the stack ``free_pages[:free_count]``.  Returns the new count [1]; the page table is left as it is (what lies behind a
     request's length has no meaning).  ``free_pages`` must have room for every page of the pool."""
-    _check_i32(page_table, free_pages, free_count, lens, keep_lens)
+    assert page_table.dtype is free_pages.dtype is free_count.dtype is lens.dtype is keep_lens.dtype is _i32
+    assert (page_table.is_contiguous() and free_pages.is_contiguous() and free_count.is_contiguous() and lens.is_contiguous()
+            and keep_lens.is_contiguous())
     assert page_table.dim() == 2 and free_pages.dim() == 1 and free_count.numel() == 1 and page_size > 0
     batch, width = page_table.shape
-    assert lens.shape == (batch,) and keep_lens.shape == (batch,)
-    dev = _device(page_table, free_pages, free_count, lens, keep_lens)
+    assert lens.shape == keep_lens.shape == (batch,)
+    dev = page_table.get_device()
+    if dev < 0 or not dev == free_pages.get_device() == free_count.get_device() == lens.get_device() == keep_lens.get_device():
+        _lib.require_cuda(page_table, free_pages, free_count, lens, keep_lens)
     left = free_count.new_empty(1)
     _call("page_release_cuda", dev, page_table.data_ptr(), free_pages.data_ptr(), free_count.data_ptr(), lens.data_ptr(),
           keep_lens.data_ptr(), left.data_ptr(), batch, width, free_pages.numel(), page_size)
     return left
-
-
-def _check_caches(k_cache: torch.Tensor, v_cache: torch.Tensor) -> None:
-    assert k_cache.dtype == torch.bfloat16 and v_cache.dtype == torch.bfloat16
-    assert k_cache.dim() == 4 and v_cache.shape == k_cache.shape and k_cache.stride(3) == 1 and v_cache.stride(3) == 1
 
 
 def rope_paged_append(
@@ -127,21 +124,25 @@ def rope_paged_append(
     caches [num_pages, page_size, n_kv_head, head_dim].  Returns the queries [rows, n_head, head_dim].  Rows with a slot or a
     position outside (``page_assign`` gives -1 to rows that are not in use) are left out: nothing of them is written.  The slots
     of one call must differ."""
-    _check_caches(k_cache, v_cache)
     num_pages, page_size, n_kv_head, head_dim = k_cache.shape
-    assert qkv.dtype == torch.bfloat16 and qkv.dim() == 2 and qkv.stride(1) == 1 and qkv.size(1) == (n_head + 2 * n_kv_head) * head_dim
+    k_strides, v_strides = k_cache.stride(), v_cache.stride()
+    assert k_cache.dtype is v_cache.dtype is _bf16 and v_cache.shape == k_cache.shape and k_strides[3] == v_strides[3] == 1
+    assert qkv.dtype is _bf16 and qkv.dim() == 2 and qkv.stride(1) == 1 and qkv.size(1) == (n_head + 2 * n_kv_head) * head_dim
     rows = qkv.size(0)
-    assert table.dtype in (torch.bfloat16, torch.float32) and table.is_contiguous() and table.shape[1:] == (head_dim // 2, 2)
-    _check_i32(positions)
-    assert slots.dtype == torch.int64 and slots.is_contiguous() and positions.shape == (rows,) and slots.shape == (rows,)
+    assert (table.dtype is _bf16 or table.dtype is torch.float32) and table.is_contiguous() and table.shape[1:] == (head_dim // 2, 2)
+    assert positions.dtype is _i32 and slots.dtype is torch.int64 and positions.is_contiguous() and slots.is_contiguous()
+    assert positions.shape == slots.shape == (rows,)
     if q_out is None:
         q_out = qkv.new_empty((rows, n_head, head_dim))
-    assert q_out.shape == (rows, n_head, head_dim) and q_out.dtype == torch.bfloat16 and q_out.is_contiguous()
-    dev = _device(qkv, table, positions, slots, k_cache, v_cache, q_out)
-    strides = _Strides6(*k_cache.stride()[:3], *v_cache.stride()[:3])
+    assert q_out.shape == (rows, n_head, head_dim) and q_out.dtype is _bf16 and q_out.is_contiguous()
+    dev = qkv.get_device()
+    if dev < 0 or not (dev == table.get_device() == positions.get_device() == slots.get_device() == k_cache.get_device() == v_cache.get_device()
+                       == q_out.get_device()):
+        _lib.require_cuda(qkv, table, positions, slots, k_cache, v_cache, q_out)
+    strides = _Strides6(*k_strides[:3], *v_strides[:3])
     at = ctypes.addressof(strides)
     _call("rope_paged_append_cuda_bf16", dev, qkv.data_ptr(), qkv.stride(0) if rows > 1 else qkv.size(1), table.data_ptr(),
-          table.dtype is torch.bfloat16, positions.data_ptr(), slots.data_ptr(), k_cache.data_ptr(), at, v_cache.data_ptr(), at + 24,
+          table.dtype is _bf16, positions.data_ptr(), slots.data_ptr(), k_cache.data_ptr(), at, v_cache.data_ptr(), at + 24,
           q_out.data_ptr(), rows, n_head, n_kv_head, head_dim, table.size(0), num_pages, page_size)
     return q_out
 
@@ -171,21 +172,26 @@ def paged_attention(
     128 of them the same.  Rows that see no key (kv_lens 0: refused by ``page_assign``) give zeros; rows outside every request are
     not written.  What the pages hold behind a request's tokens does not matter, nor what a row does not see (later tokens of its
     chunk, whatever they are).  head_dim 64 or 128, page_size a power of two from 16 to 1024; q and out may be views (strides in
-    multiples of 8 elements).  For inference: nothing is recorded for autograd."""
-    _check_caches(k_cache, v_cache)
+    multiples of 8 elements), out without memory in common with the inputs.  For inference: nothing is recorded for autograd."""
     num_pages, page_size, n_kv_head, head_dim = k_cache.shape
-    assert q.dtype == torch.bfloat16 and q.dim() == 3 and q.stride(2) == 1 and q.size(2) == head_dim
-    rows, n_head = q.size(0), q.size(1)
-    _check_i32(page_table, kv_lens, cu_new)
-    assert page_table.dim() == 2
+    rows, n_head, columns = q.shape
     batch, width = page_table.shape
+    q_strides, k_strides, v_strides = q.stride(), k_cache.stride(), v_cache.stride()
+    assert q.dtype is k_cache.dtype is v_cache.dtype is _bf16 and v_cache.shape == k_cache.shape and columns == head_dim
+    assert q_strides[2] == k_strides[3] == v_strides[3] == 1
+    assert page_table.dtype is kv_lens.dtype is cu_new.dtype is _i32
+    assert page_table.is_contiguous() and kv_lens.is_contiguous() and cu_new.is_contiguous()
     assert kv_lens.shape == (batch,) and cu_new.shape == (batch + 1,)
     if out is None:
         out = q.new_empty((rows, n_head, head_dim))
-    assert out.shape == q.shape and out.dtype == torch.bfloat16 and out.stride(2) == 1
-    dev = _device(q, k_cache, v_cache, page_table, kv_lens, cu_new, out)
+    out_strides = out.stride()
+    assert out.shape == q.shape and out.dtype is _bf16 and out_strides[2] == 1
+    dev = q.get_device()
+    if dev < 0 or not (dev == k_cache.get_device() == v_cache.get_device() == page_table.get_device() == kv_lens.get_device()
+                       == cu_new.get_device() == out.get_device()):
+        _lib.require_cuda(q, k_cache, v_cache, page_table, kv_lens, cu_new, out)
     workspace = q.new_empty(_workspace(dev, rows, n_head // n_kv_head if n_kv_head else 0, head_dim))
-    strides = _Strides10(*out.stride()[:2], *q.stride()[:2], *k_cache.stride()[:3], *v_cache.stride()[:3])
+    strides = _Strides10(*out_strides[:2], *q_strides[:2], *k_strides[:3], *v_strides[:3])
     at = ctypes.addressof(strides)
     _call("paged_attention_cuda_bf16", dev, out.data_ptr(), at, q.data_ptr(), at + 16, k_cache.data_ptr(), at + 32, v_cache.data_ptr(), at + 56,
           page_table.data_ptr(), kv_lens.data_ptr(), cu_new.data_ptr(), workspace.data_ptr(), head_dim ** -0.5 if scale is None else float(scale),
@@ -210,18 +216,21 @@ def verify_drafts(
     the last uniform from max(target - draft, 0) of the first refused row, or from the row behind the last draft: the first whose
     running sum (in 64 bits) passes u times the total.  ``tokens`` holds the kept drafts, that token, and -1 behind it.  Drafts
     beyond ``max_drafts`` are not looked at."""
-    assert target_probs.dtype in (torch.float32, torch.bfloat16) and target_probs.dim() == 2 and target_probs.is_contiguous()
-    assert draft_tokens.dtype == torch.int64 and draft_tokens.dim() == 1 and draft_tokens.is_contiguous()
-    _check_i32(cu_drafts)
+    assert (target_probs.dtype is torch.float32 or target_probs.dtype is _bf16) and target_probs.dim() == 2 and target_probs.is_contiguous()
+    assert draft_tokens.dtype is torch.int64 and draft_tokens.dim() == 1 and draft_tokens.is_contiguous()
+    assert cu_drafts.dtype is _i32 and cu_drafts.dim() == 1 and cu_drafts.is_contiguous()
     n, batch, vocab = draft_tokens.numel(), cu_drafts.numel() - 1, target_probs.size(1)
-    assert cu_drafts.dim() == 1 and batch >= 0 and max_drafts >= 0 and target_probs.size(0) == n + batch
-    assert uniforms.dtype == torch.float32 and uniforms.is_contiguous() and uniforms.shape == (n + batch,)
-    assert draft_probs is None or (draft_probs.dtype == target_probs.dtype and draft_probs.shape == (n, vocab) and draft_probs.is_contiguous())
-    dev = _device(target_probs, draft_tokens, cu_drafts, uniforms, *(() if draft_probs is None else (draft_probs,)))
+    assert batch >= 0 and max_drafts >= 0 and target_probs.size(0) == n + batch
+    assert uniforms.dtype is torch.float32 and uniforms.is_contiguous() and uniforms.shape == (n + batch,)
+    assert draft_probs is None or (draft_probs.dtype is target_probs.dtype and draft_probs.shape == (n, vocab) and draft_probs.is_contiguous())
+    dev = target_probs.get_device()
+    if dev < 0 or not (dev == draft_tokens.get_device() == cu_drafts.get_device() == uniforms.get_device()
+                       == (dev if draft_probs is None else draft_probs.get_device())):
+        _lib.require_cuda(target_probs, draft_tokens, cu_drafts, uniforms, draft_probs)
     tokens = draft_tokens.new_empty((batch, max_drafts + 1))
     accepted = cu_drafts.new_empty(batch)
     # an empty draft_probs (no request has drafts) has no address and stands for nothing
-    _call("verify_drafts_cuda", dev, target_probs.data_ptr(), _lib.ptr(draft_probs), target_probs.dtype is torch.bfloat16,
+    _call("verify_drafts_cuda", dev, target_probs.data_ptr(), _lib.ptr(draft_probs), target_probs.dtype is _bf16,
           draft_tokens.data_ptr(), cu_drafts.data_ptr(), uniforms.data_ptr(), tokens.data_ptr(), accepted.data_ptr(), batch, n, vocab,
           max_drafts)
     return tokens, accepted
