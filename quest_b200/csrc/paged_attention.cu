@@ -20,15 +20,15 @@
 // computes its places in the lines from the lengths on the device.  An item that crosses from one piece to the next leaves partial
 // (O, m, l) in the workspace, and a second kernel joins them in order, so results do not depend on timing.
 //
-// Measured in a graph (copy 6.55 TB/s, matrix product 1655 TFLOP/s, 1396 sustained):
-//   64 requests at 4096 tokens on average, 64 / 8 heads of 128, one new token    110 - 119 us, 4.7 - 5.1 TB/s; of that 10 us until
-//                                               the first product, about 90 at the rate of HBM, 7 for the join
-//   one request of 1024 tokens, 32 / 8 heads of 128, one new token               13 us, nearly all of it the chain of latencies
-//   one request of 32768 tokens, 64 / 8 heads                                    39 us, 3.4 TB/s
-//   16 prompts of 1024, 32 heads of 128                                          118 - 122 us; tensor pipe and exponentials a third each
-//   4 prompts of 4096, 32 / 8 heads of 128                                       572 - 610 us, 900 - 960 TFLOP/s
-//   a chunk of 4096 behind 28672 tokens, 64 / 8 heads                            3.45 ms at 1965 MHz, 1194 TFLOP/s; 3.85 - 4.1 ms where the
-//                                               power limit lowers the clock (1000 - 1070)
+// Measured in a graph (copy 6.55 TB/s, matrix product 1655 TFLOP/s, 1408 sustained; heads of 128):
+//   64 requests of up to 16384 tokens (137000 in all), 64 / 8 heads, one new token   110 - 119 us, 4.7 - 5.1 TB/s; of that 10 us until
+//                                                the first product, about 90 at the rate of HBM, 7 for the join
+//   one request of 1001 tokens, 16 / 16 heads, one new token    13 us, nearly all of it the chain of latencies
+//   one request of 32768 tokens, 64 / 8 heads, one new token    39 us, 3.4 TB/s
+//   16 prompts of 1024, 16 / 16 heads                           118 - 122 us; tensor pipe and exponentials a third each
+//   4 prompts of 4096, 32 / 8 heads                             572 - 610 us, 900 - 960 TFLOP/s
+//   a chunk of 4096 behind 28672 tokens, among 15 single tokens, 64 / 8 heads    3.45 ms at 1965 MHz, 1194 TFLOP/s; 3.85 - 4.1 ms
+//                                                (1000 - 1070) where the power limit lowers the clock
 // A step of 128 rows by 128 keys costs the tensor core 2 x 8 products of 64 cycles and its warps 128 exponentials per thread, 16 a
 // cycle and SM: 1024 cycles each.  Long chunks are bound by both at once.
 // Other splits that were built: an issuing warp per stream for pairs 4.2 ms for the chunk; keys as the rows of S for tiles of at most 32
