@@ -7,8 +7,8 @@
 //   P = exp2(c S - c m), running maximum m and sum l per row in fp32: thread = row, four warps per stream
 //   O += P V    tcgen05.mma with P (bf16, over its S) in tensor memory, V [keys][columns] in shared memory as it lies in the page
 // P is rounded to bf16 (at most 2^-8 of itself, and it is the weight of one key among many) because the second product takes 16-bit
-// operands; O, m and l stay in fp32.  O is rescaled only when a row's maximum has grown by more than 2^8: until then P and l simply
-// exceed one.
+// operands; O, m and l stay in fp32.  O is rescaled only when a row's weights have grown far beyond one; until then P and l simply
+// exceed it.
 // A tile has whole tokens: 128 / group of them per stream.  The two streams of a block work in one of two ways.  As a pair they share
 // the keys and values of one tile of 256 rows, and while one stream's warps work on its scores the tensor core works for the
 // other.  Alone (tiles of at most 128 rows: decoding, the ends of chunks) each stream has tiles of its own, with half of the
@@ -85,10 +85,11 @@ struct Params {
 struct Item {
     int start, n, kv, b, hk;  // rows start .. start + n of the batch, kv keys
     int tok0;                 // first token (the second stream of a pair: p.tokens further)
-    int t0, steps[2];         // first step, steps of each stream
+    int t0, steps0, steps1;   // first step, steps of each stream
     int slot;                 // -1: the whole item; else the place of the partial result (second stream: 2 gridDim.x further)
     int last;                 // nothing behind this descriptor (it carries no work)
 };
+// (Two members and no array: indexed by the stream, an array of a local Item would lie in memory.)
 static_assert(sizeof(Item) <= 64, "descriptor");
 
 constexpr int HEADER = 8;  // ints: pieces (0: none), start, hk, tok0, rows
@@ -107,19 +108,21 @@ __device__ __forceinline__ int steps_of(int keys) { return max((keys + BN - 1) /
 __device__ __forceinline__ int pair_tiles(const Request& q, int tokens) { return (q.n + tokens - 1) / (2 * tokens); }
 __device__ __forceinline__ bool has_single(const Request& q, int tokens) { return q.n > 0 && (q.n - 1) % (2 * tokens) < tokens; }
 
-// sum over i < n of floor((a i + b) / m), a, b >= 0 (the Euclidean descent on a and m)
-__device__ __forceinline__ long long sum_of_quotients(long long n, long long m, long long a, long long b) {
+// sum over i < n of floor((a i + b) / 128), a, b >= 0, a n + b < 2^31: whole multiples of the divisor out of a and b, then the same
+// sum the other way round (over the values of the quotient), until the slope is zero.
+__device__ __forceinline__ long long sum_of_quotients(uint32_t n, uint32_t a, uint32_t b) {
     long long sum = 0;
-    while (n > 0) {
-        sum += n * (n - 1) / 2 * (a / m) + n * (b / m);
-        a %= m, b %= m;
-        const long long y = a * n + b;
-        n = y / m, b = y % m;
-        const long long t = m;
+    uint32_t m = BN;
+    while (true) {
+        const uint32_t qa = a / m, qb = b / m;
+        sum += (long long)n * (n - 1) / 2 * qa + (long long)n * qb;
+        a -= qa * m, b -= qb * m;
+        const uint32_t y = a * n + b;
+        if (y < m) return sum;
+        n = y / m, b = y - n * m;
+        const uint32_t t = m;
         m = a, a = t;
-        if (m == 0) break;
     }
-    return sum;
 }
 // Places that the first `tiles` pair tiles of a request and one head take in the line: their steps and kItemCost each.  A full
 // tile i of w = 2 tokens ends with token (i + 1) w - 1, so it takes max(floor(((i + 1) w - 1 + kv - n) / 128), 0) + 1 steps;
@@ -131,7 +134,7 @@ __device__ __forceinline__ long long pairs_before(const Request& q, int tiles, i
         const int w = 2 * tokens, e = w - 1 + q.kv - q.n;
         const int first = e >= 0 ? 0 : (-e + w - 1) / w;
         sum += tiles;
-        if (tiles > first) sum += sum_of_quotients(tiles - first, BN, w, e + w * first);
+        if (tiles > first) sum += sum_of_quotients(tiles - first, w, e + w * first);
     }
     return sum;
 }
@@ -232,69 +235,119 @@ __device__ __forceinline__ void store_row32(__nv_bfloat16* dst, const uint32_t (
 struct RowState {
     float m, l;  // m in units of the scores; -inf: nothing seen
 };
+constexpr float kMostSum = 1024.f;  // of a step's weights before the reference maximum is looked at again
+
+// exp2 of a pair on the arithmetic pipes: the nearest integer n by adding 1.5 2^23, 2^n by shifting it into place, and a polynomial
+// of degree 3 for the rest in [-1/2, 1/2] (best in relative error: 7.5e-5, a twenty-sixth of what rounding to bf16 may add).
+// From 2^-126.5 down the result is zero, as what is masked has to be.
+__device__ __forceinline__ void ex2_pair(uint64_t x2, float& r0, float& r1) {
+    float a, b;
+    unpack2(x2, a, b);
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(-127.f));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(b) : "f"(-127.f));
+    asm("min.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(127.f));
+    asm("min.NaN.f32 %0, %0, %1;" : "+f"(b) : "f"(127.f));
+    x2 = pack2(a, b);
+    const uint64_t t = add2(x2, pack2(12582912.f, 12582912.f)), n = add2(t, pack2(-12582912.f, -12582912.f)), f = fma2(n, pack2(-1.f, -1.f), x2);
+    uint64_t p = fma2(pack2(0.0551716685f, 0.0551716685f), f, pack2(0.2426111251f, 0.2426111251f));
+    p = fma2(p, f, pack2(0.6932609677f, 0.6932609677f));
+    p = fma2(p, f, pack2(0.9999280572f, 0.9999280572f));
+    unpack2(t, a, b);
+    const float e0 = __int_as_float((__float_as_int(a) << 23) + 0x3f800000), e1 = __int_as_float((__float_as_int(b) << 23) + 0x3f800000);
+    unpack2(fma2(p, pack2(e0, e1), 0), r0, r1);
+}
+// exp2(c s + off) of 32 scores, packed to bf16, and their sum.  The special function unit gives 16 a cycle; some pairs go the other
+// way: at D 128, where the products cost as much as the exponentials, two of sixteen (4 prompts of 4096: 530 us with none, 495 with
+// two, 502 with three, 549 with four), at D 64, where they cost half, five (485 with none, 442 with two, 430 with three or six, 426 with
+// five, 438 with eight).
+template <int D>
+__device__ __forceinline__ void weights32(const uint32_t (&s)[32], uint64_t c2, uint64_t off2, uint32_t* pk, uint64_t (&sum)[2]) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        float x0, x1;
+        const uint64_t x2 = fma2(pack2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), c2, off2);
+        if (D == 64 ? i % 3 == 2 : i % 8 == 7) {
+            ex2_pair(x2, x0, x1);
+        } else {
+            unpack2(x2, x0, x1);
+            x0 = ex2(x0), x1 = ex2(x1);
+        }
+        sum[i & 1] = add2(sum[i & 1], pack2(x0, x1));
+        pk[i] = pack_bf16x2(x0, x1);
+    }
+}
 
 // One step of a row: scores in tensor memory -> probabilities over them.  `seen` keys of this step are visible to the row.
+// Mostly all of them are, and the reference maximum still serves: then nothing has to be known of the scores before their
+// exponentials, and the sum tells afterwards (no weight beyond kMostSum can hide in it, nor a NaN).  Else a pass for the maximum comes
+// first, which writes what is masked back as minus infinity.  A chunk of 4096 behind 28672 tokens: 3.35 ms with the maximum taken in
+// every step, 3.10 like this.  The code is kept short for calls of many short items, between which the roles' instructions have to
+// come in again: with 26 KB more of it 128 requests of 1000 tokens took 138 us in place of 115.
 template <int D>
 __device__ __forceinline__ void softmax_step(RowState& st, const uint32_t s_addr, const uint32_t o_addr, const int seen, const bool live, const bool first, const float c) {
-    uint32_t s[4][32];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) tmem_ld32(s_addr + 32 * i, s[i]);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) tmem_ld_wait32(s[i]);
-    if (__any_sync(~0u, seen < BN)) {
-#pragma unroll
-        for (int i = 0; i < 128; ++i)
-            if (i >= seen) s[i / 32][i % 32] = 0xff800000u;  // whatever stands there
-    }
-    float top = -CUDART_INF_F;
-    {
-        float t[4] = {top, top, top, top};
-#pragma unroll
-        for (int i = 0; i < 32; i += 2)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) t[j] = fmaxf(fmaxf(t[j], __uint_as_float(s[j][i])), __uint_as_float(s[j][i + 1]));
-        top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
-    }
-    top = fmaxf(top, st.m);
-    // 2^8 of growth is harmless in fp32 sums and bf16 probabilities alike
-    const bool grown = live && (top * c > st.m * c + 8.f || (st.m == -CUDART_INF_F && top != -CUDART_INF_F));
-    if (__any_sync(~0u, grown)) {
-        const float a = st.m == -CUDART_INF_F ? 0.f : ex2((st.m - top) * c);
-        st.m = top;
-        st.l *= a;
-        if (!first) {
+    const bool partial = __any_sync(~0u, seen < BN);
+    bool check = !partial && !__any_sync(~0u, live && st.m == -CUDART_INF_F);
+    uint32_t pk[2][32];
+    float l, slack = 8.f;
+    while (true) {
+        if (!check) {
+            float top = st.m;
 #pragma unroll 1
-            for (int i = 0; i < D / 32; ++i) {
-                uint32_t o[32];
-                tmem_ld32(o_addr + 32 * i, o);
-                tmem_ld_wait32(o);
+            for (int i0 = 0; i0 < BN; i0 += 32) {
+                uint32_t s[32];
+                tmem_ld32(s_addr + i0, s);
+                tmem_ld_wait32(s);
+                if (partial) {
 #pragma unroll
-                for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * a);
-                tmem_st32(o_addr + 32 * i, o);
+                    for (int i = 0; i < 32; ++i)
+                        if (i0 + i >= seen) s[i] = 0xff800000u;  // whatever stands there
+                    tmem_st32(s_addr + i0, s);
+                }
+                float t[4] = {top, top, top, top};
+#pragma unroll
+                for (int i = 0; i < 32; i += 2) t[i / 2 % 4] = fmaxf(fmaxf(t[i / 2 % 4], __uint_as_float(s[i])), __uint_as_float(s[i + 1]));
+                top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
             }
-        }
-    }
-    const float off = st.m == -CUDART_INF_F ? 0.f : -st.m * c;
-    const uint64_t c2 = pack2(c, c), off2 = pack2(off, off);
-    uint64_t sum[2] = {0, 0};
+            // 2^8 of growth is harmless in fp32 sums and bf16 probabilities alike; where the sum has shown more the maximum follows at once
+            const bool grown = live && (top * c > st.m * c + slack || (st.m == -CUDART_INF_F && top != -CUDART_INF_F));
+            if (__any_sync(~0u, grown)) {
+                const float a = st.m == -CUDART_INF_F ? 0.f : ex2((st.m - top) * c);
+                st.m = top;
+                st.l *= a;
+                if (!first) {
+#pragma unroll 1
+                    for (int i = 0; i < D / 32; ++i) {
+                        uint32_t o[32];
+                        tmem_ld32(o_addr + 32 * i, o);
+                        tmem_ld_wait32(o);
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-        uint32_t pk[32];
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-            const int e = half * 64 + 2 * i;
-            const uint64_t x = fma2(pack2(__uint_as_float(s[e / 32][e % 32]), __uint_as_float(s[e / 32][e % 32 + 1])), c2, off2);
-            float x0, x1;
-            unpack2(x, x0, x1);
-            x0 = ex2(x0), x1 = ex2(x1);
-            sum[i & 1] = add2(sum[i & 1], pack2(x0, x1));
-            pk[i] = pack_bf16x2(x0, x1);
+                        for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * a);
+                        tmem_st32(o_addr + 32 * i, o);
+                    }
+                }
+            }
+            tmem_st_wait();
         }
-        tmem_st32(s_addr + half * 32, pk);
+        const float off = st.m == -CUDART_INF_F ? 0.f : -st.m * c;
+        const uint64_t c2 = pack2(c, c), off2 = pack2(off, off);
+        uint64_t sum[2] = {0, 0};
+        uint32_t s[2][32];
+        tmem_ld32(s_addr, s[0]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            tmem_ld_wait32(s[i & 1]);
+            if (i < 3) tmem_ld32(s_addr + 32 * (i + 1), s[(i + 1) & 1]);
+            weights32<D>(s[i & 1], c2, off2, pk[i / 2] + 16 * (i & 1), sum);
+        }
+        float a, b;
+        unpack2(add2(sum[0], sum[1]), a, b);
+        l = a + b;
+        if (!check || !__any_sync(~0u, live && !(l <= kMostSum))) break;
+        check = false, slack = 0.f;
     }
-    float a, b;
-    unpack2(add2(sum[0], sum[1]), a, b);
-    st.l += a + b;
+    st.l += l;
+    tmem_st32(s_addr, pk[0]);
+    tmem_st32(s_addr + 32, pk[1]);
     tmem_st_wait();
 }
 
@@ -483,7 +536,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
             uint32_t s_ph = 0, o_ph = 0;
             Item d;
             for (uint32_t it = 0; take(list, it, d);) {
-                const int steps = d.steps[s], tok0 = d.tok0 + (list == 0 ? s * p.tokens : 0);
+                const int steps = s == 0 ? d.steps0 : d.steps1, tok0 = d.tok0 + (list == 0 ? s * p.tokens : 0);
                 // Where few rows are there the second stream's lie in the other two quadrants: its warps run on other parts of the SM.
                 const int row = lane_row - (list > 0 && s == 1 && d.n - tok0 <= p.half_tokens ? BM / 2 : 0);
                 const int row_token = row >= 0 ? row / p.group : 0, row_head = row - row_token * p.group, token = tok0 + row_token;
@@ -512,7 +565,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
                 // Values that are not finite at keys which a row does not see (later tokens of its chunk) must not reach it.
                 const int stop = min((d.t0 + steps) * BN, d.kv);
                 const bool hidden = __any_sync(~0u, live && keys < stop);
-                float check[4] = {0, 0, 0, 0};  // NaN where a column is not finite
+                uint64_t check[2] = {0, 0};  // NaN where a column is not finite
                 if (d.slot < 0) {
                     const float inv = 1.f / l;
                     const bool empty = l == 0.f;  // no key in sight: zeros
@@ -527,7 +580,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
                             w[j] = empty ? 0u : pack_bf16x2(__uint_as_float(o[2 * j]) * inv, __uint_as_float(o[2 * j + 1]) * inv);
                         if (hidden) {
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) check[j % 4] = fmaf(__uint_as_float(o[j]), 0.f, check[j % 4]);
+                            for (int j = 0; j < 16; ++j) check[j % 2] = fma2(pack2(__uint_as_float(o[2 * j]), __uint_as_float(o[2 * j + 1])), 0, check[j % 2]);
                         }
                         if (live) store_row32(dst + c0, w, p.wide_stores);
                     }
@@ -548,13 +601,15 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
                         for (int j = 0; j < 8; ++j) {
                             uint4 x = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
                             if (nothing) x = make_uint4(0, 0, 0, 0);
-                            check[0] = fmaf(__uint_as_float(x.x), 0.f, check[0]), check[1] = fmaf(__uint_as_float(x.y), 0.f, check[1]);
-                            check[2] = fmaf(__uint_as_float(x.z), 0.f, check[2]), check[3] = fmaf(__uint_as_float(x.w), 0.f, check[3]);
+                            check[0] = fma2(pack2(__uint_as_float(x.x), __uint_as_float(x.y)), 0, check[0]);
+                            check[1] = fma2(pack2(__uint_as_float(x.z), __uint_as_float(x.w)), 0, check[1]);
                             if (mine) reinterpret_cast<uint4*>(slot)[(c0 / 4 + j) * p.slot_rows + row] = x;
                         }
                     }
                 }
-                uint32_t bad = __ballot_sync(~0u, hidden && live && !((check[0] + check[1]) + (check[2] + check[3]) == 0.f) && l > 0.f && l < CUDART_INF_F && keys < stop);
+                float nan0, nan1;
+                unpack2(add2(check[0], check[1]), nan0, nan1);
+                uint32_t bad = __ballot_sync(~0u, hidden && live && !(nan0 + nan1 == 0.f) && l > 0.f && l < CUDART_INF_F && keys < stop);
                 if (bad != 0) __syncwarp();  // the rows' stores are behind
                 while (bad != 0) {
                     const int from = __ffs(bad) - 1, r = __shfl_sync(~0u, row, from), t = __shfl_sync(~0u, token, from);
@@ -595,8 +650,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
             };
             auto load_queries = [&](int tile, int set, uint32_t& ph, int token, int hk, bool upper) {
                 const uint32_t full = bar(C::Q_FULL + 2 * set + tile);
-                ok = __all_sync(~0u, ok && wait_bar(bar(C::Q_EMPTY + 2 * set + tile), ph ^ 1u));
-                ph ^= 1u;
+                ok = __all_sync(~0u, ok && wait_bar(bar(C::Q_EMPTY + 2 * set + tile), ((ph >> tile) & 1u) ^ 1u));
+                ph ^= 1u << tile;
                 if (ok && lane == 0) {
                     mbar_arrive_expect_tx(full, (upper ? p.half_tokens : p.tokens) * p.group * D * 2);
                     for (int h = 0; h < C::HALVES; ++h)
@@ -651,8 +706,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
                     const bool begins = d.t0 == 0, ends = to == cost;
                     if (t1 > d.t0) {
                         d.slot = begins && ends ? -1 : 2 * (int)blockIdx.x + (begins ? 1 : 0);
-                        d.steps[0] = max(min(t1, steps_of(keys_of(q, d.tok0 + p.tokens - 1))) - d.t0, 0);  // its tokens see fewer keys
-                        d.steps[1] = t1 - d.t0;
+                        d.steps0 = max(min(t1, steps_of(keys_of(q, d.tok0 + p.tokens - 1))) - d.t0, 0);  // its tokens see fewer keys
+                        d.steps1 = t1 - d.t0;
                         publish(0, it, d);
                         if (begins && !ends && lane < 2) {  // the pieces behind this one: one per worker, up to that of the last place
                             int* h = p.headers + (lane * blocks + blockIdx.x) * HEADER;
@@ -660,14 +715,15 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
                             h[1] = q.start, h[2] = hk, h[3] = tok0, h[4] = max(min(p.tokens, q.n - tok0), 0) * p.group;
                             h[0] = (int)((u + (cost - off) - 1) / w.share) - (int)blockIdx.x + 1;
                         }
-                        const int n = d.steps[1];
-                        int ids[3] = {page_at(d, d.t0), n > 1 ? page_at(d, d.t0 + 1) : 0, 0};  // asked for a step before they are needed
-                        load(&kmap, d, d.t0, ids[0]);
-                        for (int i = 0; ok && i < n; ++i) {  // keys run one step ahead of the values
-                            if (i + 2 < n) ids[2] = page_at(d, d.t0 + i + 2);
-                            if (i + 1 < n) load(&kmap, d, d.t0 + i + 1, ids[1]);
-                            load(&vmap, d, d.t0 + i, ids[0]);
-                            ids[0] = ids[1], ids[1] = ids[2];
+                        const int n = d.steps1;
+                        int id = 0, next_id = page_at(d, d.t0);
+#pragma unroll 1
+                        for (int i = -1; ok && i < n; ++i) {  // keys run one step ahead of the values
+                            const int far_id = i + 2 < n ? page_at(d, d.t0 + i + 2) : 0;  // asked for a step before it is needed
+#pragma unroll 1
+                            for (int k = 1; k >= 0; --k)
+                                if (i + k >= 0 && i + k < n) load(k ? &kmap : &vmap, d, d.t0 + i + k, k ? next_id : id);
+                            id = next_id, next_id = far_id;
                         }
                     }
                     u += to - off;
@@ -688,11 +744,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
                 d.last = 1;
                 publish(0, it, d);
             } else if (has_pairs) {
-                uint32_t q_ph[2] = {0, 0};
+                uint32_t q_ph = 0;
                 Item d;
                 for (uint32_t it = 0; take(0, it, d);) {
-                    if (d.steps[0] > 0) load_queries(0, 0, q_ph[0], d.start + d.tok0, d.hk, false);
-                    load_queries(1, 0, q_ph[1], d.start + d.tok0 + p.tokens, d.hk, false);
+#pragma unroll 1
+                    for (int t = 0; t < 2; ++t)
+                        if ((t == 0 ? d.steps0 : d.steps1) > 0) load_queries(t, 0, q_ph, d.start + d.tok0 + t * p.tokens, d.hk, false);
                 }
             }
             const Place w = places[1 + s];
@@ -703,7 +760,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
                 const int id = s * blocks + (int)blockIdx.x;
                 uint32_t it = 0, slot = 0, ph = 0, q_ph = 0;
                 auto load = [&](const CUtensorMap* map, const Item& d, int step, int page_id) {
-#pragma unroll
+#pragma unroll 1
                     for (int h = 0; h < 2; ++h) {
                         ok = __all_sync(~0u, ok && wait_bar(bar(C::SLOT_EMPTY + first + slot), ph ^ 1u));
                         if (!ok) return;
@@ -728,15 +785,17 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
                     if (t1 > d.t0) {
                         d.start = q.start, d.n = q.n, d.kv = q.kv, d.b = b, d.hk = hk, d.last = 0;
                         d.tok0 = (q.n - 1) / (2 * p.tokens) * (2 * p.tokens);
-                        d.steps[s] = t1 - d.t0, d.steps[s ^ 1] = 0;
+                        d.steps0 = d.steps1 = t1 - d.t0;  // the list's stream looks at its own
                         d.slot = begins && ends ? -1 : 4 * blocks + 2 * id + (begins ? 1 : 0);
                         int ids[3] = {page_at(d, d.t0), d.t0 + 1 < t1 ? page_at(d, d.t0 + 1) : 0, 0};  // asked for a step before they are needed
                         publish(1 + s, it, d);
                         for (int step = d.t0; ok && step < t1; ++step) {
                             if (step + 2 < t1) ids[2] = page_at(d, step + 2);
-                            load(&kmap, d, step, ids[0]);
-                            if (step == d.t0) load_queries(s, 1, q_ph, d.start + d.tok0, d.hk, s == 1 && d.n - d.tok0 <= p.half_tokens);
-                            load(&vmap, d, step, ids[0]);
+#pragma unroll 1
+                            for (int k = 1; k >= 0; --k) {
+                                load(k ? &kmap : &vmap, d, step, ids[0]);
+                                if (k && step == d.t0) load_queries(s, 1, q_ph, d.start + d.tok0, d.hk, s == 1 && d.n - d.tok0 <= p.half_tokens);
+                            }
                             ids[0] = ids[1], ids[1] = ids[2];
                         }
                         if (begins && !ends && lane == 0) {
@@ -775,7 +834,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
                 Item x;
                 const bool more = take(list, it, x);
                 d.n = __shfl_sync(~0u, x.n, 0), d.kv = __shfl_sync(~0u, x.kv, 0), d.t0 = __shfl_sync(~0u, x.t0, 0);
-                d.steps[0] = __shfl_sync(~0u, x.steps[0], 0), d.steps[1] = __shfl_sync(~0u, x.steps[1], 0);
+                d.steps0 = __shfl_sync(~0u, x.steps0, 0), d.steps1 = __shfl_sync(~0u, x.steps1, 0);
                 return __all_sync(~0u, more) != 0;
             };
             // Rows of the last page behind the request's tokens hold anything; a zero weight does not make a NaN harmless.
@@ -836,7 +895,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
                 };
                 Item d;
                 for (uint32_t it = 0; take_uniform(0, it, d);) {
-                    const int n0 = d.steps[0], n1 = d.steps[1];
+                    const int n0 = d.steps0, n1 = d.steps1;
                     wait_in(C::PAIR_FULL + next.at, next.ph);
                     if (n0 > 0) {
                         wait_q(0);
@@ -878,7 +937,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
                 };
                 Item d;
                 for (uint32_t it = 0; take_uniform(1 + s, it, d);) {
-                    const int n = d.steps[s];
+                    const int n = d.steps0;
                     wait_in(C::Q_FULL + 2 + s, q_parity), q_parity ^= 1u;
                     for (int i = 0; ok && i < n; ++i) {
 #pragma unroll

@@ -219,6 +219,61 @@ def test_attention_of_extreme_scores():
     assert ((got - want).abs() <= (2 ** -8 + 2 ** -7) * size + 2 ** -8 * want.abs()).all()
 
 
+def scores_case(profile, d, hq=4, hkv=2, new=3):
+    """A request whose score at key j is near profile[j] for every row (natural units): queries along one direction."""
+    kv, page = len(profile), 64
+    g = torch.Generator().manual_seed(kv + d)
+    u = torch.randn(d, generator=g)
+    u /= u.norm()
+    pages = ref.ceil_div(kv, page)
+    q = (d ** 0.5 * u + 0.02 * torch.randn(new, hq, d, generator=g)).bfloat16().cuda()  # scale q.k is then u.k
+    k = torch.tensor(profile)[:, None, None] * u + 0.02 * torch.randn(kv, hkv, d, generator=g)
+    cache = torch.zeros(2, pages * page, hkv, d)
+    cache[0, :kv], cache[1, :kv] = k, torch.randn(kv, hkv, d, generator=g)
+    k_cache, v_cache = cache.bfloat16().cuda().view(2, pages, page, hkv, d).unbind(0)
+    return dict(q=q, k_cache=k_cache, v_cache=v_cache, page_table=torch.arange(pages, dtype=torch.int32, device="cuda")[None], kv_lens=i32([kv]),
+                cu_new=i32([0, new]))
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("new", [3, 200])
+@pytest.mark.parametrize("name", ["rise", "fall", "leap", "slope", "spikes", "plateau", "waves"])
+def test_attention_follows_the_maximum_from_step_to_step(name, new, d):
+    """Scores that grow or fall between steps, by a little, by what fp32 can no longer hold, and at single keys of any place in a
+    step.  With scores up to 250 their sums in fp32 (128 products of at most about 40, of both signs) are off by less than 2^-14, as
+    check_attention allows for; bf16 queries and keys make the scores themselves uneven, which the oracle sees, too."""
+    kv = 128 * 9 + 40
+    profile = {
+        "rise": [j // 128 * 3.0 for j in range(kv)],  # 2^4.3 a step: the sum passes its limit every few steps
+        "fall": [30.0 - j // 128 * 9.0 for j in range(kv)],
+        "leap": [-120.0 if j < 500 else 120.0 for j in range(kv)],  # 2^346 at once
+        "slope": [-200.0 + 400.0 * j / kv for j in range(kv)],
+        "spikes": [25.0 + j / 100 if j % 131 == 14 else 0.0 for j in range(kv)],
+        "plateau": [0.0 if j < 128 else 4.9 for j in range(kv)],  # 128 weights of 2^7
+        "waves": [60.0 if j // 128 % 2 else -60.0 for j in range(kv)],
+    }[name]
+    check_attention(scores_case(profile, d, new=new))
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+def test_attention_keys_that_are_seen_and_not_finite(bad, d):
+    """As in the formula: a score that is NaN or +inf makes its row NaN, one that is -inf has no weight.  Every place of a step's
+    first 36 keys, in the first step and in a later one."""
+    for at in [*range(36), *range(256, 292), 127, 511]:
+        s = scores_case([0.0] * 600, d, new=2)
+        s["k_cache"].view(-1, 2, d)[at, 0] = bad * s["q"][0, 0].sign()  # key/value head 0: of the query heads 0 and 1
+        got = quest.paged_attention(**s)
+        clean = scores_case([0.0] * at + [-1e4] + [0.0] * (599 - at), d, new=2)
+        if bad == float("-inf"):
+            check_attention(clean)
+            same = (s["q"][:, :2].sign() == s["q"][0, 0].sign()).all(dim=-1)  # rows whose products all have one sign
+            assert same[0, 0] and torch.isfinite(got[:, :2][same]).all()
+        else:
+            assert torch.isnan(got[0, 0]).all()
+        assert torch.isfinite(got[:, 2:]).all()
+
+
 def test_attention_pages_outside_the_pool_read_as_nothing():
     """A table entry that points nowhere is not read (keys and values 0), wherever it stands."""
     s = ref.paged_state(9, [64, 40], [1, 1], 2, 2, 64, 16)
