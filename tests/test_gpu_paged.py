@@ -420,6 +420,21 @@ def test_verify_drafts(dtype, with_draft, counts, vocab, most):
     assert kept.tolist() == accepted and got.tolist() == want
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("vocab", [5, 8, 15, *range(2040, 2049)])
+def test_verify_drafts_rows_of_any_alignment(vocab, dtype):
+    """Rows and tensors that begin anywhere in 16 bytes, up to the last element of their memory, between entries that would be drawn."""
+    target, draft, tokens, cu, u = drafts_case(vocab, [3, 0, 2, 4, 1] * 3, vocab, dtype)
+    want, accepted = ref.verify(target, draft, tokens.tolist(), cu, u, 4)
+    for offset in range(8):
+        def placed(x):
+            buffer = torch.full((offset + x.numel() + offset,), 1000.0, dtype=dtype, device="cuda")
+            buffer[offset:offset + x.numel()] = x.cuda().view(-1)
+            return buffer[offset:offset + x.numel()].view_as(x)
+        got, kept = quest.verify_drafts(placed(target), tokens.cuda(), i32(cu), u.cuda(), 4, draft_probs=placed(draft))
+        assert kept.tolist() == accepted and got.tolist() == want, offset
+
+
 def test_verify_drafts_at_the_borders():
     """Equal distributions (nothing left to draw from when a draft is refused all the same), zero probabilities, uniforms of 0 and
     nearly 1, tokens outside the vocabulary, rows without any weight, NaN."""
