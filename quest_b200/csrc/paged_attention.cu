@@ -16,23 +16,27 @@
 // steps (its queries, its result) disappears behind the other stream.
 //
 // Work is cut by steps, not by tiles: the steps of all pair items form one line, those of all single items another; every block
-// takes an equal piece of the first, then each of its streams an equal piece of the second, whatever the lengths are.  Each block
-// computes its places in the lines from the lengths on the device.  An item that crosses from one piece to the next leaves partial
-// (O, m, l) in the workspace, and a second kernel joins them in order, so results do not depend on timing.
+// takes an equal piece of the first (cut at an item's edge where one is near), then each of its streams an equal piece of the second,
+// whatever the lengths are.  Each block computes its places in the lines from the lengths on the device.  An item that crosses from
+// one piece to the next leaves partial (O, m, l) in the workspace, and a second kernel joins them in order, so results do not depend on
+// timing.
 //
-// Measured in a graph (copy 6.55 TB/s, matrix product 1655 TFLOP/s, 1408 sustained; heads of 128):
-//   64 requests of up to 16384 tokens (137000 in all), 64 / 8 heads, one new token   110 - 119 us, 4.7 - 5.1 TB/s; of that 10 us until
-//                                                the first product, about 90 at the rate of HBM, 7 for the join
+// Measured in a graph (copy 6.55 TB/s, matrix product 1655 TFLOP/s, 1408 sustained; heads of 128; a range ends with what the power
+// limit leaves when the calls go on for long):
+//   64 requests of up to 16384 tokens (137000 in all), 64 / 8 heads, one new token   102 - 112 us, 5.0 - 5.5 TB/s; of that 9 us until
+//                                                the first product, 85 - 90 at the rate of HBM, 6 for the join
 //   one request of 1001 tokens, 16 / 16 heads, one new token    13 us, nearly all of it the chain of latencies
-//   one request of 32768 tokens, 64 / 8 heads, one new token    39 us, 3.4 TB/s
-//   16 prompts of 1024, 16 / 16 heads                           118 - 122 us; tensor pipe and exponentials a third each
-//   4 prompts of 4096, 32 / 8 heads                             572 - 610 us, 900 - 960 TFLOP/s
-//   a chunk of 4096 behind 28672 tokens, among 15 single tokens, 64 / 8 heads    3.45 ms at 1965 MHz, 1194 TFLOP/s; 3.85 - 4.1 ms
-//                                                (1000 - 1070) where the power limit lowers the clock
+//   one request of 32768 tokens, 64 / 8 heads, one new token    38 us, 3.5 TB/s
+//   128 requests of at most 1000 tokens, 32 / 32 heads          116 - 130 us, 3.9 - 4.3 TB/s
+//   16 prompts of 1024, 16 / 16 heads                           107 - 120 us; tensor pipe and exponentials a third each
+//   4 prompts of 4096, 32 / 8 heads                             471 - 535 us, 1167 - 1028 TFLOP/s; head_dim 64 410 us
+//   a chunk of 4096 behind 28672 tokens, among 15 single tokens, 64 / 8 heads    3.10 - 3.62 ms, 1330 - 1139 TFLOP/s
 // A step of 128 rows by 128 keys costs the tensor core 2 x 8 products of 64 cycles and its warps 128 exponentials per thread, 16 a
-// cycle and SM: 1024 cycles each.  Long chunks are bound by both at once.
-// Other splits that were built: an issuing warp per stream for pairs 4.2 ms for the chunk; keys as the rows of S for tiles of at most 32
-// rows 12.3 us for one request, but 118 for the 64; the result through shared memory 146 us for the 16 prompts.
+// cycle and SM: 1024 cycles each.  A stream's steps form a chain, 1900 cycles of softmax and 1330 of products and their hand-over; two
+// streams keep the tensor core busy two thirds of that.
+// Other splits that were built: an issuing warp per stream for pairs 4.2 ms for the chunk (3.45 then); keys as the rows of S for tiles of
+// at most 32 rows 12.3 us for one request, but 118 for the 64 (110 then); the result through shared memory 146 us for the 16 prompts (134
+// then), or with four lanes to a row of it 117 (108 then).
 #include <math_constants.h>
 
 #include "tcgen05.cuh"
@@ -46,7 +50,11 @@ constexpr int kCopyWarp0 = 0, kMmaWarp0 = 1, kMmaWarp1 = 2, kCopyWarp1 = 3, kFir
 constexpr int ITEMS = 4;                            // descriptors in flight on each list
 constexpr int kControlRegs = 96, kSoftmaxRegs = 200;  // 128 x 96 + 256 x 200 is what the block is launched with, 384 x 168, or less
 static_assert(128 * kControlRegs + 256 * kSoftmaxRegs <= kThreads * 168, "register shares exceed the launch");
-constexpr int kItemCost = 1;  // steps that an item's queries and result are worth in the lines (0 and 2 left blocks up to 10 % longer at work)
+// Steps that an item's queries and result are worth in the lines, and how near to an item's edge a pair's line is cut there and not in
+// the item (4 prompts of 4096: 500 us with one step for a pair, 471 with two, 481 with three; 16 of at most 200: 29 us with two
+// and every cut where it falls, 23 like this.  Single items: 128 requests of 1000 tokens 115 us with one step, 129 with two; cuts
+// moved by up to two places leave 5 drafts for 32 requests at 38 us in place of 34.5).
+constexpr int kPairCost = 2, kPairNear = 1, kSingleCost = 1;
 
 template <int D>
 struct Cfg {
@@ -124,11 +132,11 @@ __device__ __forceinline__ long long sum_of_quotients(uint32_t n, uint32_t a, ui
         m = a, a = t;
     }
 }
-// Places that the first `tiles` pair tiles of a request and one head take in the line: their steps and kItemCost each.  A full
+// Places that the first `tiles` pair tiles of a request and one head take in the line: their steps and kPairCost each.  A full
 // tile i of w = 2 tokens ends with token (i + 1) w - 1, so it takes max(floor(((i + 1) w - 1 + kv - n) / 128), 0) + 1 steps;
 // one that is not full ends with the last token.
 __device__ __forceinline__ long long pairs_before(const Request& q, int tiles, int tokens) {
-    long long sum = (long long)tiles * kItemCost;
+    long long sum = (long long)tiles * kPairCost;
     if ((long long)tiles * 2 * tokens > q.n) sum += steps_of(q.kv), --tiles;
     if (tiles > 0) {
         const int w = 2 * tokens, e = w - 1 + q.kv - q.n;
@@ -139,7 +147,7 @@ __device__ __forceinline__ long long pairs_before(const Request& q, int tiles, i
     return sum;
 }
 __device__ __forceinline__ long long single_places(const Params& p, const Request& q) {
-    return has_single(q, p.tokens) ? (long long)(steps_of(q.kv) + kItemCost) * p.hkv : 0;
+    return has_single(q, p.tokens) ? (long long)(steps_of(q.kv) + kSingleCost) * p.hkv : 0;
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -238,7 +246,7 @@ struct RowState {
 constexpr float kMostSum = 1024.f;  // of a step's weights before the reference maximum is looked at again
 
 // exp2 of a pair on the arithmetic pipes: the nearest integer n by adding 1.5 2^23, 2^n by shifting it into place, and a polynomial
-// of degree 3 for the rest in [-1/2, 1/2] (best in relative error: 7.5e-5, a twenty-sixth of what rounding to bf16 may add).
+// of degree 3 for the rest in [-1/2, 1/2] (best in relative error: 7.5e-5, a fiftieth of what rounding to bf16 may add).
 // From 2^-126.5 down the result is zero, as what is masked has to be.
 __device__ __forceinline__ void ex2_pair(uint64_t x2, float& r0, float& r1) {
     float a, b;
@@ -403,6 +411,15 @@ __device__ __forceinline__ void visible_row(const Params& p, const Item& d, int 
             for (int e = 0; e < E; ++e) o[e] = fmaf(w, x[i][e], o[e]);
         }
     }
+}
+
+// Where a line is cut `off` places into an item of `cost`: at the item's edge if that is at most `near` places away.
+__device__ __forceinline__ int cut_at(int off, int cost, int near) { return off <= near ? 0 : cost - off <= near ? cost : off; }
+// Pieces of an item that begins in worker w's part and goes on: one per worker up to that of its last place, where the cut before
+// that is not moved to the item's end.
+__device__ __forceinline__ int pieces_of(long long item_end, long long share, int near, int w) {
+    const int last = (int)((item_end - 1) / share);
+    return last - w + (last == w || item_end - last * share > near);
 }
 
 // A worker's place in a line: from u to end, beginning in request b `rest` places behind the request's first.
@@ -696,13 +713,18 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
                     if (at <= rest) tile = mid, begin = at; else hi = mid - 1;
                 }
                 int off = (int)(rest - begin);
+                const int near = (int)min((long long)kPairNear, (w.share - 1) / 2);  // half a piece would reach the next cut
+                long long u = w.u - off;
+                off = cut_at(off, steps_of(keys_of(q, min((tile + 1) * 2 * p.tokens, q.n) - 1)) + kPairCost, near);
                 Item d;
-                for (long long u = w.u; ok && u < w.end;) {
+                for (u += off; ok && u < w.end;) {
                     d.start = q.start, d.n = q.n, d.kv = q.kv, d.b = b, d.hk = hk, d.tok0 = tile * 2 * p.tokens, d.last = 0;
-                    const int steps = steps_of(keys_of(q, min(d.tok0 + 2 * p.tokens, q.n) - 1)), cost = steps + kItemCost;
-                    const int to = (int)min((long long)cost, off + (w.end - u));
-                    d.t0 = max(off - kItemCost, 0);
-                    const int t1 = max(to - kItemCost, 0);
+                    const int steps = steps_of(keys_of(q, min(d.tok0 + 2 * p.tokens, q.n) - 1)), cost = steps + kPairCost;
+                    int to = (int)min((long long)cost, off + (w.end - u));
+                    if (to < cost) to = cut_at(to, cost, near);
+                    if (to <= off && to < cost) break;
+                    d.t0 = max(off - kPairCost, 0);
+                    const int t1 = max(to - kPairCost, 0);
                     const bool begins = d.t0 == 0, ends = to == cost;
                     if (t1 > d.t0) {
                         d.slot = begins && ends ? -1 : 2 * (int)blockIdx.x + (begins ? 1 : 0);
@@ -713,7 +735,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
                             int* h = p.headers + (lane * blocks + blockIdx.x) * HEADER;
                             const int tok0 = d.tok0 + lane * p.tokens;
                             h[1] = q.start, h[2] = hk, h[3] = tok0, h[4] = max(min(p.tokens, q.n - tok0), 0) * p.group;
-                            h[0] = (int)((u + (cost - off) - 1) / w.share) - (int)blockIdx.x + 1;
+                            h[0] = pieces_of(u + (cost - off), w.share, near, (int)blockIdx.x);
                         }
                         const int n = d.steps1;
                         int id = 0, next_id = page_at(d, d.t0);
@@ -774,13 +796,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
                 };
                 int b = w.b;
                 Request q = w.q;
-                int cost = steps_of(q.kv) + kItemCost;
+                int cost = steps_of(q.kv) + kSingleCost;
                 int hk = (int)(w.rest / cost), off = (int)(w.rest - (long long)hk * cost);
                 Item d;
                 for (long long u = w.u; ok && u < w.end;) {
                     const int to = (int)min((long long)cost, off + (w.end - u));
-                    d.t0 = max(off - kItemCost, 0);
-                    const int t1 = max(to - kItemCost, 0);
+                    d.t0 = max(off - kSingleCost, 0);
+                    const int t1 = max(to - kSingleCost, 0);
                     const bool begins = d.t0 == 0, ends = to == cost;
                     if (t1 > d.t0) {
                         d.start = q.start, d.n = q.n, d.kv = q.kv, d.b = b, d.hk = hk, d.last = 0;
@@ -801,7 +823,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
                         if (begins && !ends && lane == 0) {
                             int* h = p.headers + (2 * blocks + id) * HEADER;
                             h[1] = q.start, h[2] = hk, h[3] = d.tok0, h[4] = (q.n - d.tok0) * p.group;
-                            h[0] = (int)((u + (cost - off) - 1) / w.share) - id + 1;
+                            h[0] = pieces_of(u + (cost - off), w.share, 0, id);
                         }
                     }
                     u += to - off;
@@ -813,7 +835,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
                             q = request_of(p, b);
                         } while (!has_single(q, p.tokens));
                         if (b >= p.batch) break;
-                        cost = steps_of(q.kv) + kItemCost;
+                        cost = steps_of(q.kv) + kSingleCost;
                     }
                 }
                 d.last = 1;

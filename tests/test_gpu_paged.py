@@ -329,6 +329,16 @@ def test_attention_random_batches(seed):
     check_attention(ref.paged_state(100 + seed, kv, new, hq, hkv, rng.choice([64, 128]), rng.choice([16, 32, 64, 128, 512, 1024]), pad=rng.choice([0, 5])))
 
 
+@pytest.mark.parametrize("seed", range(8))
+def test_attention_of_prompts_whose_tiles_are_cut_near_their_edges(seed):
+    """From one to some ten places of the line per SM, in items of three to twelve places: cuts fall at, beside and into items."""
+    rng = random.Random(seed)
+    hq, hkv = rng.choice([(16, 16), (12, 12), (24, 8), (32, 4)])
+    new = [rng.randint(100, 420) for _ in range(rng.randint(4, 9))]
+    kv = [n + rng.choice([0, 0, rng.randint(1, 700)]) for n in new]
+    check_attention(ref.paged_state(200 + seed, kv, new, hq, hkv, rng.choice([64, 128]), 64))
+
+
 def test_attention_of_many_requests():
     """More requests than a block has threads: the sums take several rounds."""
     rng = random.Random(1)
