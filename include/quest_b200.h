@@ -368,7 +368,7 @@ int rope_paged_append_cuda_bf16(const void* qkv, long long ld, const void* table
  * once more without them, a warp per row at about 150 cycles a key: where more than 800 000 keys per SM come together with such rows
  * a wait may reach its limit (two seconds), and the call ends with a device status.
  * head_dim 64 or 128; page_size a power of two from 16 to 1024; n_head a multiple of n_kv_head, at most 128 times it; width * page_size at
- * most 2^25; strides multiples of 8, bases 16-byte aligned (QB200_ERR_UNSUPPORTED otherwise); scale not negative.  workspace:
+ * most 2^25, rows 2^29, batch 2^20 (requests without rows are walked over one by one); strides multiples of 8, bases 16-byte aligned (QB200_ERR_UNSUPPORTED otherwise); scale not negative.  workspace:
  * paged_attention_workspace(...) bytes for the current device, 16-byte aligned, used by this call alone while it runs.  Two kernels.
  */
 int paged_attention_cuda_bf16(void* out, const long long* out_strides, const void* q, const long long* q_strides,

@@ -1186,7 +1186,7 @@ extern "C" int paged_attention_cuda_bf16(void* out, const long long* out_strides
         !k_cache || !v_cache || num_pages == 0)
         return QB200_ERR_INVALID_ARGUMENT;
     if ((head_dim != 64 && head_dim != 128) || n_head % n_kv_head != 0 || n_head / n_kv_head > pa::BM || (page_size & (page_size - 1)) != 0 ||
-        page_size < 16 || page_size > 1024 || (long long)width * page_size > (1ll << 25) || rows > (1 << 29) || !aligned16(out) || !aligned16(q) ||
+        page_size < 16 || page_size > 1024 || (long long)width * page_size > (1ll << 25) || rows > (1 << 29) || batch > (1 << 20) || !aligned16(out) || !aligned16(q) ||
         !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(workspace))
         return QB200_ERR_UNSUPPORTED;
     for (int i = 0; i < 3; ++i)

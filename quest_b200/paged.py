@@ -171,7 +171,7 @@ def paged_attention(
     prompt, drafted tokens, or a mixture over the batch.  Query head h reads key and value head h / (n_head / n_kv_head), at most
     128 of them the same.  Rows that see no key (kv_lens 0: refused by ``page_assign``) give zeros; rows outside every request are
     not written.  What the pages hold behind a request's tokens does not matter, nor what a row does not see (later tokens of its
-    chunk, whatever they are).  head_dim 64 or 128, page_size a power of two from 16 to 1024; q and out may be views (strides in
+    chunk, whatever they are).  head_dim 64 or 128, page_size a power of two from 16 to 1024, at most 2^20 requests; q and out may be views (strides in
     multiples of 8 elements), out without memory in common with the inputs.  For inference: nothing is recorded for autograd."""
     num_pages, page_size, n_kv_head, head_dim = k_cache.shape
     rows, n_head, columns = q.shape

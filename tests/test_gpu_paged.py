@@ -347,6 +347,15 @@ def test_attention_of_many_requests():
     check_attention(ref.paged_state(12, kv, new, 2, 1, 64, 16))
 
 
+def test_attention_of_few_requests_among_very_many_without_rows():
+    """The warp that lists the work walks over every request between two that have rows."""
+    count = 150000
+    kv, new = [0] * count, [0] * count
+    for b, held, rows in ((0, 300, 1), (777, 140, 140), (90000, 17, 2), (count - 1, 600, 129)):
+        kv[b], new[b] = held, rows
+    check_attention(ref.paged_state(13, kv, new, 2, 2, 64, 64))
+
+
 def test_attention_with_scale_zero_is_the_mean_of_what_is_seen():
     s = ref.paged_state(13, [150, 20], [30, 1], 2, 2, 64, 16)
     check_attention(s, scale=0.0)

@@ -158,3 +158,10 @@ def test_attention_entry_refuses_scales_and_groups():
 
     assert call(scale=-1.0) == INVALID and call(scale=float("nan")) == INVALID
     assert call(hq=129) == UNSUPPORTED and call(page=2048) == UNSUPPORTED and call(width=(1 << 21) + 1) == UNSUPPORTED
+
+
+def test_attention_entry_refuses_more_requests_than_it_can_walk_over_within_its_waits():
+    lib = _lib.load()
+    buf, p = aligned_buffer()
+    two, three = (ctypes.c_longlong * 2)(64 * 256, 64), (ctypes.c_longlong * 3)(1024, 64, 64)
+    assert lib.paged_attention_cuda_bf16(p, two, p, two, p, three, p, three, p, p, p, p, 0.1, 2, (1 << 20) + 1, 3, 2, 1, 64, 4, 16, None) == UNSUPPORTED
