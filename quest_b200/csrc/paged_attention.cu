@@ -27,6 +27,7 @@
 //                                                the first product, 85 - 90 at the rate of HBM, 6 for the join
 //   one request of 1001 tokens, 16 / 16 heads, one new token    13 us, nearly all of it the chain of latencies
 //   one request of 32768 tokens, 64 / 8 heads, one new token    38 us, 3.5 TB/s
+//   the same with 8 / 1 heads                                  23 us, 0.7 TB/s: a chain of latencies, the join among them
 //   128 requests of at most 1000 tokens, 32 / 32 heads          116 - 130 us, 3.9 - 4.3 TB/s
 //   16 prompts of 1024, 16 / 16 heads                           107 - 120 us; tensor pipe and exponentials a third each
 //   4 prompts of 4096, 32 / 8 heads                             471 - 535 us, 1167 - 1028 TFLOP/s; head_dim 64 410 us
@@ -55,6 +56,10 @@ static_assert(128 * kControlRegs + 256 * kSoftmaxRegs <= kThreads * 168, "regist
 // and every cut where it falls, 23 like this.  Single items: 128 requests of 1000 tokens 115 us with one step, 129 with two; cuts
 // moved by up to two places leave 5 drafts for 32 requests at 38 us in place of 34.5).
 constexpr int kPairCost = 2, kPairNear = 1, kSingleCost = 1;
+// Steps of a single item from which a stream's piece of the line has three places at least (two from a quarter of that), however few
+// requests there are: pieces have to be joined, too (256 steps: 28.4 us with one, 23.8 with two, 23.0 with three, 23.6 with four; 70: 23.1,
+// 19.6, 20.3; 32: 17.2, 16.6, 20.0; 16: 15.1 with one, 16.5 with two).
+constexpr int kLongItem = 128;
 
 template <int D>
 struct Cfg {
@@ -441,6 +446,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
     Item* const items = reinterpret_cast<Item*>(gen + (bars - base) + 8 * C::NUM_BARS);  // three lists: pairs, stream 0, stream 1
     uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(items + 3 * ITEMS);
     __shared__ long long scan[2][kThreads / 32];
+    __shared__ int scan_longest[kThreads / 32];
     __shared__ Place places[3];  // of this block's pair, of its streams
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, blocks = gridDim.x;
@@ -464,6 +470,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
 
     // ---- the lines: all requests' sums, and the requests in which this block's pieces begin
     Request mine;
+    int longest = 0;  // steps of the longest single item
     long long per_head, places_of[2], run[2], carry[2] = {0, 0};  // of this thread's request; up to and with it; of all rounds so far
     auto sum_round = [&](int b) {
         mine = Request{0, 0, 0};
@@ -478,9 +485,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
                 if (lane >= d) run[k] += o;
             }
         }
+        const int most = __reduce_max_sync(~0u, places_of[1] > 0 ? steps_of(mine.kv) : 0);
         __syncthreads();
-        if (lane == 31) scan[0][warp] = run[0], scan[1][warp] = run[1];
+        if (lane == 31) scan[0][warp] = run[0], scan[1][warp] = run[1], scan_longest[warp] = most;
         __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kThreads / 32; ++w) longest = max(longest, scan_longest[w]);
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
             long long all = 0;
@@ -510,7 +520,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
         }
         if (pass == 0) {
             total[0] = carry[0], total[1] = carry[1], carry[0] = carry[1] = 0;
-            share[0] = max((total[0] + blocks - 1) / blocks, 1ll), share[1] = max((total[1] + 2 * blocks - 1) / (2 * blocks), 1ll);
+            share[0] = max((total[0] + blocks - 1) / blocks, 1ll);
+            share[1] = max((total[1] + 2 * blocks - 1) / (2 * blocks), longest >= kLongItem ? 3ll : longest >= kLongItem / 4 ? 2ll : 1ll);
             if (p.batch <= kThreads) {  // this thread's sums are still at hand
                 find((int)threadIdx.x);
                 break;
@@ -1016,53 +1027,69 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
     }
 }
 
-// Joins the pieces of the item that begins at worker x of the first kernel and goes on behind it: 32 rows and four pieces of four
-// columns each per warp, or eight rows at once where there are few.  A thread reads the results of several workers at a time, so
-// that an item cut over all blocks costs a few latencies and not one per block.
-template <int D, int WIDE, int AT_ONCE>
-__device__ __forceinline__ void join_row(const Params& p, const float* tail, int pieces, int row, const int (&at)[WIDE], __nv_bfloat16* dst) {
-    const long long slot_floats = (long long)p.slot_rows * (D + 2);
-    float top = -CUDART_INF_F, l = 0;
+// Joins the pieces of the item that begins at worker x of the first kernel and goes on behind it.  A thread reads the results of several
+// workers at a time, so that an item cut over many blocks costs a few latencies and not one per block.  SPREAD, for calls of so few
+// requests and heads that an item is cut over hundreds of blocks: a row has a block, a thread an eighth of its pieces (one request of
+// 32768 tokens, 8 / 1 heads: 46.7 -> 28.4 us at one step a piece; two of 16384, 12 / 2 heads of 64, four tokens: 64 -> 23; where items have less pieces the
+// blocks that it takes cost more than that: one request of 1001 tokens, 16 / 16 heads 13.2 us, 15.4 with SPREAD).
+template <int WIDE>
+struct Joined {
+    float top, l;
     float4 o[WIDE];
+};
+// Pieces first .. last - 1, AT_ONCE of them read at a time.
+template <int D, int WIDE, int AT_ONCE>
+__device__ __forceinline__ Joined<WIDE> join_pieces(const Params& p, const float* tail, int first, int last, int row, const int (&at)[WIDE]) {
+    const long long slot_floats = (long long)p.slot_rows * (D + 2);
+    Joined<WIDE> r;
+    r.top = -CUDART_INF_F, r.l = 0;
 #pragma unroll
-    for (int k = 0; k < WIDE; ++k) o[k] = make_float4(0, 0, 0, 0);
-    for (int i0 = 0; i0 < pieces; i0 += AT_ONCE) {
+    for (int k = 0; k < WIDE; ++k) r.o[k] = make_float4(0, 0, 0, 0);
+    for (int i0 = first; i0 < last; i0 += AT_ONCE) {
         float m[AT_ONCE], s[AT_ONCE];
         float4 x[AT_ONCE][WIDE];
 #pragma unroll
         for (int j = 0; j < AT_ONCE; ++j) {
             const int i = i0 + j;
             const float* slot = tail + (2ll * i - (i == 0 ? 0 : 1)) * slot_floats;  // the first piece is a tail, the others are heads
-            const bool there = i < pieces;
+            const bool there = i < last;
             m[j] = there ? slot[p.slot_rows * D + row] : -CUDART_INF_F;
             s[j] = there ? slot[p.slot_rows * (D + 1) + row] : 0.f;
 #pragma unroll
             for (int k = 0; k < WIDE; ++k) x[j][k] = there ? reinterpret_cast<const float4*>(slot)[at[k]] : make_float4(0, 0, 0, 0);
         }
-        float up = top;
+        float up = r.top;
 #pragma unroll
         for (int j = 0; j < AT_ONCE; ++j) up = fmaxf(up, m[j]);
-        const float w0 = weight_to(top, up);
-        top = up;
-        l *= w0;
+        const float w0 = weight_to(r.top, up);
+        r.top = up;
+        r.l *= w0;
 #pragma unroll
-        for (int k = 0; k < WIDE; ++k) o[k].x *= w0, o[k].y *= w0, o[k].z *= w0, o[k].w *= w0;
+        for (int k = 0; k < WIDE; ++k) r.o[k].x *= w0, r.o[k].y *= w0, r.o[k].z *= w0, r.o[k].w *= w0;
 #pragma unroll
         for (int j = 0; j < AT_ONCE; ++j) {
             const float w = weight_to(m[j], up);
-            l += w * s[j];
+            r.l += w * s[j];
 #pragma unroll
-            for (int k = 0; k < WIDE; ++k) o[k].x += w * x[j][k].x, o[k].y += w * x[j][k].y, o[k].z += w * x[j][k].z, o[k].w += w * x[j][k].w;
+            for (int k = 0; k < WIDE; ++k) r.o[k].x += w * x[j][k].x, r.o[k].y += w * x[j][k].y, r.o[k].z += w * x[j][k].z, r.o[k].w += w * x[j][k].w;
         }
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    return r;
+}
+template <int WIDE>
+__device__ __forceinline__ void store_joined(const Joined<WIDE>& r, __nv_bfloat16* dst) {
+    const float inv = r.l == 0.f ? 0.f : 1.f / r.l;
 #pragma unroll
     for (int k = 0; k < WIDE; ++k)
-        *reinterpret_cast<uint2*>(dst + 4 * k) = make_uint2(pack_bf16x2(o[k].x * inv, o[k].y * inv), pack_bf16x2(o[k].z * inv, o[k].w * inv));
+        *reinterpret_cast<uint2*>(dst + 4 * k) = make_uint2(pack_bf16x2(r.o[k].x * inv, r.o[k].y * inv), pack_bf16x2(r.o[k].z * inv, r.o[k].w * inv));
 }
 
-template <int D>
+constexpr int kSpreadItems = 4, kSpreadBlocks = 8;  // at most so many requests times heads; blocks for their rows
+template <int D, bool SPREAD>
 __global__ void __launch_bounds__(2 * D) paged_attention_join_kernel(const Params p) {
+    constexpr int PARTS = 8, MEMBERS = 2 * D / PARTS;  // of the pieces; a row's pieces of four columns
+    __shared__ float4 s_o[SPREAD ? PARTS : 1][MEMBERS];
+    __shared__ float2 s_ml[SPREAD ? PARTS : 1][MEMBERS];
     wait_for_preceding_grid();
     const int* header = p.headers + blockIdx.x * HEADER;
     const int4 h = *reinterpret_cast<const int4*>(header);
@@ -1073,17 +1100,38 @@ __global__ void __launch_bounds__(2 * D) paged_attention_join_kernel(const Param
         const int token = row / p.group, head = hk * p.group + (row - token * p.group);
         return p.out + (long long)(start + tok0 + token) * p.o_token + (long long)head * p.o_head;
     };
-    if (rows > 32) {
+    if (rows > 32) {  // 32 rows and four pieces of four columns each per warp
         const int chunk = threadIdx.x / 32 * 4;
         for (int row = blockIdx.y * 32 + threadIdx.x % 32; row < rows; row += gridDim.y * 32) {
             const int at[4] = {chunk * p.slot_rows + row, (chunk + 1) * p.slot_rows + row, (chunk + 2) * p.slot_rows + row, (chunk + 3) * p.slot_rows + row};
-            join_row<D, 4, 2>(p, tail, pieces, row, at, out_of(row) + 4 * chunk);
+            store_joined(join_pieces<D, 4, 2>(p, tail, 0, pieces, row, at), out_of(row) + 4 * chunk);
         }
-    } else {
+    } else if (!SPREAD) {  // eight rows at once
         const int chunk = threadIdx.x / 8;
         for (int row = blockIdx.y * 8 + threadIdx.x % 8; row < rows; row += gridDim.y * 8) {
             const int at[1] = {chunk * p.slot_rows + row};
-            join_row<D, 1, 8>(p, tail, pieces, row, at, out_of(row) + 4 * chunk);
+            store_joined(join_pieces<D, 1, 8>(p, tail, 0, pieces, row, at), out_of(row) + 4 * chunk);
+        }
+    } else {  // the parts' results in order, too
+        const int part = threadIdx.x / MEMBERS, chunk = threadIdx.x % MEMBERS;
+        const int share = (pieces + PARTS - 1) / PARTS, first = min(part * share, pieces), last = min(first + share, pieces);
+        for (int row = blockIdx.y; row < rows; row += gridDim.y) {
+            const int at[1] = {chunk * p.slot_rows + row};
+            Joined<1> r = join_pieces<D, 1, 8>(p, tail, first, last, row, at);
+            s_o[part][chunk] = r.o[0], s_ml[part][chunk] = make_float2(r.top, r.l);
+            __syncthreads();
+            if (part == 0) {
+#pragma unroll
+                for (int i = 1; i < PARTS; ++i) {
+                    const float2 ml = s_ml[i][chunk];
+                    const float4 o = s_o[i][chunk];
+                    const float up = fmaxf(r.top, ml.x), a = weight_to(r.top, up), b = weight_to(ml.x, up);
+                    r.top = up, r.l = r.l * a + ml.y * b;
+                    r.o[0].x = r.o[0].x * a + b * o.x, r.o[0].y = r.o[0].y * a + b * o.y, r.o[0].z = r.o[0].z * a + b * o.z, r.o[0].w = r.o[0].w * a + b * o.w;
+                }
+                store_joined(r, out_of(row) + 4 * chunk);
+            }
+            __syncthreads();
         }
     }
 }
@@ -1150,7 +1198,8 @@ static int launch(const Params& p, const CUtensorMap& qmap, const CUtensorMap& h
     const int st = launch_status();
     if (st != QB200_OK) return st;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(4 * blocks, (p.slot_rows + 63) / 64);  // one wave of blocks
+    const bool spread = (long long)p.batch * p.hkv <= kSpreadItems;
+    cfg.gridDim = dim3(4 * blocks, spread ? kSpreadBlocks : (p.slot_rows + 63) / 64);  // one wave of blocks where there are more items
     cfg.blockDim = dim3(2 * D);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
@@ -1158,7 +1207,7 @@ static int launch(const Params& p, const CUtensorMap& qmap, const CUtensorMap& h
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cuda_status(cudaLaunchKernelEx(&cfg, paged_attention_join_kernel<D>, p));
+    return cuda_status(spread ? cudaLaunchKernelEx(&cfg, paged_attention_join_kernel<D, true>, p) : cudaLaunchKernelEx(&cfg, paged_attention_join_kernel<D, false>, p));
 }
 
 }  // namespace pa
