@@ -56,9 +56,10 @@ static_assert(128 * kControlRegs + 256 * kSoftmaxRegs <= kThreads * 168, "regist
 // and every cut where it falls, 23 like this.  Single items: 128 requests of 1000 tokens 115 us with one step, 129 with two; cuts
 // moved by up to two places leave 5 drafts for 32 requests at 38 us in place of 34.5).
 constexpr int kPairCost = 2, kPairNear = 1, kSingleCost = 1;
-// Steps of a single item from which a stream's piece of the line has three places at least (two from a quarter of that), however few
-// requests there are: pieces have to be joined, too (256 steps: 28.4 us with one, 23.8 with two, 23.0 with three, 23.6 with four; 70: 23.1,
-// 19.6, 20.3; 32: 17.2, 16.6, 20.0; 16: 15.1 with one, 16.5 with two).
+// Steps of an item from which a stream's piece of the line has three places at least (two from a quarter of that), and a pair's eight,
+// however few requests there are: pieces have to be joined, too (single items of 256 steps: 28.4 us with one, 23.8 with two, 23.0 with
+// three, 23.6 with four; 70: 23.1, 19.6, 20.3; 32: 17.2, 16.6, 20.0; 16: 15.1 with one, 16.5 with two.  64 tokens behind 32704, 8 / 1
+// heads, two pairs of 256 steps: 57 us at four, 44 at eight, 37 with the join's reads of four pieces at once).
 constexpr int kLongItem = 128;
 
 template <int D>
@@ -470,7 +471,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
 
     // ---- the lines: all requests' sums, and the requests in which this block's pieces begin
     Request mine;
-    int longest = 0;  // steps of the longest single item
+    int longest = 0;  // steps of the longest item, or a little more
     long long per_head, places_of[2], run[2], carry[2] = {0, 0};  // of this thread's request; up to and with it; of all rounds so far
     auto sum_round = [&](int b) {
         mine = Request{0, 0, 0};
@@ -485,7 +486,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
                 if (lane >= d) run[k] += o;
             }
         }
-        const int most = __reduce_max_sync(~0u, places_of[1] > 0 ? steps_of(mine.kv) : 0);
+        const int most = __reduce_max_sync(~0u, mine.n > 0 ? steps_of(mine.kv) : 0);
         __syncthreads();
         if (lane == 31) scan[0][warp] = run[0], scan[1][warp] = run[1], scan_longest[warp] = most;
         __syncthreads();
@@ -520,7 +521,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
         }
         if (pass == 0) {
             total[0] = carry[0], total[1] = carry[1], carry[0] = carry[1] = 0;
-            share[0] = max((total[0] + blocks - 1) / blocks, 1ll);
+            share[0] = max((total[0] + blocks - 1) / blocks, longest >= kLongItem ? 8ll : 1ll);
             share[1] = max((total[1] + 2 * blocks - 1) / (2 * blocks), longest >= kLongItem ? 3ll : longest >= kLongItem / 4 ? 2ll : 1ll);
             if (p.batch <= kThreads) {  // this thread's sums are still at hand
                 find((int)threadIdx.x);
@@ -1104,7 +1105,7 @@ __global__ void __launch_bounds__(2 * D) paged_attention_join_kernel(const Param
         const int chunk = threadIdx.x / 32 * 4;
         for (int row = blockIdx.y * 32 + threadIdx.x % 32; row < rows; row += gridDim.y * 32) {
             const int at[4] = {chunk * p.slot_rows + row, (chunk + 1) * p.slot_rows + row, (chunk + 2) * p.slot_rows + row, (chunk + 3) * p.slot_rows + row};
-            store_joined(join_pieces<D, 4, 2>(p, tail, 0, pieces, row, at), out_of(row) + 4 * chunk);
+            store_joined(join_pieces<D, 4, SPREAD ? 4 : 2>(p, tail, 0, pieces, row, at), out_of(row) + 4 * chunk);
         }
     } else if (!SPREAD) {  // eight rows at once
         const int chunk = threadIdx.x / 8;

@@ -341,7 +341,7 @@ def test_attention_of_prompts_whose_tiles_are_cut_near_their_edges(seed):
 
 @pytest.mark.parametrize("hq, hkv, d, kv, new", [
     (8, 1, 128, [20000], [1]), (12, 2, 64, [9000, 3000], [4, 1]), (4, 4, 128, [4095], [1]), (5, 5, 64, [4097], [2]), (32, 1, 128, [6000, 1, 0, 40], [1, 1, 0, 3]),
-    (1, 1, 64, [16385], [64]), (128, 1, 128, [8000], [1])])
+    (1, 1, 64, [16385], [64]), (128, 1, 128, [8000], [1]), (8, 1, 128, [17000], [40]), (3, 1, 64, [16400, 700], [100, 300])])
 def test_attention_of_few_long_items(hq, hkv, d, kv, new):
     """Items cut over hundreds of blocks, joined by a block per row or by eight rows a block, at one to three steps a piece."""
     check_attention(ref.paged_state(14 + hq, kv, new, hq, hkv, d, 64))
