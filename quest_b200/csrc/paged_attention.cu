@@ -31,7 +31,7 @@
 //   128 requests of at most 1000 tokens, 32 / 32 heads          116 - 130 us, 3.9 - 4.3 TB/s
 //   16 prompts of 1024, 16 / 16 heads                           107 - 120 us; tensor pipe and exponentials a third each
 //   4 prompts of 4096, 32 / 8 heads                             471 - 535 us, 1167 - 1028 TFLOP/s; head_dim 64 410 us
-//   a chunk of 4096 behind 28672 tokens, among 15 single tokens, 64 / 8 heads    3.10 - 3.62 ms, 1330 - 1139 TFLOP/s
+//   a chunk of 4096 behind 28672 tokens, among 15 single tokens, 64 / 8 heads    3.10 - 3.68 ms, 1330 - 1120 TFLOP/s
 // A step of 128 rows by 128 keys costs the tensor core 2 x 8 products of 64 cycles and its warps 128 exponentials per thread, 16 a
 // cycle and SM: 1024 cycles each.  A stream's steps form a chain, 1900 cycles of softmax and 1330 of products and their hand-over; two
 // streams keep the tensor core busy two thirds of that.
