@@ -527,10 +527,11 @@ __global__ void __launch_bounds__(kVerifyThreads, 3) verify_drafts_kernel(const 
 
 using namespace qb;
 
-// More than 48 KB of dynamic shared memory has to be asked for, once per device.
+// What a launch may have without asking, 48 KB, holds the kernel's static shared memory, too (150 bytes at most here), so large
+// batches ask; always for the most that any batch needs, since host threads share the setting.
 template <typename Kernel>
 static int allow_smem(Kernel kernel, size_t bytes) {
-    return bytes <= 48 * 1024 ? QB200_OK : cuda_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    return bytes <= 32 * 1024 ? QB200_OK : cuda_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 8 * kMaxRequests));
 }
 
 extern "C" int page_assign_cuda(int* page_table, const int* free_pages, const int* free_count, const int* cached_lens,

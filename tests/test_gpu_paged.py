@@ -1,7 +1,11 @@
 """The serving operators on the GPU against plain 64-bit implementations."""
 from __future__ import annotations
 
+import os
 import random
+import subprocess
+import sys
+import threading
 
 import pytest
 import torch
@@ -554,3 +558,51 @@ def test_serving_step_in_a_graph_follows_the_lengths():
                 assert (error <= (2 ** -8 + 2 ** -10) * size + 2 ** -8 * want.abs()).all()
             row += n
     assert lens.tolist() == [h.size(0) for h in history]
+
+
+_BATCHES_OF_A_NEW_PROCESS = """
+import torch
+import quest_b200 as quest
+
+i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+for batch in range(6116, 6150):  # shared memory goes from below to beyond what a launch has without asking, the kernels' own variables included
+    table, free = torch.full((batch, 1), -1, dtype=torch.int32, device="cuda"), torch.arange(batch, dtype=torch.int32, device="cuda")
+    zeros, ones = torch.zeros(batch, dtype=torch.int32, device="cuda"), torch.ones(batch, dtype=torch.int32, device="cuda")
+    step = quest.page_assign(table, free, i32([batch]), zeros, ones, batch, 16)
+    assert step.free_count.tolist() == [0] and torch.equal(step.kv_lens, ones) and torch.equal(table[:, 0], free.flip(0)), batch
+    assert torch.equal(step.slots, 16 * free.flip(0).long()), batch
+    left = quest.page_release(table, free, step.free_count, step.lens, zeros, 16)
+    assert left.tolist() == [batch] and torch.equal(free, table[:, 0]), batch
+print("every batch was served")
+"""
+
+
+def test_page_tables_of_batches_that_just_need_more_shared_memory():
+    """In a process that has asked for nothing larger before, ascending."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(quest.__file__)))
+    run = subprocess.run([sys.executable, "-c", _BATCHES_OF_A_NEW_PROCESS], cwd=root, capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and "every batch was served" in run.stdout, run.stderr[-2000:]
+
+
+def test_page_tables_of_two_threads_with_different_batches():
+    """The shared memory that one call asks for does not shrink what another call's launch has."""
+    failures = []
+
+    def work(batch):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                table, free = torch.zeros(batch, 1, dtype=torch.int32, device="cuda"), torch.arange(batch, dtype=torch.int32, device="cuda")
+                zeros, ones, count = torch.zeros_like(free), torch.ones_like(free), i32([batch])
+                for _ in range(400):
+                    step = quest.page_assign(table, free, count, zeros, ones, batch, 16)
+                    quest.page_release(table, free.clone(), step.free_count, step.lens, zeros, 16)
+                assert step.free_count.item() == 0
+        except Exception as e:  # noqa: BLE001
+            failures.append(e)
+
+    threads = [threading.Thread(target=work, args=(batch,)) for batch in (8192, 6200, 7000)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failures, failures
