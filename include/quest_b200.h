@@ -386,8 +386,9 @@ int paged_attention_workspace(int rows, int batch, int n_head, int n_kv_head, in
  * inverting the running sum of max(target - draft, 0) of the first refused row (of its target row where that is zero
  * everywhere) or of the row behind the last draft: the first token whose running sum passes u times the total.
  *   tokens int64 [batch, max_drafts + 1]: the kept drafts, the drawn token, -1 behind it     accepted int32 [batch]: drafts kept
- * Drafts beyond max_drafts are not looked at.  Probabilities fp32 or bf16; negative ones and NaN count as 0, a drafted token
- * outside the vocabulary is refused.  vocab at most 8388608 (QB200_ERR_UNSUPPORTED beyond).
+ * Drafts beyond max_drafts are not looked at.  Probabilities fp32 or bf16; negative ones count as 0 and a NaN of the target's, too; a
+ * draft whose own probability is NaN is refused, and nothing is drawn where a draft's probability is NaN.  A drafted token outside the
+ * vocabulary is refused.  vocab at most 8388608 (QB200_ERR_UNSUPPORTED beyond).
  */
 int verify_drafts_cuda(const void* target_probs, const void* draft_probs, int probs_are_bf16, const long long* draft_tokens,
                        const int* cu_drafts, const float* uniforms, long long* tokens, int* accepted, int batch, int n_drafts,

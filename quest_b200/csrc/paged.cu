@@ -228,6 +228,14 @@ constexpr int kVerifyThreads = 256, kVerifyWarps = kVerifyThreads / 32, kSegment
 __device__ __forceinline__ float as_float(float v) { return v; }
 __device__ __forceinline__ float as_float(__nv_bfloat16 v) { return __bfloat162float(v); }
 
+// A draft's probability: what is negative counts as 0, a NaN stays one (no comparison holds for it, so its draft is refused and nothing
+// is drawn in its place).
+__device__ __forceinline__ float not_negative(float q) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(q), "f"(0.f));
+    return r;
+}
+
 // Rows of probabilities, and the memory that they are part of.
 template <typename T>
 struct Rows {
@@ -365,7 +373,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 3) verify_drafts_kernel(const 
         const long long x = p.tokens[c0 + i];
         bool good = false;
         if (x >= 0 && x < p.vocab) {
-            const double q = p.draft == nullptr ? 1.0 : (double)as_float(draft[(long long)i * p.vocab + x]);
+            const double q = p.draft == nullptr ? 1.0 : (double)not_negative(as_float(draft[(long long)i * p.vocab + x]));
             good = (double)p.u[c0 + b + i] * q < (double)as_float(target[(long long)i * p.vocab + x]);
         }
         if (!good) atomicMin(&s_refused, i);
@@ -387,6 +395,8 @@ __global__ void __launch_bounds__(kVerifyThreads, 3) verify_drafts_kernel(const 
         values8(a, x);
         if (residual && both) {
             values8(b, q);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) q[j] = not_negative(q[j]);
         } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {

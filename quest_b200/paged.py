@@ -215,7 +215,8 @@ def verify_drafts(
     ``draft_probs`` (same type, [drafts, vocab]) a draft has probability 1 in its own distribution.  The next token is drawn with
     the last uniform from max(target - draft, 0) of the first refused row, or from the row behind the last draft: the first whose
     running sum (in 64 bits) passes u times the total.  ``tokens`` holds the kept drafts, that token, and -1 behind it.  Drafts
-    beyond ``max_drafts`` are not looked at."""
+    beyond ``max_drafts`` are not looked at.  Negative probabilities count as 0, and so does a NaN of the target's; a draft whose own
+    probability is NaN is refused, and nothing is drawn where a draft's is NaN."""
     assert (target_probs.dtype is torch.float32 or target_probs.dtype is _bf16) and target_probs.dim() == 2 and target_probs.is_contiguous()
     assert draft_tokens.dtype is torch.int64 and draft_tokens.dim() == 1 and draft_tokens.is_contiguous()
     assert cu_drafts.dtype is _i32 and cu_drafts.dim() == 1 and cu_drafts.is_contiguous()

@@ -606,3 +606,32 @@ def test_page_tables_of_two_threads_with_different_batches():
     for t in threads:
         t.join()
     assert not failures, failures
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("vocab", [97, 2048])
+def test_verify_drafts_with_probabilities_that_are_none(vocab, dtype):
+    """Negative probabilities count as 0 on both sides.  A draft whose own probability is NaN is refused, and where a draft's probability
+    is NaN nothing is drawn in its place."""
+    target, draft, tokens, cu, u = drafts_case(vocab, [4, 2, 0, 3, 1] * 8, vocab, dtype)
+    g = torch.Generator().manual_seed(vocab)
+    n = tokens.numel()
+    below = torch.rand(draft.shape, generator=g) < 0.3
+    below[torch.arange(n), tokens] = torch.rand(n, generator=g) < 0.3  # the drafted token's among them
+    draft = torch.where(below, -3 * draft - 0.25, draft)
+    target = torch.where(torch.rand(target.shape, generator=g) < 0.2, -target - 0.125, target)
+
+    def check(draft):
+        want, accepted = ref.verify(target.clamp(min=0), draft.clamp(min=0), tokens.tolist(), cu, u, 4)  # clamp leaves a NaN
+        got, kept = quest.verify_drafts(target.cuda(), tokens.cuda(), i32(cu), u.cuda(), 4, draft_probs=draft.cuda())
+        assert kept.tolist() == accepted and got.tolist() == want
+
+    check(draft)
+    none = torch.rand(draft.shape, generator=g) < 0.2
+    none[torch.arange(n), tokens] = torch.rand(n, generator=g) < 0.3
+    check(torch.where(none, float("nan"), draft))
+    # nothing of the target's mass lies where a draft was below zero: what is drawn there is the target's own row
+    p = torch.tensor([[0.0, 0.0, 0.25, 0.75], [0.25] * 4]).to(dtype).cuda()
+    q = torch.tensor([[0.5, -4.0, 0.5, 0.0]]).to(dtype).cuda()
+    got, kept = quest.verify_drafts(p, torch.tensor([1], device="cuda"), i32([0, 1]), torch.tensor([0.5, 0.0], device="cuda"), 1, draft_probs=q)
+    assert kept.tolist() == [0] and got.tolist() == [[3, -1]]
