@@ -37,19 +37,24 @@ class PagedCache:
     def __init__(self, cfg: DecoderConfig, num_pages: int, max_requests: int, max_length: int = None, page_size: int = 64, device="cuda"):
         head_dim = cfg.n_embd // cfg.n_head
         max_length = cfg.sequence_length if max_length is None else max_length
-        assert page_size <= max_length <= cfg.sequence_length, "whole pages, up to the end of the rotary table"
-        self.page_size, self.num_pages = page_size, num_pages
+        assert page_size > 0 and 0 < max_length <= cfg.sequence_length, "up to the end of the rotary table"
+        self.page_size, self.num_pages, self.max_length = page_size, num_pages, max_length
         self.k, self.v = ([torch.zeros(num_pages, page_size, cfg.n_head, head_dim, dtype=torch.bfloat16, device=device)
                            for _ in range(cfg.n_layer)] for _ in range(2))
-        # whole pages would let a request grow beyond max_length by part of a page: the table has only full ones
-        self.page_table = torch.zeros(max_requests, max(1, max_length // page_size), dtype=torch.int32, device=device)
+        self.page_table = torch.zeros(max_requests, -(-max_length // page_size), dtype=torch.int32, device=device)
         self.free_pages = torch.arange(num_pages, dtype=torch.int32, device=device)
         self.free_count = torch.full((1,), num_pages, dtype=torch.int32, device=device)
         self.lens = torch.zeros(max_requests, dtype=torch.int32, device=device)
 
     def assign(self, new_lens: torch.Tensor, num_tokens: int) -> PageStep:
         """Room for ``new_lens[b]`` more tokens of every request; requests without room are refused (``page_assign``)."""
-        step = quest.page_assign(self.page_table, self.free_pages, self.free_count, self.lens, new_lens, num_tokens, self.page_size)
+        lens, room = self.lens, self.page_table.size(1) * self.page_size
+        if room > self.max_length:  # the table's last page goes beyond max_length: who would, too, is refused as one who has no page left
+            beyond = new_lens > self.max_length - lens
+            lens = torch.where(beyond, room, lens)
+        step = quest.page_assign(self.page_table, self.free_pages, self.free_count, lens, new_lens, num_tokens, self.page_size)
+        if room > self.max_length:
+            step = step._replace(lens=torch.where(beyond, self.lens, step.lens))
         self.lens.copy_(step.lens)
         self.free_count.copy_(step.free_count)
         return step
@@ -89,7 +94,9 @@ def generate(model: Decoder, cache: PagedCache, prompts: list[torch.Tensor], max
     if bool((cache.lens[:n] != 0).any()):
         raise ValueError("places of the cache are in use")
     held = [p.numel() + max(max_new - 1, 0) for p in prompts]  # the last new token is not kept
-    if max(held, default=0) > cache.page_table.size(1) * cache.page_size or sum(-(-h // cache.page_size) for h in held) > int(cache.free_count):
+    if max(held, default=0) > cache.max_length:
+        raise ValueError(f"a prompt and its continuation are longer than the cache's length of {cache.max_length} tokens")
+    if sum(-(-h // cache.page_size) for h in held) > int(cache.free_count):
         raise ValueError("the cache has too few free pages for these prompts and their continuation")
     if n == 0:
         return torch.empty(0, max_new, dtype=torch.long, device=device)

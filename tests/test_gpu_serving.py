@@ -271,3 +271,51 @@ def test_shorten_takes_negative_lengths_for_zero():
     serving.extend(model, cache, prompts_of([40])[0].cuda(), torch.tensor([20, 20], dtype=torch.int32, device="cuda"))
     cache.shorten(torch.tensor([-5, 100], dtype=torch.int32, device="cuda"))
     assert cache.lens.tolist() == [0, 20] and cache.free_count.item() == 2
+
+
+@pytest.mark.parametrize("max_length", [100, 33, 9])
+def test_requests_grow_to_the_cache_length_whatever_the_page_size(max_length):
+    """A length that is not whole pages: the last page is used up to it, and not beyond."""
+    model = make_model("bf16")
+    page = 16
+    cache = serving.PagedCache(CFG, 24, 3, max_length=max_length, page_size=page)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    prompt = prompts_of([max_length])[0].cuda()
+    hidden, step = serving.extend(model, cache, prompt, torch.tensor([max_length, 0, 0], **i32))
+    assert step.kv_lens.tolist() == [max_length, 0, 0] == cache.lens.tolist() and cache.free_count.item() == 24 - -(-max_length // page)
+    with torch.inference_mode():
+        assert relative(hidden, model(prompt[None])[0]) < 10 * 2 ** -9
+    # one token more is refused, what lies behind it in the batch is served, and what the step says is what the cache holds
+    free = cache.free_count.item()
+    for new in ([1, 3, max_length], [2 ** 31 - 1, 0, 0], [5, 0, 1]):
+        before = cache.lens.tolist()
+        rows = sum(min(n, 2 * max_length) for n in new)
+        _, step = serving.extend(model, cache, torch.zeros(rows, dtype=torch.long, device="cuda"), torch.tensor(new, **i32))
+        # (where the rows end within a request those behind it are refused, too: the second batch's)
+        served = [held + n <= max_length and sum(new[:b + 1]) <= rows for b, (held, n) in enumerate(zip(before, new))]
+        held = [b + n if s else b for b, n, s in zip(before, new, served)]
+        assert cache.lens.tolist() == held == step.lens.tolist()
+        assert step.kv_lens.tolist() == [h if s else 0 for h, s in zip(held, served)]
+        assert cache.free_count.item() == 24 - sum(-(-h // page) for h in held)
+        slots = step.slots.tolist()
+        assert all(s == -1 for s in slots[:min(new[0], rows)])
+    # a step of fewer new tokens is granted as always, negative ones count as none
+    _, step = serving.extend(model, cache, torch.zeros(2, dtype=torch.long, device="cuda"), torch.tensor([-7, 2, 0], **i32))
+    assert step.kv_lens.tolist() == [max_length, 5, max_length]
+    cache.shorten(torch.zeros(3, **i32))
+    assert cache.free_count.item() == 24 and free <= 24
+    tokens = serving.generate(model, cache, [prompt[:4].cpu()], max_length - 3)  # the last one is not kept
+    assert tokens.shape == (1, max_length - 3) and cache.free_count.item() == 24
+    with pytest.raises(ValueError, match="length"):
+        serving.generate(model, cache, [prompt[:4].cpu()], max_length - 2)
+
+
+def test_verify_at_the_cache_length():
+    model = make_model("bf16")
+    cache = serving.PagedCache(CFG, 24, 2, max_length=40, page_size=16)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    serving.extend(model, cache, prompts_of([70])[0].cuda(), torch.tensor([38, 32], **i32))
+    drafts, u = torch.zeros(2, 2, dtype=torch.long, device="cuda"), torch.zeros(2, 3, device="cuda")
+    tokens, kept = serving.verify(model, cache, torch.tensor([1, 2], device="cuda"), drafts, u)  # 38 + 3 do not fit, 32 + 3 do
+    assert tokens[0].tolist() == [-1] * 3 and kept.tolist() == [0, 2] and cache.lens.tolist() == [38, 35]
+    assert cache.free_count.item() == 24 - 3 - 3
