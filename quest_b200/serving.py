@@ -74,8 +74,9 @@ def extend(model: Decoder, cache: PagedCache, tokens: torch.Tensor, new_lens: to
     """Runs ``tokens`` [rows], the new tokens of the requests packed one after the other (``new_lens`` [max_requests] int32 of
     them; rows behind the last are padding), through the model.  Returns (hidden states [rows, n_embd], step).  Nothing is
     read on the host: a step of fixed size can be captured in a graph and replayed."""
-    step = cache.assign(new_lens, tokens.numel())
-    return model(tokens.view(1, -1), cache.layers(step))[0], step
+    rows = tokens.reshape(1, -1)
+    step = cache.assign(new_lens, rows.size(1))
+    return model(rows, cache.layers(step))[0], step
 
 
 def last_rows(step: PageStep) -> torch.Tensor:
@@ -124,9 +125,20 @@ def verify(model: Decoder, cache: PagedCache, tokens: torch.Tensor, drafts: torc
     out of the cache again.  ``uniforms`` [R, K + 1] fp32 in [0, 1); ``draft_probs`` [R, K, vocab] fp32.  Returns (new tokens
     [R, K + 1], -1 behind the last one; drafts kept [R]); the last new token is the next call's ``tokens``.  Places that are not
     ``active`` ([R] bool; all are by default) stay as they are, whatever their tokens are; they, and requests for which there are not
-    enough pages, get -1 throughout and 0."""
+    enough pages, get -1 throughout and 0.  Arguments are checked before the cache changes."""
+    device = cache.lens.device
+    if drafts.dim() != 2 or drafts.size(0) != cache.lens.numel() or drafts.dtype != torch.int64 or tokens.shape != drafts.shape[:1]:
+        raise ValueError("tokens [R] and drafts [R, K] int64, R the places of the cache")
     requests, count = drafts.shape
-    rows, device = requests * (count + 1), cache.lens.device
+    rows, vocab = requests * (count + 1), model.lm_head.out_features
+    if uniforms.numel() != rows or uniforms.dtype != torch.float32:
+        raise ValueError("uniforms [R, K + 1] fp32")
+    if draft_probs is not None and (draft_probs.numel() != requests * count * vocab or draft_probs.dtype != torch.float32):
+        raise ValueError("draft_probs [R, K, vocab] fp32")
+    if active is not None and (active.shape != (requests,) or active.dtype != torch.bool):
+        raise ValueError("active [R] bool")
+    if any(t is not None and t.device != device for t in (tokens, drafts, uniforms, draft_probs, active)):
+        raise ValueError(f"all tensors on the device of the cache, {device}")
     before = cache.lens.clone()
     new = torch.full((requests,), count + 1, dtype=torch.int32, device=device)
     packed = torch.cat([tokens[:, None], drafts], dim=1).view(-1)
@@ -142,7 +154,7 @@ def verify(model: Decoder, cache: PagedCache, tokens: torch.Tensor, drafts: torc
     probs = torch.softmax(model.lm_head(hidden).float(), dim=-1)
     cu = torch.arange(requests + 1, dtype=torch.int32, device=device) * count
     result, kept = quest.verify_drafts(probs, drafts.reshape(-1), cu, uniforms.reshape(-1), count,
-                                       draft_probs=None if draft_probs is None else draft_probs.reshape(requests * count, -1))
+                                       draft_probs=None if draft_probs is None else draft_probs.reshape(requests * count, vocab))
     served = step.kv_lens > 0
     if active is not None:
         served &= active

@@ -319,3 +319,33 @@ def test_verify_at_the_cache_length():
     tokens, kept = serving.verify(model, cache, torch.tensor([1, 2], device="cuda"), drafts, u)  # 38 + 3 do not fit, 32 + 3 do
     assert tokens[0].tolist() == [-1] * 3 and kept.tolist() == [0, 2] and cache.lens.tolist() == [38, 35]
     assert cache.free_count.item() == 24 - 3 - 3
+
+
+def test_verify_without_drafts_but_with_their_probabilities():
+    model = make_model("bf16")
+    cache, other = (serving.PagedCache(CFG, 16, 2, page_size=16) for _ in range(2))
+    for c in (cache, other):
+        serving.extend(model, c, prompts_of([30])[0].cuda(), torch.tensor([10, 20], dtype=torch.int32, device="cuda"))
+    last, drafts, u = torch.tensor([7, 11], device="cuda"), torch.empty(2, 0, dtype=torch.long, device="cuda"), torch.tensor([[0.2], [0.7]], device="cuda")
+    want, _ = serving.verify(model, other, last, drafts, u)
+    got, kept = serving.verify(model, cache, last, drafts, u, draft_probs=torch.empty(2, 0, CFG.vocab_size, device="cuda"))
+    assert got.tolist() == want.tolist() and got.shape == (2, 1) and kept.tolist() == [0, 0] and cache.lens.tolist() == [11, 21]
+
+
+def test_verify_refuses_before_the_cache_changes():
+    model = make_model("bf16")
+    cache = serving.PagedCache(CFG, 16, 2, page_size=16)
+    serving.extend(model, cache, prompts_of([30])[0].cuda(), torch.tensor([10, 20], dtype=torch.int32, device="cuda"))
+    good = dict(tokens=torch.tensor([7, 11], device="cuda"), drafts=torch.zeros(2, 3, dtype=torch.long, device="cuda"), uniforms=torch.zeros(2, 4, device="cuda"),
+                draft_probs=torch.zeros(2, 3, CFG.vocab_size, device="cuda"), active=torch.tensor([True, False], device="cuda"))
+    table = cache.page_table.clone()
+    for name, bad in (("tokens", torch.zeros(3, dtype=torch.long, device="cuda")), ("drafts", torch.zeros(3, 3, dtype=torch.long, device="cuda")),
+                      ("drafts", torch.zeros(2, 3, dtype=torch.int32, device="cuda")), ("drafts", torch.zeros(2, dtype=torch.long, device="cuda")),
+                      ("uniforms", torch.zeros(2, 3, device="cuda")), ("uniforms", torch.zeros(2, 4, dtype=torch.float64, device="cuda")),
+                      ("uniforms", torch.zeros(2, 4)), ("draft_probs", torch.zeros(2, 3, CFG.vocab_size + 1, device="cuda")),
+                      ("draft_probs", torch.zeros(2, 3, CFG.vocab_size, dtype=torch.bfloat16, device="cuda")),
+                      ("active", torch.ones(2, dtype=torch.int32, device="cuda")), ("active", torch.ones(3, dtype=torch.bool, device="cuda"))):
+        with pytest.raises(ValueError):
+            serving.verify(model, cache, **{**good, name: bad})
+        assert cache.lens.tolist() == [10, 20] and cache.free_count.item() == 13 and torch.equal(cache.page_table, table)
+    assert serving.verify(model, cache, **good)[1].tolist() == [3, 0] and cache.lens.tolist() == [14, 20]
