@@ -123,7 +123,7 @@ def rope_paged_append(
     (length, head_dim/2, 2; fp32 or bf16; the same bits as ``rope_inplace``) and writes keys and values to ``slots[r]`` of the
     caches [num_pages, page_size, n_kv_head, head_dim].  Returns the queries [rows, n_head, head_dim].  Rows with a slot or a
     position outside (``page_assign`` gives -1 to rows that are not in use) are left out: nothing of them is written.  The slots
-    of one call must differ."""
+    of one call must differ.  For inference: nothing is recorded for autograd."""
     num_pages, page_size, n_kv_head, head_dim = k_cache.shape
     k_strides, v_strides = k_cache.stride(), v_cache.stride()
     assert k_cache.dtype is v_cache.dtype is _bf16 and v_cache.shape == k_cache.shape and k_strides[3] == v_strides[3] == 1

@@ -184,7 +184,7 @@ class Decoder(nn.Module):
 
     def forward(self, idx: torch.Tensor, pages=None) -> torch.Tensor:
         """Hidden states of idx (B, T).  ``pages`` (a list with one ``serving.LayerPages`` per layer): idx (1, T) holds packed
-        tokens of many requests, which attend over the paged cache."""
+        tokens of many requests, which attend over the paged cache (for inference: refused where a gradient is asked for)."""
         x = self.transformer.wte(idx)
         for i, blk in enumerate(self.transformer.h):
             x = blk(x, self.rope, None if pages is None else pages[i])

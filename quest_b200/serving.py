@@ -11,7 +11,7 @@ import torch
 
 import quest_b200 as quest
 from .paged import PageStep
-from .prefill import Decoder, DecoderConfig
+from .prefill import Decoder, DecoderConfig, kernels_may_replace
 
 
 class LayerPages:
@@ -22,7 +22,9 @@ class LayerPages:
 
     def attend(self, qkv: torch.Tensor, table: torch.Tensor, n_head: int) -> torch.Tensor:
         """qkv [rows, 3 n_head head_dim], not rotated yet -> attention [rows, n_head, head_dim]; keys and values go to the pages.
-        Rows that belong to no request come out as zeros."""
+        Rows that belong to no request come out as zeros.  For inference: refused where a gradient is asked for."""
+        if not kernels_may_replace(qkv, table, self.k, self.v):
+            raise RuntimeError("attention over pages leaves no graph for a gradient: run the model under torch.no_grad() or torch.inference_mode()")
         head_dim = self.k.size(3)
         rows = qkv.size(0)
         q = quest.rope_paged_append(qkv, table, self.step.positions, self.step.slots, self.k, self.v, n_head)

@@ -349,3 +349,22 @@ def test_verify_refuses_before_the_cache_changes():
             serving.verify(model, cache, **{**good, name: bad})
         assert cache.lens.tolist() == [10, 20] and cache.free_count.item() == 13 and torch.equal(cache.page_table, table)
     assert serving.verify(model, cache, **good)[1].tolist() == [3, 0] and cache.lens.tolist() == [14, 20]
+
+
+@pytest.mark.parametrize("mode", ["bf16", "int4_fused"])
+def test_pages_refuse_where_a_gradient_is_asked_for(mode):
+    """The attention over pages leaves no graph: outside no_grad its part of a gradient would be missing without a word."""
+    model = make_model("bf16")
+    prompt = prompts_of([20])[0].cuda()
+    cache = serving.PagedCache(CFG, 8, 1, page_size=16)
+    step = cache.assign(torch.tensor([20], dtype=torch.int32, device="cuda"), 20)
+    with pytest.raises(RuntimeError, match="gradient"):
+        model(prompt[None], cache.layers(step))
+    assert not any(k.any() for k in cache.k)  # before anything is written
+    if mode != "bf16":
+        model = swap_linears(model, mode)
+    with torch.no_grad():
+        a = model(prompt[None], cache.layers(step))[0]
+    with torch.inference_mode():
+        b = model(prompt[None], cache.layers(step))[0]
+    assert torch.equal(a, b)

@@ -165,3 +165,19 @@ def test_attention_entry_refuses_more_requests_than_it_can_walk_over_within_its_
     buf, p = aligned_buffer()
     two, three = (ctypes.c_longlong * 2)(64 * 256, 64), (ctypes.c_longlong * 3)(1024, 64, 64)
     assert lib.paged_attention_cuda_bf16(p, two, p, two, p, three, p, three, p, p, p, p, 0.1, 2, (1 << 20) + 1, 3, 2, 1, 64, 4, 16, None) == UNSUPPORTED
+
+
+def test_pages_of_a_layer_refuse_where_a_gradient_is_asked_for():
+    from quest_b200.serving import LayerPages
+    k, v = (torch.zeros(5, 16, 4, 64, dtype=torch.bfloat16) for _ in range(2))
+    step = quest.PageStep(_i32(2), _i32(1), _i32(1), torch.zeros(3, dtype=torch.int64), _i32(3), _i32(1))
+    pages = LayerPages(k, v, _i32(1, 4), step)
+    qkv, table = torch.zeros(3, 3 * 4 * 64, dtype=torch.bfloat16), torch.zeros(9, 32, 2)
+    with pytest.raises(RuntimeError, match="gradient"):
+        pages.attend(qkv.clone().requires_grad_(), table, 4)
+    with pytest.raises(RuntimeError, match="gradient"), torch.autograd.forward_ad.dual_level():
+        pages.attend(qkv, table, 4)
+    with pytest.raises(RuntimeError, match="CUDA"):  # as far as the kernels
+        pages.attend(qkv, table, 4)
+    with pytest.raises(RuntimeError, match="CUDA"), torch.no_grad():
+        pages.attend(qkv.clone().requires_grad_(), table, 4)
