@@ -336,8 +336,8 @@ int rmsnorm_cuda_bf16(void* y, const void* x, const void* weight, float eps, int
  *   cu_new      [batch + 1] first row of each request (at most rows)        kv_lens [batch]  tokens to attend over, 0: refused
  *   lens        [batch] tokens held afterwards (cached_lens where refused)  slots int64 / positions int32 [rows], -1 / 0 behind the last
  * page_release_cuda: request b keeps keep_lens[b] of lens[b] tokens; the pages behind them return to the stack (what does not fit
- * into its `pool` entries is dropped).  The outputs of both must not overlap their inputs.  At most 8192 requests
- * (QB200_ERR_UNSUPPORTED beyond), width * page_size below 2^31.
+ * into its `pool` entries is dropped).  The outputs of both must not overlap their inputs.  At most 8192 requests; of
+ * page_assign_cuda rows at most 2^30 and width * page_size below 2^31, of page_release_cuda pool at most 2^30 (QB200_ERR_UNSUPPORTED beyond).
  */
 int page_assign_cuda(int* page_table, const int* free_pages, const int* free_count, const int* cached_lens, const int* new_lens,
                      int* cu_new, int* kv_lens, int* lens, long long* slots, int* positions, int* free_left, int batch, int width,
@@ -350,7 +350,7 @@ int page_release_cuda(const int* page_table, int* free_pages, const int* free_co
  * rope_inplace_cuda_bf16 does (row positions[r] of table [table_len, head_dim / 2, 2]); q goes to q_out [rows, n_head, head_dim],
  * k and v to slot slots[r] of the caches [num_pages, page_size, n_kv_head, head_dim] with strides (page, token, head) in
  * elements.  Rows whose slot or position lies outside the cache or the table are left out entirely.  Slots must differ.
- * head_dim, ld and strides multiples of 8, bases 16-byte aligned (QB200_ERR_UNSUPPORTED otherwise).
+ * head_dim, ld and strides multiples of 8, bases 16-byte aligned, at most 2^30 elements per row (QB200_ERR_UNSUPPORTED otherwise).
  */
 int rope_paged_append_cuda_bf16(const void* qkv, long long ld, const void* table, int table_is_bf16, const int* positions,
                                 const long long* slots, void* k_cache, const long long* k_strides, void* v_cache,
@@ -388,7 +388,7 @@ int paged_attention_workspace(int rows, int batch, int n_head, int n_kv_head, in
  *   tokens int64 [batch, max_drafts + 1]: the kept drafts, the drawn token, -1 behind it     accepted int32 [batch]: drafts kept
  * Drafts beyond max_drafts are not looked at.  Probabilities fp32 or bf16; negative ones count as 0 and a NaN of the target's, too; a
  * draft whose own probability is NaN is refused, and nothing is drawn where a draft's probability is NaN.  A drafted token outside the
- * vocabulary is refused.  vocab at most 8388608 (QB200_ERR_UNSUPPORTED beyond).
+ * vocabulary is refused.  vocab at most 2^23, batch 2^27, n_drafts and max_drafts 2^30 (QB200_ERR_UNSUPPORTED beyond).
  */
 int verify_drafts_cuda(const void* target_probs, const void* draft_probs, int probs_are_bf16, const long long* draft_tokens,
                        const int* cu_drafts, const float* uniforms, long long* tokens, int* accepted, int batch, int n_drafts,

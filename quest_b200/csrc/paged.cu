@@ -10,6 +10,7 @@ namespace cg = cooperative_groups;
 
 constexpr int kPageThreads = 512;
 constexpr int kMaxRequests = 8192;  // of one step: two arrays of that length lie in shared memory (64 KB)
+constexpr int kMaxEntries = 1 << 30;  // of what threads walk over in strides of a grid: an int index stays below 2^31
 
 // Inclusive sum over the block; `carry` is the sum of all earlier rounds and is advanced.  scratch: one word per warp.
 __device__ __forceinline__ long long block_inclusive_sum(long long v, long long& carry, long long* scratch) {
@@ -548,7 +549,7 @@ extern "C" int page_assign_cuda(int* page_table, const int* free_pages, const in
                                 const int* new_lens, int* cu_new, int* kv_lens, int* lens, long long* slots, int* positions,
                                 int* free_left, int batch, int width, int pool, int rows, int page_size, cudaStream_t stream) {
     if (batch < 0 || width < 0 || pool < 0 || rows < 0 || page_size <= 0) return QB200_ERR_INVALID_ARGUMENT;
-    if (batch > kMaxRequests || (long long)width * page_size > 0x7fffffffll) return QB200_ERR_UNSUPPORTED;
+    if (batch > kMaxRequests || (long long)width * page_size > 0x7fffffffll || rows > kMaxEntries) return QB200_ERR_UNSUPPORTED;
     if (!free_count || !cu_new || !free_left || (batch && (!cached_lens || !new_lens || !kv_lens || !lens)) || (rows && (!slots || !positions)) ||
         (batch && width && !page_table) || (pool && !free_pages))
         return QB200_ERR_INVALID_ARGUMENT;
@@ -566,7 +567,7 @@ extern "C" int page_release_cuda(const int* page_table, int* free_pages, const i
                                  const int* keep_lens, int* free_left, int batch, int width, int pool, int page_size,
                                  cudaStream_t stream) {
     if (batch < 0 || width < 0 || pool < 0 || page_size <= 0) return QB200_ERR_INVALID_ARGUMENT;
-    if (batch > kMaxRequests) return QB200_ERR_UNSUPPORTED;
+    if (batch > kMaxRequests || pool > kMaxEntries) return QB200_ERR_UNSUPPORTED;
     if (!free_count || !free_left || (batch && (!lens || !keep_lens)) || (batch && width && !page_table) || (pool && !free_pages))
         return QB200_ERR_INVALID_ARGUMENT;
     ReleaseParams p{page_table, free_pages, free_count, lens, keep_lens, free_left, batch, width, pool, page_size};
@@ -589,7 +590,7 @@ extern "C" int rope_paged_append_cuda_bf16(const void* qkv, long long ld, const 
     if (rows == 0 || n_head + n_kv_head == 0 || num_pages == 0 || table_len == 0) return QB200_OK;
     if (!qkv || !table || !positions || !slots || (n_head && !q_out) || !k_strides || !v_strides || (n_kv_head && (!k_cache || !v_cache)))
         return QB200_ERR_INVALID_ARGUMENT;
-    if (head_dim % 8 != 0 || ld % 8 != 0 || !aligned16(qkv) || !aligned16(table) || !aligned16(q_out) || !aligned16(k_cache) || !aligned16(v_cache))
+    if (n_head + 2ll * n_kv_head > kMaxEntries / head_dim || head_dim % 8 != 0 || ld % 8 != 0 || !aligned16(qkv) || !aligned16(table) || !aligned16(q_out) || !aligned16(k_cache) || !aligned16(v_cache))
         return QB200_ERR_UNSUPPORTED;
     for (int i = 0; i < 3; ++i)
         if (k_strides[i] % 8 != 0 || v_strides[i] % 8 != 0) return QB200_ERR_UNSUPPORTED;
@@ -619,7 +620,7 @@ extern "C" int verify_drafts_cuda(const void* target_probs, const void* draft_pr
     if (batch < 0 || n_drafts < 0 || vocab <= 0 || max_drafts < 0) return QB200_ERR_INVALID_ARGUMENT;
     if (batch == 0) return QB200_OK;
     if (!target_probs || !cu_drafts || !uniforms || !tokens || !accepted || (n_drafts && !draft_tokens)) return QB200_ERR_INVALID_ARGUMENT;
-    if (vocab > (1 << 23) || batch > (1 << 27)) return QB200_ERR_UNSUPPORTED;
+    if (vocab > (1 << 23) || batch > (1 << 27) || n_drafts > kMaxEntries || max_drafts > kMaxEntries) return QB200_ERR_UNSUPPORTED;
     VerifyParams p{target_probs, draft_probs, draft_tokens, cu_drafts, uniforms, tokens, accepted, batch, n_drafts, vocab, max_drafts};
     const bool vec = vocab % 8 == 0 && aligned16(target_probs) && aligned16(draft_probs);
     if (probs_are_bf16) return vec ? launch_verify<__nv_bfloat16, true>(p, stream) : launch_verify<__nv_bfloat16, false>(p, stream);

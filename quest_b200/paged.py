@@ -22,6 +22,7 @@ _Strides6, _Strides10 = ctypes.c_longlong * 6, ctypes.c_longlong * 10
 # These calls are short (a few microseconds on the device), so what Python does around them counts: types are compared by
 # identity, devices by index, and entry points looked up once.
 _i32, _bf16 = torch.int32, torch.bfloat16
+_MOST_INT = 2 ** 31 - 1  # ctypes cuts a larger argument to 32 bits without a word
 _entries: dict = {}
 
 
@@ -64,11 +65,12 @@ def page_assign(
 
     Requests are served in order.  One whose rows, table row or pages do not suffice is refused as a whole: it gets no page, its
     rows the slot -1 and its ``kv_lens`` is 0; where rows or pages have run out, so are the later ones that come behind them or need
-    a page.  Negative lengths count as 0.  At most 8192 requests."""
+    a page.  Negative lengths count as 0.  At most 8192 requests and 2^30 rows."""
     assert page_table.dtype is free_pages.dtype is free_count.dtype is cached_lens.dtype is new_lens.dtype is _i32
     assert (page_table.is_contiguous() and free_pages.is_contiguous() and free_count.is_contiguous() and cached_lens.is_contiguous()
             and new_lens.is_contiguous())
     assert page_table.dim() == 2 and free_pages.dim() == 1 and free_count.numel() == 1 and page_size > 0 and num_tokens >= 0
+    assert num_tokens <= _MOST_INT and page_size <= _MOST_INT and free_pages.numel() <= _MOST_INT
     batch, width = page_table.shape
     assert cached_lens.shape == new_lens.shape == (batch,)
     dev = page_table.get_device()
@@ -93,11 +95,12 @@ def page_release(
 ) -> torch.Tensor:
     """Shortens request b from ``lens[b]`` to ``keep_lens[b]`` tokens (0: it has finished): the pages behind them go to the end of
     the stack ``free_pages[:free_count]``.  Returns the new count [1]; the page table is left as it is (what lies behind a
-    request's length has no meaning).  ``free_pages`` must have room for every page of the pool."""
+    request's length has no meaning).  ``free_pages`` must have room for every page of the pool (2^30 at most)."""
     assert page_table.dtype is free_pages.dtype is free_count.dtype is lens.dtype is keep_lens.dtype is _i32
     assert (page_table.is_contiguous() and free_pages.is_contiguous() and free_count.is_contiguous() and lens.is_contiguous()
             and keep_lens.is_contiguous())
     assert page_table.dim() == 2 and free_pages.dim() == 1 and free_count.numel() == 1 and page_size > 0
+    assert page_size <= _MOST_INT and free_pages.numel() <= _MOST_INT
     batch, width = page_table.shape
     assert lens.shape == keep_lens.shape == (batch,)
     dev = page_table.get_device()
@@ -216,12 +219,12 @@ def verify_drafts(
     the last uniform from max(target - draft, 0) of the first refused row, or from the row behind the last draft: the first whose
     running sum (in 64 bits) passes u times the total.  ``tokens`` holds the kept drafts, that token, and -1 behind it.  Drafts
     beyond ``max_drafts`` are not looked at.  Negative probabilities count as 0, and so does a NaN of the target's; a draft whose own
-    probability is NaN is refused, and nothing is drawn where a draft's is NaN."""
+    probability is NaN is refused, and nothing is drawn where a draft's is NaN.  ``max_drafts`` and the drafts at most 2^30."""
     assert (target_probs.dtype is torch.float32 or target_probs.dtype is _bf16) and target_probs.dim() == 2 and target_probs.is_contiguous()
     assert draft_tokens.dtype is torch.int64 and draft_tokens.dim() == 1 and draft_tokens.is_contiguous()
     assert cu_drafts.dtype is _i32 and cu_drafts.dim() == 1 and cu_drafts.is_contiguous()
     n, batch, vocab = draft_tokens.numel(), cu_drafts.numel() - 1, target_probs.size(1)
-    assert batch >= 0 and max_drafts >= 0 and target_probs.size(0) == n + batch
+    assert batch >= 0 and 0 <= max_drafts <= _MOST_INT and n <= _MOST_INT and target_probs.size(0) == n + batch
     assert uniforms.dtype is torch.float32 and uniforms.is_contiguous() and uniforms.shape == (n + batch,)
     assert draft_probs is None or (draft_probs.dtype is target_probs.dtype and draft_probs.shape == (n, vocab) and draft_probs.is_contiguous())
     dev = target_probs.get_device()

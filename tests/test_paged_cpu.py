@@ -181,3 +181,27 @@ def test_pages_of_a_layer_refuse_where_a_gradient_is_asked_for():
         pages.attend(qkv, table, 4)
     with pytest.raises(RuntimeError, match="CUDA"), torch.no_grad():
         pages.attend(qkv.clone().requires_grad_(), table, 4)
+
+
+def test_entries_refuse_what_an_index_of_32_bits_cannot_walk_over():
+    """Threads go through rows, pages and places in strides of a grid: near 2^31 the next index would be negative.  (Without a
+    GPU a call that is not refused ends at its launch.)"""
+    lib = _lib.load()
+    buf, p = aligned_buffer()
+    most, beyond = 2 ** 31 - 1, 2 ** 30 + 1
+    for rows in (beyond, most):
+        assert lib.page_assign_cuda(*[p] * 11, 2, 4, 4, rows, 16, None) == UNSUPPORTED
+    for pool in (beyond, most):
+        assert lib.page_release_cuda(*[p] * 6, 2, 4, pool, 16, None) == UNSUPPORTED
+    for drafts, places in ((4, beyond), (4, most), (beyond, 4), (most, 4)):
+        assert lib.verify_drafts_cuda(p, p, 0, p, p, p, p, p, 1, drafts, 100, places, None) == UNSUPPORTED
+    strides = (ctypes.c_longlong * 3)(1024, 64, 64)
+    for heads, kv_heads, d in ((1 << 27, 1, 8), (1, 1 << 30, 8), (most, most, most - 7)):
+        assert lib.rope_paged_append_cuda_bf16(p, (1 << 62), p, 0, p, p, p, strides, p, strides, p, 1, heads, kv_heads, d, 8, 4, 16, None) == UNSUPPORTED
+
+
+@pytest.mark.parametrize("op, bad", [(_assign, dict(num_tokens=2 ** 32 + 3)), (_assign, dict(page_size=2 ** 32 + 16)), (_release, dict(page_size=2 ** 32 + 16)),
+                                     (_verify, dict(max_drafts=2 ** 32 + 2))])
+def test_arguments_beyond_32_bits_are_not_cut(op, bad):
+    with pytest.raises(AssertionError):
+        op(**bad)
