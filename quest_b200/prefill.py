@@ -111,9 +111,10 @@ class Block(nn.Module):
         self.ln_2, self.mlp = RMSNorm(cfg.n_embd, cfg.rmsnorm_eps), MLP(cfg)
 
     def forward(self, x, table, pages=None):
+        over = () if pages is None else (pages,)  # modules, and hooks on them, that know no pages are called as ever
         if getattr(self, "fused", False):
-            return self.forward_fused(x, table, pages)
-        x = x + self.attn(self.ln_1(x), table, pages)
+            return self.forward_fused(x, table, *over)
+        x = x + self.attn(self.ln_1(x), table, *over)
         return x + self.mlp(self.ln_2(x))
 
     def forward_fused(self, x, table, pages=None):
@@ -187,7 +188,7 @@ class Decoder(nn.Module):
         tokens of many requests, which attend over the paged cache (for inference: refused where a gradient is asked for)."""
         x = self.transformer.wte(idx)
         for i, blk in enumerate(self.transformer.h):
-            x = blk(x, self.rope, None if pages is None else pages[i])
+            x = blk(x, self.rope) if pages is None else blk(x, self.rope, pages[i])
         return self.transformer.ln_f(x)
 
 

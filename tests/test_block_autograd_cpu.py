@@ -107,3 +107,41 @@ def test_the_norm_keeps_its_eager_form_where_the_kernel_cannot_follow(monkeypatc
         norm.weight = nn.Parameter(torch.ones(1).to(torch.bfloat16))  # broadcast
         norm(x)
     assert len(calls) == 1
+
+
+def test_modules_that_know_no_pages_are_called_with_what_they_take():
+    """A forward pass without a paged cache hands its blocks and attentions the hidden states and the table, no more: modules put in
+    their place, and hooks on them, take two arguments."""
+
+    class Inner(nn.Module):
+        def __init__(self, module):
+            super().__init__()
+            self.module = module
+
+        def forward(self, x, table):
+            return self.module(x, table)
+
+    torch.manual_seed(0)
+    model = prefill.Decoder(DecoderConfig(n_embd=32, n_layer=3, n_head=2, ffn=64, vocab_size=50, sequence_length=16)).eval()
+    idx = torch.randint(0, 50, (2, 9))
+    with torch.no_grad():
+        want = model(idx)
+        seen = []
+        for blk in model.transformer.h:
+            blk.register_forward_pre_hook(lambda m, args: seen.append(len(args)))
+            blk.attn.register_forward_pre_hook(lambda m, args: seen.append(len(args)))
+        model.transformer.h[0] = Inner(model.transformer.h[0])
+        model.transformer.h[1].attn = Inner(model.transformer.h[1].attn)
+        assert torch.equal(model(idx), want)
+    assert seen == [2] * 6
+
+
+def test_a_fused_forward_of_two_arguments_is_called_with_them():
+    class Own(Block):
+        def forward_fused(self, x, table):
+            return x + 1
+
+    blk = Own(DecoderConfig(n_embd=32, n_layer=1, n_head=2, ffn=64))
+    blk.fused = True
+    x = torch.zeros(1, 3, 32)
+    assert torch.equal(blk(x, rope_table(16, 8)), x + 1)
