@@ -365,8 +365,7 @@ int rope_paged_append_cuda_bf16(const void* qkv, long long ld, const void* table
  * not matter, nor does what a row does not see (later tokens of its chunk that are not finite); a page table entry outside the pool
  * reads as keys and values of 0.  Strides in elements: q, out (token, head); caches (page, token, head).  Results do not depend on
  * timing: the same call gives the same bits.  out must not overlap an input.  Rows behind which values are not finite are summed
- * once more without them, a warp per row at about 150 cycles a key: where more than 800 000 keys per SM come together with such rows
- * a wait may reach its limit (two seconds), and the call ends with a device status.
+ * once more without them, a warp per row at about 150 cycles a key (32 rows over a million keys: 2.4 s); waits allow for it.
  * head_dim 64 or 128; page_size a power of two from 16 to 1024; n_head a multiple of n_kv_head, at most 128 times it; width * page_size at
  * most 2^25, rows 2^29, batch 2^20 (requests without rows are walked over one by one); strides multiples of 8, bases 16-byte aligned (QB200_ERR_UNSUPPORTED otherwise); scale not negative.  workspace:
  * paged_attention_workspace(...) bytes for the current device, 16-byte aligned, used by this call alone while it runs.  Two kernels.

@@ -215,16 +215,30 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
           "r"(r[31]), "r"(taddr)
         : "memory");
 }
-// A bounded wait (about two seconds), without a call - behind one the compiler cannot give the roles registers of their own - and
-// short: it stands at some fifty places, and the kernel's time on small calls is the time that its instructions take to arrive.
-constexpr uint32_t kLimitCycles = 4000000000u;
+// Units of 2^32 cycles (some two seconds) that a wait lasts at most.  A warp that sums rows again (visible_row), which over a long context
+// may take that long, adds what this may take before it begins.
+__device__ __forceinline__ int& wait_units() {
+    __shared__ int units;
+    return units;
+}
+constexpr int kWaitUnits = 2;  // the first begins anywhere in a unit: two to four seconds
+constexpr long long kAgainCycles = 1000;  // of visible_row per key, at the very most (about 150 measured)
+__device__ __forceinline__ uint32_t clock_units() {
+    uint32_t t;
+    asm volatile("mov.u32 %0, %%clock_hi;" : "=r"(t));
+    return t;
+}
+// A bounded wait, without a call - behind one the compiler cannot give the roles registers of their own - and
+// short: it stands at some fifty places, and the kernel's time on small calls is the time that its instructions take to arrive (128
+// requests of 1000 tokens: 113.4 us with a limit of 4 10^9 cycles and no more, 115.6 like this, 119 - 122 where every wait looked whether a
+// warp sums again and began anew).
 __device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity) {
     if (mbar_try_wait(bar, parity)) return true;
-    const uint32_t t0 = (uint32_t)clock();
+    const uint32_t t0 = clock_units();
 #pragma unroll 1
     do {
         if (mbar_try_wait(bar, parity)) return true;
-    } while ((uint32_t)clock() - t0 < kLimitCycles);
+    } while (clock_units() - t0 < (uint32_t)*(volatile int*)&wait_units());
     return false;
 }
 
@@ -466,6 +480,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
         fence_barrier_init();
     }
     if (threadIdx.x < 3) places[threadIdx.x].b = -1;
+    if (threadIdx.x == 0) wait_units() = kWaitUnits;
     if (threadIdx.x >= 32 && threadIdx.x < 36) p.headers[((threadIdx.x - 32) * blocks + blockIdx.x) * HEADER] = 0;
     let_dependents_launch();  // the joining kernel, which waits for this one's end
 
@@ -639,7 +654,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const Para
                 float nan0, nan1;
                 unpack2(add2(check[0], check[1]), nan0, nan1);
                 uint32_t bad = __ballot_sync(~0u, hidden && live && !(nan0 + nan1 == 0.f) && l > 0.f && l < CUDART_INF_F && keys < stop);
-                if (bad != 0) __syncwarp();  // the rows' stores are behind
+                if (bad != 0) {
+                    __syncwarp();  // the rows' stores are behind
+                    if (lane == 0) atomicAdd(&wait_units(), (int)(__popc(bad) * (stop - d.t0 * BN) * kAgainCycles >> 32));
+                }
                 while (bad != 0) {
                     const int from = __ffs(bad) - 1, r = __shfl_sync(~0u, row, from), t = __shfl_sync(~0u, token, from);
                     const int h = d.hk * p.group + __shfl_sync(~0u, row_head, from);

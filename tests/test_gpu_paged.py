@@ -415,6 +415,30 @@ def test_attention_and_append_in_a_cache_with_more_than_2_31_elements():
     assert torch.equal(v_cache[-1, 63].flatten(), qkv[0, (1 + hkv) * d:]) and torch.equal(v_cache[-1, 0].flatten(), qkv[1, (1 + hkv) * d:])
 
 
+def test_attention_waits_as_long_as_rows_in_front_of_a_nan_are_summed_again():
+    """Eleven requests of 2^25 tokens over nine pages, two new tokens each, the second one's values NaN.  The first token's 32 rows are
+    summed once more over up to 1.1 million keys by a warp, nearly three seconds in which the same stream's next item waits.  All scores
+    are zero, so weights are one (some exponentials are off by 7.5e-5, the sums of 9743 steps in fp32 by at most 9743 * 2^-24; together
+    below 2^-10), sums of values 0 and 1 are exact below 2^24, and a row is the mean of what it sees."""
+    batch, page, d, heads, width = 11, 1024, 64, 32, 2 ** 15
+    kv = width * page
+    g = torch.Generator().manual_seed(0)
+    v = torch.randint(0, 2, (9, page, 1, d), generator=g).bfloat16()
+    v[8, -1] = float("nan")
+    row = (torch.arange(width) % 8).int()
+    row[-1] = 8
+    q = torch.randn(2 * batch, heads, d, generator=g).bfloat16().cuda()
+    table = row.expand(batch, width).contiguous().cuda()
+    quest._lib.device_status()
+    got = quest.paged_attention(q, torch.zeros_like(v).cuda(), v.cuda(), table, i32([kv] * batch), i32(list(range(0, 2 * batch + 1, 2))))
+    got = got.double().cpu().view(batch, 2, heads, d)
+    assert quest._lib.device_status() == 0
+    sums = v.double()[:, :, 0].nan_to_num(0).sum(dim=1)
+    want = (torch.bincount(row.long(), minlength=9).double() @ sums) / (kv - 1)
+    assert ((got[:, 0] - want).abs() <= (2 ** -8 + 2 ** -10) * want).all()
+    assert torch.isnan(got[:, 1]).all()
+
+
 def test_attention_nothing_to_do():
     s = ref.paged_state(11, [5], [0], 4, 2, 64, 16)
     assert quest.paged_attention(**s).shape == (0, 4, 64)
