@@ -368,3 +368,52 @@ def test_pages_refuse_where_a_gradient_is_asked_for(mode):
     with torch.inference_mode():
         b = model(prompt[None], cache.layers(step))[0]
     assert torch.equal(a, b)
+
+
+class Follows(torch.nn.Module):
+    """A model whose next token is a function of the last one alone, with all of the probability on it."""
+
+    def __init__(self, successor):
+        super().__init__()
+        vocab = len(successor)
+        self.lm_head = torch.nn.Linear(vocab, vocab, bias=False, device="cuda")
+        self.lm_head.weight.data.zero_()
+        self.lm_head.weight.data[successor, torch.arange(vocab)] = 1e4
+
+    def forward(self, idx, pages):
+        return torch.nn.functional.one_hot(idx, self.lm_head.in_features).float()
+
+
+@pytest.mark.parametrize("count", [0, 1, 3])
+def test_verify_reads_every_active_place_its_own_logits(count):
+    """Every subset of four places: drafts are kept as far as they follow, the next token is what follows the last kept one, whichever
+    rows the places' tokens have in the packed batch."""
+    vocab, places = 50, 4
+    g = torch.Generator().manual_seed(count)
+    successor = torch.randperm(vocab, generator=g)
+    model = Follows(successor)
+    for subset in [None, *range(16)]:
+        cache = serving.PagedCache(CFG, 16, places, page_size=16)
+        cache.assign(torch.tensor([3, 20, 0, 15], dtype=torch.int32, device="cuda"), 38)
+        active = None if subset is None else [bool(subset >> b & 1) for b in range(places)]
+        last = torch.randint(0, vocab, (places,), generator=g)
+        drafts, right = torch.empty(places, count, dtype=torch.long), []
+        for b in range(places):
+            follows = int(torch.randint(0, count + 1, (1,), generator=g))
+            token = last[b]
+            for i in range(count):
+                token = successor[token] if i != follows else (successor[token] + 1) % vocab
+                drafts[b, i] = token
+            right.append(follows)
+        want, kept = [], []
+        for b in range(places):
+            if active is not None and not active[b]:
+                want.append([-1] * (count + 1)), kept.append(0)
+                last[b], drafts[b] = (-1, 10 ** 6)[b % 2], 10 ** 6  # never looked up
+            else:
+                sequence = [int(last[b]), *drafts[b, :right[b]].tolist()]
+                want.append(sequence[1:] + [int(successor[sequence[-1]])] + [-1] * (count - right[b])), kept.append(right[b])
+        u = torch.rand(places, count + 1, generator=g)
+        got, accepted = serving.verify(model, cache, last.cuda(), drafts.cuda(), u.cuda(), active=None if active is None else torch.tensor(active, device="cuda"))
+        assert got.tolist() == want and accepted.tolist() == kept
+        assert cache.lens.tolist() == [n + (0 if active is not None and not active[b] else 1 + kept[b]) for b, n in enumerate([3, 20, 0, 15])]
