@@ -417,3 +417,49 @@ def test_verify_reads_every_active_place_its_own_logits(count):
         got, accepted = serving.verify(model, cache, last.cuda(), drafts.cuda(), u.cuda(), active=None if active is None else torch.tensor(active, device="cuda"))
         assert got.tolist() == want and accepted.tolist() == kept
         assert cache.lens.tolist() == [n + (0 if active is not None and not active[b] else 1 + kept[b]) for b, n in enumerate([3, 20, 0, 15])]
+
+
+def test_captured_steps_run_up_to_the_cache_length_and_verify():
+    """A step of single tokens and a speculative step, captured over a cache whose length is not whole pages, replayed past its end."""
+    vocab, count = 50, 2
+    successor = torch.randperm(vocab, generator=torch.Generator().manual_seed(1))
+    model = Follows(successor)
+    i32 = dict(dtype=torch.int32, device="cuda")
+
+    def run(graphed):
+        cache = serving.PagedCache(CFG, 16, 2, max_length=39, page_size=16)
+        cache.assign(torch.tensor([30, 31], **i32), 61)
+        state = [t.clone() for t in (cache.lens, cache.free_count, cache.page_table, cache.free_pages)]
+        one, last = torch.ones(2, **i32), torch.tensor([3, 4], device="cuda")
+        drafts, u, active = torch.zeros(2, count, dtype=torch.long, device="cuda"), torch.full((2, count + 1), 0.5, device="cuda"), torch.tensor([True, False], device="cuda")
+
+        def step():
+            tokens, kept = serving.verify(model, cache, last, drafts, u, active=active)
+            _, single = serving.extend(model, cache, last, one)
+            return tokens, kept, single.kv_lens, single.slots, cache.lens.clone(), cache.free_count.clone()
+
+        if graphed:
+            side = torch.cuda.Stream()
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                step()
+            torch.cuda.current_stream().wait_stream(side)
+            for t, x in zip((cache.lens, cache.free_count, cache.page_table, cache.free_pages), state):
+                t.copy_(x)
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                results = step()
+        out = []
+        for i in range(8):
+            last.copy_(torch.tensor([3 + i, 4]))
+            first = int(successor[3 + i])
+            drafts[0] = torch.tensor([first, int(successor[first]) if i % 2 else 0])
+            active.copy_(torch.tensor([True, i > 4]))
+            if graphed:
+                graph.replay()
+            out.append([x.tolist() for x in (results if graphed else step())])
+        return out
+
+    eager = run(False)
+    assert run(True) == eager
+    assert eager[-1][4] == [39, 39] and eager[-1][0] == [[-1] * 3] * 2 and eager[-1][2] == [0, 0]  # by then both are full
