@@ -1103,7 +1103,7 @@ __device__ __forceinline__ void store_joined(const Joined<WIDE>& r, __nv_bfloat1
         *reinterpret_cast<uint2*>(dst + 4 * k) = make_uint2(pack_bf16x2(r.o[k].x * inv, r.o[k].y * inv), pack_bf16x2(r.o[k].z * inv, r.o[k].w * inv));
 }
 
-constexpr int kSpreadItems = 4, kSpreadBlocks = 8;  // at most so many requests times heads; blocks for their rows
+constexpr int kSpreadItems = 4, kSpreadBlocks = 8;  // at most so many rows of the page table times heads; blocks for their rows
 template <int D, bool SPREAD>
 __global__ void __launch_bounds__(2 * D) paged_attention_join_kernel(const Params p) {
     constexpr int PARTS = 8, MEMBERS = 2 * D / PARTS;  // of the pieces; a row's pieces of four columns
