@@ -224,7 +224,7 @@ struct VerifyParams {
     int batch, n_tokens, vocab, most;
 };
 
-constexpr int kVerifyThreads = 256, kVerifyWarps = kVerifyThreads / 32, kSegment = 256;
+constexpr int kVerifyThreads = 256, kVerifyWarps = kVerifyThreads / 32, kSegment = 256, kMostCluster = 8;
 
 __device__ __forceinline__ float as_float(float v) { return v; }
 __device__ __forceinline__ float as_float(__nv_bfloat16 v) { return __bfloat162float(v); }
@@ -244,8 +244,8 @@ struct Rows {
 };
 // Eight neighbouring entries of a row as they are read, zeros behind its end.  A row that does not begin on 16 bytes (an odd
 // vocabulary) is read in whole pieces all the same, one more of them, and shifted into place by values8; single entries are read where
-// a piece would reach beyond the tensor or the row.  500 requests at a vocabulary of 50257 take 45 us, and took 64
-// entry by entry.
+// a piece would reach beyond the tensor or the row.  500 requests at a vocabulary of 50257 took 45 us when
+// this was built, and 64 entry by entry (bf16; now 50, fp32 65).
 template <typename T, bool VEC>
 struct Raw8 {
     static constexpr int PIECES = (int)sizeof(T) / 2 + (VEC ? 0 : 1);
@@ -305,6 +305,24 @@ __device__ __forceinline__ void values8(const Raw8<T, VEC>& r, float (&x)[8]) {
     for (int j = 0; j < 8; ++j) x[j] = sizeof(T) == 4 ? __uint_as_float(w[j % OWN]) : j % 2 ? bf16hi_to_f32(w[j / 2]) : bf16lo_to_f32(w[j / 2]);
 }
 
+// The same of a draft's row: what is negative counts as 0, a NaN as more than any probability, so that nothing is left of the target's.
+template <typename T, bool VEC>
+__device__ __forceinline__ void draft8(Raw8<T, VEC> r, float (&q)[8]) {
+    if (sizeof(T) == 2) {  // two at once
+        uint32_t* const w = reinterpret_cast<uint32_t*>(r.w);
+#pragma unroll
+        for (int j = 0; j < 4 * r.PIECES; ++j) {
+            asm("min.bf16x2 %0, %0, %1;" : "+r"(w[j]) : "r"(0x7f7f7f7fu));  // the largest finite value
+            asm("max.bf16x2 %0, %0, %1;" : "+r"(w[j]) : "r"(0u));
+        }
+    }
+    values8(r, q);
+    if (sizeof(T) == 4) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) q[j] = fmaxf(fminf(q[j], 3e38f), 0.f);
+    }
+}
+
 __device__ __forceinline__ uint64_t pair_of(float a, float b) {
     uint64_t r;
     asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
@@ -323,175 +341,84 @@ __device__ __forceinline__ uint64_t sub_pair(uint64_t a, uint64_t b) {  // one r
 }
 
 // Sum of eight weights max(p - q, 0).  It decides between tokens, so it has to be as good as one in 64 bits, but 64-bit arithmetic
-// per entry cost more than reading it: the difference d is split into a multiple of 2^-16, whose sums are exact in fp32, and a
-// rest below 2^-17, whose sums lose less than 2^-38; two conversions for eight entries.  For fp32 the rounding of d itself is added back
-// (d + e = p - q exactly where p > q >= 0); the difference of two bf16 numbers has none unless one is 2^16 times the other.
-template <bool EXACT>
+// per entry cost more than reading it: with m = max(p, q) the difference m - q is split into h, its nearest multiple of 2^-16, whose sums
+// are exact in fp32, and the rest (m - h) - q, below 2^-17, whose sums lose less than 2^-38; two conversions for eight entries.  (m - h is
+// exact: both are multiples of m's last place, and h is no larger than m or, by less than that, the next multiple.  So what rounding the
+// difference itself would lose, next to a q of 2^-17 of p and less, is in the rest.)  What rests lose in all is far less than what u can
+// tell apart; where the aim is as near to a border as that, the decision is made in 64 bits (near_border).
 __device__ __forceinline__ double sum8(const float (&p)[8], const float (&q)[8]) {
     uint64_t high = 0, low = 0;
     const uint64_t magic = pair_of(192.f, 192.f);
 #pragma unroll
     for (int j = 0; j < 8; j += 2) {
-        const uint64_t p2 = pair_of(p[j], p[j + 1]), q2 = pair_of(q[j], q[j + 1]), d2 = sub_pair(p2, q2);
-        float d0, d1;
-        of_pair(d2, d0, d1);
-        const float w0 = fmaxf(d0, 0.f), w1 = fmaxf(d1, 0.f);  // what is not positive (a NaN among it) counts as nothing
-        const uint64_t w2 = pair_of(w0, w1), h = sub_pair(add_pair(w2, magic), magic);
-        uint64_t r = sub_pair(w2, h);
-        if (EXACT) {
-            float e0, e1;
-            of_pair(sub_pair(sub_pair(p2, d2), q2), e0, e1);
-            r = add_pair(r, pair_of(d0 > 0 ? e0 : 0.f, d1 > 0 ? e1 : 0.f));
-        }
-        high = add_pair(high, h), low = add_pair(low, r);
+        const uint64_t m2 = pair_of(fmaxf(p[j], q[j]), fmaxf(p[j + 1], q[j + 1])), q2 = pair_of(q[j], q[j + 1]);  // a NaN of p counts as nothing
+        const uint64_t h = sub_pair(add_pair(sub_pair(m2, q2), magic), magic);
+        high = add_pair(high, h), low = add_pair(low, sub_pair(sub_pair(m2, h), q2));
     }
     float a, b, c, d;
     of_pair(high, a, b), of_pair(low, c, d);
     return (double)(a + b) + (double)(c + d);
 }
 
-// Rejection sampling against a draft, one cluster of blocks per request.  Draft i is kept while u_i q_i(x_i) < p_i(x_i);
-// the next token is drawn from max(p - q, 0) of the first refused row, or from the row behind the last draft, by inverting the
-// running sum at u times the total.  Every warp of the cluster sums a stretch of the vocabulary; the totals go round the cluster, and
-// the block that holds the border reads the stretch of that warp again, a segment of 256 entries per warp.  So a row is read once;
-// without clusters a request would have a single SM's bandwidth or a second launch.  The chain of reads (offsets, tokens, their
-// probabilities, rows, the border) is what small calls wait for: seven requests at 32000 take 6 us; 200 at 131072, two rows of bf16
-// for two thirds of them, 27.5 us, 3.2 TB/s.
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(kVerifyThreads, 3) verify_drafts_kernel(const VerifyParams p) {
-    __shared__ int s_refused, s_last, s_hit, s_fall;  // s_last: last entry of this block with a weight, -1: none
-    __shared__ double s_warp[kVerifyWarps], s_total;
-    cg::cluster_group cluster = cg::this_cluster();
-    const int blocks = (int)cluster.num_blocks(), b = blockIdx.x / blocks, rank = blockIdx.x % blocks;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int c0 = min(max(p.cu[b], 0), p.n_tokens), c1 = min(max(p.cu[b + 1], c0), p.n_tokens);
-    const int drafts = min(c1 - c0, p.most);
-    const T* target = static_cast<const T*>(p.target) + (long long)(c0 + b) * p.vocab;
-    const T* draft = static_cast<const T*>(p.draft) + (p.draft == nullptr ? 0 : (long long)c0 * p.vocab);
-    if (threadIdx.x == 0) s_refused = drafts;
-    __syncthreads();
-    for (int i = threadIdx.x; i < drafts; i += kVerifyThreads) {
-        const long long x = p.tokens[c0 + i];
-        bool good = false;
-        if (x >= 0 && x < p.vocab) {
-            const double q = p.draft == nullptr ? 1.0 : (double)not_negative(as_float(draft[(long long)i * p.vocab + x]));
-            good = (double)p.u[c0 + b + i] * q < (double)as_float(target[(long long)i * p.vocab + x]);
-        }
-        if (!good) atomicMin(&s_refused, i);
-    }
-    __syncthreads();
-    const int kept = s_refused;
-    const bool refused = kept < drafts;
-    const T *targets = static_cast<const T*>(p.target), *drafted = static_cast<const T*>(p.draft);
-    const Rows<T> prow{target + (long long)kept * p.vocab, targets, targets + (long long)(p.n_tokens + p.batch) * p.vocab};
-    const Rows<T> qrow{draft + (long long)kept * p.vocab, drafted, drafted + (long long)p.n_tokens * p.vocab};
-    const long long hot = refused && p.draft == nullptr ? p.tokens[c0 + kept] : -1;  // a draft without probabilities: all on its token
+// How far from a border the sums of sum8 may be off.  A group's rests add up to at most 2^-14, or to the row's total where that is less, and
+// lose some 2^-25 of it in either direction: over the groups of a row about 2^-25 times the root of that times the total.  Eight times as
+// much is taken for near, a whole one for bf16, whose eight bits mostly leave nothing to lose (emulated on the host over rows of all kinds the sums
+// are off by at most 0.15 and 0.26 of it), and all that 24 bits can lose for weights that are no probabilities.
+template <typename T>
+__device__ __forceinline__ double near_border(double total) {
+    const float t = (float)total;
+    return t > 64.f ? t * 0x1p-21f : sqrtf(fminf(t, 0x1p-14f)) * sqrtf(t) * (sizeof(T) == 4 ? 0x1p-22f : 0x1p-25f);
+}
 
-    const int segments = (p.vocab + kSegment - 1) / kSegment;
-    const int share = (segments + blocks * kVerifyWarps - 1) / (blocks * kVerifyWarps);  // of a warp
-    const int seg0 = min((rank * kVerifyWarps + warp) * share, segments), seg1 = min(seg0 + share, segments);
-    bool residual = refused;
-    const bool both = p.draft != nullptr;
-    auto unpack = [&](const Raw8<T, VEC>& a, const Raw8<T, VEC>& b, int at, float (&x)[8], float (&q)[8]) {
+// The difference of a target's row and a draft's (or nothing, or all on the token `hot`), as verify_drafts_kernel reads it.
+template <typename T, bool VEC>
+struct Weights {
+    Rows<T> target, draft;
+    bool minus_draft;
+    long long hot;  // has no weight; -1: none
+    int vocab;
+    __device__ __forceinline__ void read(int at, Raw8<T, VEC>& a, Raw8<T, VEC>& c) const {
+        a = read8<T, VEC>(target, at, vocab);
+        if (minus_draft) c = read8<T, VEC>(draft, at, vocab);
+    }
+    __device__ __forceinline__ void unpack(const Raw8<T, VEC>& a, const Raw8<T, VEC>& c, int at, float (&x)[8], float (&q)[8]) const {
         values8(a, x);
-        if (residual && both) {
-            values8(b, q);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) q[j] = not_negative(q[j]);
+        if (minus_draft) {
+            draft8(c, q);
         } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 q[j] = 0;
-                if (residual && at + j == hot) x[j] = 0;
+                if (at + j == hot) x[j] = 0;
             }
         }
-    };
-    constexpr int AHEAD = (VEC ? 8 : 4) / sizeof(T);  // segments whose reads are under way at once
-    double total = 0, before = 0;  // of all blocks, of those before this one
-    int last = -1;
-    while (true) {
-        if (threadIdx.x == 0) s_last = -1;
-        __syncthreads();
-        double sum = 0;
-        int mine = -1;
-        for (int s = seg0; s < seg1; s += AHEAD) {
-            Raw8<T, VEC> a[AHEAD], c[AHEAD];
-#pragma unroll
-            for (int k = 0; k < AHEAD; ++k) {
-                const int at = s + k < seg1 ? (s + k) * kSegment + lane * 8 : p.vocab;
-                a[k] = read8<T, VEC>(prow, at, p.vocab);
-                if (residual && both) c[k] = read8<T, VEC>(qrow, at, p.vocab);
-            }
-#pragma unroll
-            for (int k = 0; k < AHEAD; ++k) {
-                float x[8], q[8];
-                const int at = (s + k) * kSegment + lane * 8;
-                unpack(a[k], c[k], at, x, q);
-                const double add = sum8<sizeof(T) == 4>(x, q);
-                sum += add;
-                if (add > 0) mine = at;
-            }
-        }
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
-        mine = __reduce_max_sync(~0u, mine);
-        if (lane == 0) {
-            s_warp[warp] = sum;
-            if (mine >= 0) atomicMax(&s_last, mine);
-        }
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            double t = 0;
-            for (int w = 0; w < kVerifyWarps; ++w) t += s_warp[w];
-            s_total = t;
-        }
-        cluster.sync();
-        total = before = 0;
-        last = -1;
-        for (int r = 0; r < blocks; ++r) {
-            if (r == rank) before = total;
-            total += *cluster.map_shared_rank(&s_total, r);
-            last = max(last, *cluster.map_shared_rank(&s_last, r));
-        }
-        cluster.sync();  // nobody leaves or starts over while another block reads
-        if (total > 0 || !residual) break;
-        residual = false;  // a refused draft whose distribution covers the target's: the target's own row
     }
+};
+template <typename T, bool VEC>
+__device__ __forceinline__ Weights<T, VEC> weights_of(const VerifyParams& p, int b, int c0, int kept, bool residual) {
+    const T *targets = static_cast<const T*>(p.target), *drafted = static_cast<const T*>(p.draft);
+    return Weights<T, VEC>{Rows<T>{targets + (long long)(c0 + b + kept) * p.vocab, targets, targets + (long long)(p.n_tokens + p.batch) * p.vocab},
+                           Rows<T>{p.draft == nullptr ? nullptr : drafted + (long long)(c0 + kept) * p.vocab, drafted, drafted + (long long)p.n_tokens * p.vocab},
+                           residual && p.draft != nullptr, residual && p.draft == nullptr ? p.tokens[c0 + kept] : -1, p.vocab};
+}
 
-    const double aim = fmax((double)p.u[c1 + b] * total, 0.0);
-    if (rank == 0) {
-        for (int i = threadIdx.x; i <= p.most; i += kVerifyThreads)
-            if (i != kept) p.out[(long long)b * (p.most + 1) + i] = i < kept ? p.tokens[c0 + i] : -1;
-        if (threadIdx.x == 0) p.accepted[b] = kept;
-    }
-    long long* slot = p.out + (long long)b * (p.most + 1) + kept;
-    // The block whose part holds the aim; where u rounds to one the one with the last weight, and without any weight the first.
-    const bool beyond = !(aim < total);
-    const int per_block = share * kVerifyWarps * kSegment;
-    if (beyond ? rank != (last < 0 ? 0 : last / per_block) : !(before <= aim && aim < before + s_total)) return;
-    if (beyond && last < 0) {
-        if (threadIdx.x == 0) *slot = 0;
-        return;
-    }
-    // ---- the warp's stretch, then the segment, then the entry
-    int w = 0;
-    double base = before;
-    if (beyond) {
-        w = (last - rank * per_block) / (share * kSegment);
-    } else {
-        while (w + 1 < kVerifyWarps && !(base + s_warp[w] > aim)) base += s_warp[w++];
-    }
-    const int first = (rank * kVerifyWarps + w) * share, end = min(first + share, segments);
-    if (threadIdx.x == 0) s_hit = 0x7fffffff, s_fall = -1;
+struct VerifyShared {
+    int refused, last, hit, fall, near;  // last: last entry of this block with a weight, -1: none
+    double warp[kVerifyWarps], total;
+};
+// The entry of a warp's stretch whose running sum, from base on, passes the goal (hit; none: 0x7fffffff), the last one with a weight
+// (fall), and whether the border in front of the entry or that behind it is as near to the goal as `near`.
+template <bool LAST_WORD, typename T, bool VEC>
+__device__ __forceinline__ void search_stretch(VerifyShared& sh, const Weights<T, VEC>& weights, int first, int end, double base, double goal, double near) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    if (threadIdx.x == 0) sh.hit = 0x7fffffff, sh.fall = -1, sh.near = 0;
     for (int s = first; s < end; s += kVerifyWarps) {
         float x[8], q[8];
         double v[8], sum = 0;
         const int at = (s + warp) * kSegment + lane * 8;
-        const int from = s + warp < end ? at : p.vocab;
-        Raw8<T, VEC> c;
-        const Raw8<T, VEC> a = read8<T, VEC>(prow, from, p.vocab);
-        if (residual && both) c = read8<T, VEC>(qrow, from, p.vocab);
-        unpack(a, c, at, x, q);
+        Raw8<T, VEC> a, c;
+        weights.read(s + warp < end ? at : weights.vocab, a, c);
+        weights.unpack(a, c, at, x, q);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             v[j] = (double)x[j] - (double)q[j];
@@ -505,33 +432,199 @@ __global__ void __launch_bounds__(kVerifyThreads, 3) verify_drafts_kernel(const 
             if (lane >= d) run += o;
         }
         __syncthreads();  // the round before has been read
-        if (lane == 31) s_warp[warp] = run;
+        if (lane == 31) sh.warp[warp] = run;
         __syncthreads();
         double mine = base;
         for (int k = 0; k < kVerifyWarps; ++k) {
             if (k == warp) mine = base;
-            base += s_warp[k];
+            base += sh.warp[k];
         }
-        run += mine - sum;
-        int hit = 0x7fffffff, fall = -1;
+        const double end_here = mine + run, before = __shfl_up_sync(~0u, end_here, 1), start_here = lane == 0 ? mine : before;
+        int fall = -1;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            run += v[j];
-            if (v[j] > 0) {
-                if (run > aim) hit = min(hit, at + j);
-                fall = at + j;
+        for (int j = 0; j < 8; ++j) fall = v[j] > 0 ? at + j : fall;
+        // One lane's sums pass the goal, but for their rounding in 64 bits.  Then a border is near, and the search is not the last word;
+        // where it is, the first of each warp's lanes that are behind the goal counts, and of those the first.
+        bool passes = end_here > goal && fall >= 0;
+        if (LAST_WORD) {
+            const uint32_t all = __ballot_sync(~0u, passes);
+            passes = passes && lane == __ffs(all) - 1;
+        } else {
+            passes = passes && start_here <= goal;
+        }
+        if (passes) {
+            double r = start_here, from = r, to = end_here;
+            int hit = fall;
+            bool found = false;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const double up = r + v[j];
+                if (!found && up > goal) found = true, hit = at + j, from = r, to = up;
+                r = up;
             }
+            atomicMin(&sh.hit, hit);
+            if ((from > 0 && fabs(goal - from) <= near) || to - goal <= near) sh.near = 1;
         }
-        hit = __reduce_min_sync(~0u, hit);
         fall = __reduce_max_sync(~0u, fall);
-        if (lane == 0) {
-            if (hit != 0x7fffffff) atomicMin(&s_hit, hit);
-            if (fall >= 0) atomicMax(&s_fall, fall);
-        }
+        if (lane == 0 && fall >= 0) atomicMax(&sh.fall, fall);
     }
     __syncthreads();
-    // Behind the stretch's last weight by the rounding of the sums (or of u): that weight.
-    if (threadIdx.x == 0) *slot = !beyond && s_hit != 0x7fffffff ? s_hit : s_fall >= 0 ? s_fall : last;
+}
+
+// The token once more, with all sums in 64 bits, by one block: where a border is near.  Seldom called, and a function of its own that
+// begins anew, so that it costs the kernel few registers and instructions (7 requests: 5.8 us without it, 6.2 like this, 7.1 with it inside; 200 at 131072: 27.9, 28.9 and 30.4).
+template <typename T, bool VEC>
+__device__ __noinline__ void draw_in_64_bits(const VerifyParams* params, VerifyShared* sh, int b, int c0, int kept, bool residual, float u, int stretches) {
+    __shared__ double sums[kMostCluster * kVerifyWarps];
+    const VerifyParams& p = *params;
+    const Weights<T, VEC> weights = weights_of<T, VEC>(p, b, c0, kept, residual);
+    const int lane = threadIdx.x & 31, segments = (p.vocab + kSegment - 1) / kSegment, share = (segments + stretches - 1) / stretches;
+    constexpr int AHEAD = 4 / sizeof(T);
+    for (int i = threadIdx.x >> 5; i < stretches; i += kVerifyWarps) {
+        const int end = min((i + 1) * share, segments);
+        double sum = 0;
+        for (int s = i * share; s < end; s += AHEAD) {
+            Raw8<T, VEC> a[AHEAD], c[AHEAD];
+#pragma unroll
+            for (int k = 0; k < AHEAD; ++k) weights.read(s + k < end ? (s + k) * kSegment + lane * 8 : p.vocab, a[k], c[k]);
+#pragma unroll
+            for (int k = 0; k < AHEAD; ++k) {
+                float x[8], q[8];
+                weights.unpack(a[k], c[k], (s + k) * kSegment + lane * 8, x, q);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) sum += fmax((double)x[j] - (double)q[j], 0.0);
+            }
+        }
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
+        if (lane == 0) sums[i] = sum;
+    }
+    __syncthreads();
+    double total = 0, base = 0;
+    for (int i = 0; i < stretches; ++i) total += sums[i];
+    const double aim = fmax((double)u * total, 0.0);
+    int i = 0;
+    for (; i + 1 < stretches && !(base + sums[i] > aim); ++i) base += sums[i];
+    search_stretch<true>(*sh, weights, i * share, min((i + 1) * share, segments), base, aim, -1);
+    if (threadIdx.x == 0) p.out[(long long)b * (p.most + 1) + kept] = sh->hit != 0x7fffffff ? sh->hit : sh->fall;
+}
+
+// Rejection sampling against a draft, one cluster of blocks per request.  Draft i is kept while u_i q_i(x_i) < p_i(x_i);
+// the next token is drawn from max(p - q, 0) of the first refused row, or from the row behind the last draft, by inverting the
+// running sum at u times the total.  Every warp of the cluster sums a stretch of the vocabulary; the totals go round the cluster, and
+// the block that holds the border reads the stretch of that warp again, a segment of 256 entries per warp.  So a row is read once;
+// without clusters a request would have a single SM's bandwidth or a second launch.  The chain of reads (offsets, tokens, their
+// probabilities, rows, the border) is what small calls wait for: seven requests at 32000 take 6.2 us; 200 at 131072, two rows of bf16
+// for two thirds of them, 29.0 us, 3.1 TB/s, in fp32 37.9.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kVerifyThreads, 3) verify_drafts_kernel(const __grid_constant__ VerifyParams p) {
+    __shared__ VerifyShared sh;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int blocks = (int)cluster.num_blocks(), b = blockIdx.x / blocks, rank = blockIdx.x % blocks;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int c0 = min(max(p.cu[b], 0), p.n_tokens), c1 = min(max(p.cu[b + 1], c0), p.n_tokens);
+    const int drafts = min(c1 - c0, p.most);
+    const T* target = static_cast<const T*>(p.target) + (long long)(c0 + b) * p.vocab;
+    const T* draft = static_cast<const T*>(p.draft) + (p.draft == nullptr ? 0 : (long long)c0 * p.vocab);
+    if (threadIdx.x == 0) sh.refused = drafts;
+    __syncthreads();
+    for (int i = threadIdx.x; i < drafts; i += kVerifyThreads) {
+        const long long x = p.tokens[c0 + i];
+        bool good = false;
+        if (x >= 0 && x < p.vocab) {
+            const double q = p.draft == nullptr ? 1.0 : (double)not_negative(as_float(draft[(long long)i * p.vocab + x]));
+            good = (double)p.u[c0 + b + i] * q < (double)as_float(target[(long long)i * p.vocab + x]);
+        }
+        if (!good) atomicMin(&sh.refused, i);
+    }
+    __syncthreads();
+    const int kept = sh.refused;
+    const bool refused = kept < drafts;
+    const int segments = (p.vocab + kSegment - 1) / kSegment;
+    const int share = (segments + blocks * kVerifyWarps - 1) / (blocks * kVerifyWarps);  // of a warp
+    const int seg0 = min((rank * kVerifyWarps + warp) * share, segments), seg1 = min(seg0 + share, segments);
+    bool residual = refused;
+    Weights<T, VEC> weights = weights_of<T, VEC>(p, b, c0, kept, refused);
+    constexpr int AHEAD = (VEC ? 8 : 4) / sizeof(T);  // segments whose reads are under way at once
+    double total = 0, before = 0;  // of all blocks, of those before this one
+    int last = -1;
+    while (true) {
+        if (threadIdx.x == 0) sh.last = -1;
+        __syncthreads();
+        int mine = -1;
+        double sum = 0;
+        for (int s = seg0; s < seg1; s += AHEAD) {
+            Raw8<T, VEC> a[AHEAD], c[AHEAD];
+#pragma unroll
+            for (int k = 0; k < AHEAD; ++k) weights.read(s + k < seg1 ? (s + k) * kSegment + lane * 8 : p.vocab, a[k], c[k]);
+#pragma unroll
+            for (int k = 0; k < AHEAD; ++k) {
+                float x[8], q[8];
+                const int at = (s + k) * kSegment + lane * 8;
+                weights.unpack(a[k], c[k], at, x, q);
+                const double add = sum8(x, q);
+                sum += add;
+                if (add > 0) mine = at;
+            }
+        }
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
+        mine = __reduce_max_sync(~0u, mine);
+        if (lane == 0) {
+            sh.warp[warp] = sum;
+            if (mine >= 0) atomicMax(&sh.last, mine);
+        }
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            double t = 0;
+            for (int w = 0; w < kVerifyWarps; ++w) t += sh.warp[w];
+            sh.total = t;
+        }
+        cluster.sync();
+        total = before = 0;
+        last = -1;
+        for (int r = 0; r < blocks; ++r) {
+            if (r == rank) before = total;
+            total += *cluster.map_shared_rank(&sh.total, r);
+            last = max(last, *cluster.map_shared_rank(&sh.last, r));
+        }
+        cluster.sync();  // nobody leaves or starts over while another block reads
+        if (total > 0 || !residual) break;
+        residual = weights.minus_draft = false, weights.hot = -1;  // a refused draft whose distribution covers the target's: the target's own row
+    }
+
+    const double aim = fmax((double)p.u[c1 + b] * total, 0.0);
+    if (rank == 0) {
+        for (int i = threadIdx.x; i <= p.most; i += kVerifyThreads)
+            if (i != kept) p.out[(long long)b * (p.most + 1) + i] = i < kept ? p.tokens[c0 + i] : -1;
+        if (threadIdx.x == 0) p.accepted[b] = kept;
+    }
+    long long* slot = p.out + (long long)b * (p.most + 1) + kept;
+    // The block whose part holds the aim; where u rounds to one the one with the last weight, and without any weight the first.
+    const bool beyond = !(aim < total);
+    const int per_block = share * kVerifyWarps * kSegment;
+    if (beyond ? rank != (last < 0 ? 0 : last / per_block) : !(before <= aim && aim < before + sh.total)) return;
+    if (beyond && last < 0) {
+        if (threadIdx.x == 0) *slot = 0;
+        return;
+    }
+    // ---- the warp's stretch, then the segment, then the entry
+    int stretch = last < 0 ? 0 : last / (share * kSegment);
+    double base = 0, near = -1;
+    if (!beyond) {
+        stretch = rank * kVerifyWarps, base = before;
+        for (int w = 0; w + 1 < kVerifyWarps && !(base + sh.warp[w] > aim); ++w) base += sh.warp[w], ++stretch;
+        if (aim > 0) near = near_border<T>(total);
+    }
+    search_stretch<false>(sh, weights, stretch * share, min((stretch + 1) * share, segments), base, aim, near);
+    if (!beyond && (sh.near != 0 || sh.hit == 0x7fffffff)) {
+        const float u = p.u[c1 + b];
+        __syncthreads();  // all have read
+        draw_in_64_bits<T, VEC>(&p, &sh, b, c0, kept, residual, u, blocks * kVerifyWarps);
+        return;
+    }
+    // Where u rounds to one, behind the last weight: that weight.
+    if (threadIdx.x == 0) *slot = !beyond ? sh.hit : sh.fall >= 0 ? sh.fall : last;
 }
 
 }  // namespace qb
@@ -607,7 +700,7 @@ template <typename T, bool VEC>
 static int launch_verify(const VerifyParams& p, cudaStream_t stream) {
     // As many blocks per request as are at work at once (three per SM), eight at most: with more, the same chain of reads is waited
     // for in several rounds (64 requests at a vocabulary of 32000: 13.3 us with eight, 9.2 with four).
-    int cluster = 8;
+    int cluster = kMostCluster;
     while (cluster > 1 && (long long)p.batch * cluster > 3 * 148) cluster /= 2;
     const cudaError_t e = launch_kernel_cluster(false, cluster, verify_drafts_kernel<T, VEC>, (long long)p.batch * cluster, kVerifyThreads, 0, stream, p);
     const int st = launch_status();

@@ -659,3 +659,41 @@ def test_verify_drafts_with_probabilities_that_are_none(vocab, dtype):
     q = torch.tensor([[0.5, -4.0, 0.5, 0.0]]).to(dtype).cuda()
     got, kept = quest.verify_drafts(p, torch.tensor([1], device="cuda"), i32([0, 1]), torch.tensor([0.5, 0.0], device="cuda"), 1, draft_probs=q)
     assert kept.tolist() == [0] and got.tolist() == [[3, -1]]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("kind", ["whole", "half", "tiny", "peak", "large"])
+@pytest.mark.parametrize("vocab, batch", [(40, 200), (138, 200), (5003, 100), (131072, 24)])
+def test_verify_drafts_next_to_the_borders(vocab, batch, kind, dtype):
+    """Uniforms that fall as near to a border between two tokens as fp32 can: the token is that of the sums in 64 bits, whatever is left
+    of a row (a millionth of it, or weights that are no probabilities) and however far apart the sizes of its weights are."""
+    g = torch.Generator().manual_seed(vocab + len(kind))
+    logits = 1.5 * torch.randn(batch, vocab, generator=g, dtype=torch.float64)
+    p = torch.softmax(logits, -1)
+    noise = torch.randn(batch, vocab, generator=g, dtype=torch.float64)
+    q = torch.softmax(logits + {"tiny": 1e-6 if dtype is torch.float32 else 1e-4}.get(kind, 0.7) * noise, -1)
+    if kind == "peak":
+        at = torch.randint(0, vocab, (batch, 1), generator=g)
+        p, q = (0.4 * p).scatter(1, at, 0.6), q.scatter(1, at, 1.3e-6)
+    p, q = (p * (1000 if kind == "large" else 1)).to(dtype), (q * (1000 if kind == "large" else 1)).to(dtype)
+    counts = [0 if kind == "whole" else 1] * batch
+    target = p if kind == "whole" else torch.stack([p, p], 1).flatten(0, 1)
+    draft = None if kind == "whole" else q
+    tokens = torch.empty(0, dtype=torch.int64) if draft is None else (q.double() / p.double().clamp(min=1e-300)).argmax(1)
+    cu = [sum(counts[:b]) for b in range(batch + 1)]
+    u = torch.zeros(target.size(0))
+    for b in range(batch):
+        w = p[b].double() if draft is None else (p[b].double() - q[b].double()).clamp(min=0)
+        if w.sum() == 0:  # (all refused drafts of a small vocabulary in bf16: the same rows)
+            w = p[b].double()
+        sums = w.cumsum(0)
+        border = sums[torch.randint(0, vocab, (1,), generator=g).item()] / sums[-1]
+        u[cu[b] + b + counts[b]] = border.float().clamp(max=1 - 2.0 ** -24)
+        if counts[b]:
+            u[cu[b] + b] = 1 - 2.0 ** -24  # refuses where q is more than p
+    want, accepted = ref.verify(target, draft, tokens.tolist(), cu, u, 1)
+    got, kept = quest.verify_drafts(target.cuda(), tokens.cuda(), i32(cu), u.cuda(), 1, draft_probs=None if draft is None else draft.cuda())
+    assert kept.tolist() == accepted
+    assert got.tolist() == want, [(b, x, y) for b, (x, y) in enumerate(zip(got.tolist(), want)) if x != y][:5]
+    if kind != "tiny":
+        assert sum(accepted) < batch // 8 + 1
