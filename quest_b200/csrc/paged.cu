@@ -341,14 +341,14 @@ __device__ __forceinline__ uint64_t sub_pair(uint64_t a, uint64_t b) {  // one r
 }
 
 // Sum of eight weights max(p - q, 0).  It decides between tokens, so it has to be as good as one in 64 bits, but 64-bit arithmetic
-// per entry cost more than reading it: with m = max(p, q) the difference m - q is split into h, its nearest multiple of 2^-16, whose sums
-// are exact in fp32, and the rest (m - h) - q, below 2^-17, whose sums lose less than 2^-38; two conversions for eight entries.  (m - h is
-// exact: both are multiples of m's last place, and h is no larger than m or, by less than that, the next multiple.  So what rounding the
-// difference itself would lose, next to a q of 2^-17 of p and less, is in the rest.)  What rests lose in all is far less than what u can
+// per entry cost more than reading it: with m = max(p, q) the difference m - q is split into h, its nearest multiple of 2^-22, whose sums
+// are exact in fp32 up to 4, and the rest (m - h) - q, below 2^-23, whose sums lose less than 2^-44; two conversions for eight entries.  (m - h
+// is exact: both are multiples of m's last place, and h is no larger than m or, by less than that, the next multiple.  So what rounding the
+// difference itself would lose, next to a much smaller q, is in the rest.)  What rests lose in all is far less than what u can
 // tell apart; where the aim is as near to a border as that, the decision is made in 64 bits (near_border).
 __device__ __forceinline__ double sum8(const float (&p)[8], const float (&q)[8]) {
     uint64_t high = 0, low = 0;
-    const uint64_t magic = pair_of(192.f, 192.f);
+    const uint64_t magic = pair_of(3.f, 3.f);
 #pragma unroll
     for (int j = 0; j < 8; j += 2) {
         const uint64_t m2 = pair_of(fmaxf(p[j], q[j]), fmaxf(p[j + 1], q[j + 1])), q2 = pair_of(q[j], q[j + 1]);  // a NaN of p counts as nothing
@@ -360,14 +360,14 @@ __device__ __forceinline__ double sum8(const float (&p)[8], const float (&q)[8])
     return (double)(a + b) + (double)(c + d);
 }
 
-// How far from a border the sums of sum8 may be off.  A group's rests add up to at most 2^-14, or to the row's total where that is less, and
-// lose some 2^-25 of it in either direction: over the groups of a row about 2^-25 times the root of that times the total.  Eight times as
-// much is taken for near, a whole one for bf16, whose eight bits mostly leave nothing to lose (emulated on the host over rows of all kinds the sums
-// are off by at most 0.15 and 0.26 of it), and all that 24 bits can lose for weights that are no probabilities.
-template <typename T>
+// How far from a border the sums of sum8 may be off.  A group's rests add up to at most 2^-20, or to the row's total where that is less, and
+// lose some 2^-25 of it in either direction: over the groups of a row about 2^-25 times the root of that times the total.  (Emulated on the
+// host over 70000 rows of all kinds: at most 2^-26.9 times that root where the total is above 2^-14, 2^-23.6 below.)  Weights that are no
+// probabilities may lose all that 24 bits can.  So 200 numbers at a vocabulary of 131072 come near a border in one call of 300, which then
+// takes some 45 us more.
 __device__ __forceinline__ double near_border(double total) {
     const float t = (float)total;
-    return t > 64.f ? t * 0x1p-21f : sqrtf(fminf(t, 0x1p-14f)) * sqrtf(t) * (sizeof(T) == 4 ? 0x1p-22f : 0x1p-25f);
+    return t > 2.f ? t * 0x1p-21f : t < 0x1p-14f ? t * 0x1p-22f : sqrtf(t) * 0x1p-34f;
 }
 
 // The difference of a target's row and a draft's (or nothing, or all on the token `hot`), as verify_drafts_kernel reads it.
@@ -479,7 +479,7 @@ __device__ __noinline__ void draw_in_64_bits(const VerifyParams* params, VerifyS
     const VerifyParams& p = *params;
     const Weights<T, VEC> weights = weights_of<T, VEC>(p, b, c0, kept, residual);
     const int lane = threadIdx.x & 31, segments = (p.vocab + kSegment - 1) / kSegment, share = (segments + stretches - 1) / stretches;
-    constexpr int AHEAD = 4 / sizeof(T);
+    constexpr int AHEAD = (VEC ? 8 : 4) / sizeof(T);
     for (int i = threadIdx.x >> 5; i < stretches; i += kVerifyWarps) {
         const int end = min((i + 1) * share, segments);
         double sum = 0;
@@ -614,7 +614,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 3) verify_drafts_kernel(const 
     if (!beyond) {
         stretch = rank * kVerifyWarps, base = before;
         for (int w = 0; w + 1 < kVerifyWarps && !(base + sh.warp[w] > aim); ++w) base += sh.warp[w], ++stretch;
-        if (aim > 0) near = near_border<T>(total);
+        if (aim > 0) near = near_border(total);
     }
     search_stretch<false>(sh, weights, stretch * share, min((stretch + 1) * share, segments), base, aim, near);
     if (!beyond && (sh.near != 0 || sh.hit == 0x7fffffff)) {
