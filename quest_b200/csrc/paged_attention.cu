@@ -23,7 +23,7 @@
 //
 // Measured in a graph (copy 6.55 TB/s, matrix product 1655 TFLOP/s, 1408 sustained; heads of 128; a range ends with what the power
 // limit leaves when the calls go on for long):
-//   64 requests of up to 16384 tokens (137000 in all), 64 / 8 heads, one new token   102 - 112 us, 5.0 - 5.5 TB/s; of that 9 us until
+//   64 requests of up to 16384 tokens (137000 in all), 64 / 8 heads, one new token   100 - 112 us, 5.0 - 5.6 TB/s; of that 9 us until
 //                                                the first product, 85 - 90 at the rate of HBM, 6 for the join
 //   one request of 1001 tokens, 16 / 16 heads, one new token    13 us, nearly all of it the chain of latencies
 //   one request of 32768 tokens, 64 / 8 heads, one new token    38 us, 3.5 TB/s
@@ -31,7 +31,7 @@
 //   128 requests of at most 1000 tokens, 32 / 32 heads          116 - 130 us, 3.9 - 4.3 TB/s
 //   16 prompts of 1024, 16 / 16 heads                           107 - 120 us; tensor pipe and exponentials a third each
 //   4 prompts of 4096, 32 / 8 heads                             471 - 535 us, 1167 - 1028 TFLOP/s; head_dim 64 410 us
-//   a chunk of 4096 behind 28672 tokens, among 15 single tokens, 64 / 8 heads    3.10 - 3.68 ms, 1330 - 1120 TFLOP/s
+//   a chunk of 4096 behind 28672 tokens, among 15 single tokens, 64 / 8 heads    3.10 - 3.88 ms, 1330 - 1060 TFLOP/s
 // A step of 128 rows by 128 keys costs the tensor core 2 x 8 products of 64 cycles and its warps 128 exponentials per thread, 16 a
 // cycle and SM: 1024 cycles each.  A stream's steps form a chain, 1900 cycles of softmax and 1330 of products and their hand-over; two
 // streams keep the tensor core busy two thirds of that.
